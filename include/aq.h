@@ -43,6 +43,9 @@ extern "C" {
 #define AQ_TYPE_Q4_K 12
 #define AQ_TYPE_Q5_K 13
 #define AQ_TYPE_Q6_K 14
+/* The 16-bit row and cache types of the rotary and paged-attention operators (ggml.h's ids); not weight types. */
+#define AQ_TYPE_F16 1
+#define AQ_TYPE_BF16 30
 
 /* ---------------------------------------------------------------------------------- shared plain types */
 
@@ -216,6 +219,98 @@ int aq_sampler_write_dense(aq_sampler *sp, float *dense_dev);
  * norm(max(0, p - q)); q_dev is the dense draft distribution (vocab f32). Greedy: accepted iff d is the argmax. */
 int aq_sampler_accept_or_resample(aq_sampler *sp, const float *target_dev, const float *q_dev, uint32_t d,
                                   int *accepted, uint32_t *tok);
+
+/* ------------------------------------------------------------------- rotary positions, paged attention */
+
+/* Attention for batches of sequences whose K/V rows live in pages, from the operator level: rotate, append, attend.
+ * The reference serves one sequence over one run of f32 rows (gqa_attention.rs:327-418, rope.rs:10-45); these calls do
+ * the same mathematics over pages, many sequences at once, in f32, f16 or bf16, and are not bit-exact restatements of
+ * it. All are queued on the caller's `stream` (a hipStream_t of the context's device; NULL: the context's own) without
+ * synchronising or allocating, and may be captured into a graph. The same call on the same data gives the same bits;
+ * the order of a row's sums follows the batch it is computed in.
+ *
+ * Offsets are 64-bit; data, strides and device arrays are checked as far as the host can see them. What only the device
+ * sees is bounded there: rows at or past n_rows are never touched, a page outside 0..n_pages-1 or a position past the
+ * table is a hole (nothing is stored there, nothing attended), a length below 0 counts as 0. */
+
+/* [rows][heads][head_dim] values on the device, type F32, F16 or BF16; strides in elements, head_dim contiguous. */
+typedef struct aq_heads {
+    void *data;
+    int32_t type;
+    int64_t row_stride, head_stride;
+} aq_heads;
+
+#define AQ_ROPE_HALF 0        /* pairs (i, i + dim / 2), as rope.rs:31-45 */
+#define AQ_ROPE_INTERLEAVED 1 /* pairs (2i, 2i + 1) */
+#define AQ_ROPE_PLAIN 0
+#define AQ_ROPE_LINEAR 1 /* positions divided by factor */
+#define AQ_ROPE_YARN 2   /* pairs that turn often over orig_ctx positions keep their frequency, slow ones are divided by
+                          * factor, a linear ramp between; the result times attn_factor */
+typedef struct aq_rope_config {
+    uint32_t dim;    /* rotated values of a head, even; the rest of the head passes through */
+    uint32_t layout; /* AQ_ROPE_HALF / AQ_ROPE_INTERLEAVED */
+    float theta;     /* pair i turns by theta^(-2i/dim) a position */
+    uint32_t scaling;
+    float factor;        /* LINEAR, YARN: > 0 */
+    uint32_t orig_ctx;   /* YARN: the trained length */
+    float beta_fast, beta_slow; /* YARN: turns over orig_ctx at which the ramp begins and ends (0: 32 and 1) */
+    float attn_factor;   /* YARN: multiplies cos and sin (0: 1 + 0.1 ln factor, or 1 for a factor below 1) */
+} aq_rope_config;
+
+/* The rotation's frequencies on the device (`RopeTable`-like state of rope.rs:10-28, without its position limit:
+ * angles are computed in 64 bits for any 32-bit position). Usable from any stream of the context's device. */
+typedef struct aq_rope aq_rope;
+int aq_rope_new(aq_ctx *ctx, const aq_rope_config *cfg, aq_rope **out);
+int aq_rope_free(aq_rope *r);
+/* y[r][h] = x[r][h] rotated by pos_dev[r] (`rope_apply`, rope.rs:31-45); inverse != 0 rotates back (times the same
+ * attn_factor): the gradient of the rotation, and cached keys moved to other positions. y may be x (same strides), and
+ * else must not overlap it. Same type on both sides. */
+int aq_rope_apply(const aq_rope *r, const aq_heads *x, const aq_heads *y, size_t n_rows, size_t n_heads, size_t head_dim,
+                  const int32_t *pos_dev, int inverse, void *stream);
+
+/* A pool of K/V pages on the device: the row of (page, slot, head) starts page * page_stride + slot * slot_stride +
+ * head * head_stride elements into k and into v. Type F32, F16 or BF16; head_dim a multiple of 8, at most 256; k, v
+ * and the strides in bytes multiples of 16. */
+typedef struct aq_paged_kv {
+    int32_t type;
+    uint32_t n_pages, page_size, n_head_kv, head_dim;
+    void *k, *v;
+    int64_t page_stride, slot_stride, head_stride;
+} aq_paged_kv;
+
+/* New rows of n_seq sequences: sequence s has rows row_start[s] .. row_start[s+1]-1 (row_start: n_seq + 1 values, never
+ * falling; a sequence may have none) and kv_len[s] positions with them, so its row i stands at position
+ * kv_len[s] - (its rows) + i; its position p lies in page pages[s * max_pages + p / page_size]. All three arrays on the
+ * device. n_rows: rows of the row tensors (those past row_start[n_seq] are left as they are); max_rows: the most rows a
+ * sequence has (an attention may leave rows past it unwritten); max_len: no kv_len is larger (an attention takes
+ * positions from max_len on as holes). Bounds, not exact: a captured call keeps them as the arrays' contents change. */
+typedef struct aq_paged_batch {
+    uint32_t n_seq, max_pages;
+    const int32_t *row_start, *kv_len, *pages;
+    uint32_t n_rows, max_rows, max_len;
+} aq_paged_batch;
+
+/* The new rows' k and v into their pages, rounded to the cache's type: the append of gqa_attention.rs:327-418 over
+ * pages. With a rope, k is rotated by its position on the way, and q (nullable; n_head heads) into q_out (q itself, or
+ * not overlapping it); without one q must be NULL. k, v and q have one type: F32, or the cache's. A row whose position
+ * is negative or has no page stores nothing; its q is rotated all the same. */
+int aq_paged_append(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, const aq_heads *k,
+                    const aq_heads *v, const aq_rope *rope, const aq_heads *q, const aq_heads *q_out, uint32_t n_head,
+                    void *stream);
+
+/* out[r][h] = sum_j softmax_j(scale * q[r][h] . K[j][h / (n_head / n_head_kv)]) V[j][...] over the positions j up to
+ * the row's own (with window > 0: the last `window` of them), times sigmoid(gate[r][h]) when gate is given (nullable):
+ * the attention core of gqa_attention.rs:327-418 over pages. A row that sees nothing is 0. What a row does not see
+ * never reaches it, infinities and NaN included. q, gate and out have one type: F32, or the cache's; F32 rows over a
+ * 16-bit cache keep 32-bit accuracy (queries and probabilities go through the matrix cores in pieces). out may be q or
+ * gate (same strides), and else must not overlap what the call reads. scale > 0.
+ * workspace: aq_paged_attention_workspace bytes of device memory for these arguments, 16-byte aligned, contents
+ * irrelevant before and after; calls (and captured graphs) that can run at the same time need one each. */
+int aq_paged_attention_workspace(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, uint32_t n_head,
+                                 size_t *bytes);
+int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, uint32_t n_head,
+                       const aq_heads *q, const aq_heads *out, float scale, uint32_t window, const aq_heads *gate,
+                       void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------ synthetic tensors */
 

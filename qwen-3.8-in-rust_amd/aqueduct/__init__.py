@@ -13,6 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libaq.so")
 
 F32, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K = 0, 2, 8, 12, 13, 14
+F16, BF16 = 1, 30  # row and cache types of the rotary and paged-attention operators
 BLOCK = {F32: (1, 4), Q4_0: (32, 18), Q8_0: (32, 34), Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210)}
 
 
@@ -161,6 +162,12 @@ def lib():
                                           P, P]),
         "aq_deltanet_verify_commit_dev": (i, [P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, sz, sz, P, P, P, P,
                                               P, P, P]),
+        "aq_rope_new": (i, [P, P, C.POINTER(P)]),
+        "aq_rope_free": (i, [P]),
+        "aq_rope_apply": (i, [P, P, P, sz, sz, sz, P, i, P]),
+        "aq_paged_append": (i, [P, P, P, P, P, P, P, P, C.c_uint32, P]),
+        "aq_paged_attention_workspace": (i, [P, P, P, C.c_uint32, C.POINTER(sz)]),
+        "aq_paged_attention": (i, [P, P, P, C.c_uint32, P, P, C.c_float, C.c_uint32, P, P, sz, P]),
     }
     for name, (res, args) in sigs.items():
         f = getattr(L, name)
@@ -701,6 +708,116 @@ def eval_math(ctx: Context, fn, x):
     y = np.zeros_like(x)
     check(lib().aq_eval_math(ctx.h, fn, ptr(x), ptr(y), x.size))
     return y
+
+
+# ------------------------------------------------------------------------- rotary positions, paged attention
+class AqHeads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int32), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class AqRopeConfig(C.Structure):
+    _fields_ = [("dim", C.c_uint32), ("layout", C.c_uint32), ("theta", C.c_float), ("scaling", C.c_uint32),
+                ("factor", C.c_float), ("orig_ctx", C.c_uint32), ("beta_fast", C.c_float), ("beta_slow", C.c_float),
+                ("attn_factor", C.c_float)]
+
+
+class AqPagedKv(C.Structure):
+    _fields_ = [("type", C.c_int32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_head_kv", C.c_uint32),
+                ("head_dim", C.c_uint32), ("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64),
+                ("slot_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class AqPagedBatch(C.Structure):
+    _fields_ = [("n_seq", C.c_uint32), ("max_pages", C.c_uint32), ("row_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("pages", C.c_void_p), ("n_rows", C.c_uint32), ("max_rows", C.c_uint32), ("max_len", C.c_uint32)]
+
+
+def dev_ptr(x):
+    """A device address: a DeviceBuffer's, or an integer (a tensor's data_ptr())."""
+    return x.p.value if isinstance(x, DeviceBuffer) else x
+
+
+def heads(data, type, row_stride, head_stride):
+    """aq_heads: [rows][heads][head_dim] values at a device address (or DeviceBuffer), strides in elements."""
+    h = AqHeads(dev_ptr(data), type, row_stride, head_stride)
+    h.keep = data
+    return h
+
+
+def paged_kv(k, v, type, n_pages, page_size, n_head_kv, head_dim, page_stride=None, slot_stride=None, head_stride=None):
+    """aq_paged_kv: a pool of K/V pages; strides default to [page][slot][head][head_dim] without gaps."""
+    head_stride = head_dim if head_stride is None else head_stride
+    slot_stride = n_head_kv * head_dim if slot_stride is None else slot_stride
+    page_stride = page_size * slot_stride if page_stride is None else page_stride
+    kv = AqPagedKv(type, n_pages, page_size, n_head_kv, head_dim, dev_ptr(k), dev_ptr(v), page_stride, slot_stride,
+                   head_stride)
+    kv.keep = (k, v)
+    return kv
+
+
+def paged_batch(n_seq, row_start, kv_len, pages, max_pages, n_rows, max_rows, max_len):
+    """aq_paged_batch: the new rows of n_seq sequences (device int32 arrays)."""
+    b = AqPagedBatch(n_seq, max_pages, dev_ptr(row_start), dev_ptr(kv_len), dev_ptr(pages), n_rows, max_rows, max_len)
+    b.keep = (row_start, kv_len, pages)
+    return b
+
+
+class Rope:
+    """aq_rope: a rotation's frequencies on the device (rope.rs:10-28); layout "half" or "interleaved", scaling "none",
+    "linear" or "yarn"."""
+    LAYOUTS = {"half": 0, "interleaved": 1}
+    SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
+
+    def __init__(self, ctx: Context, dim, theta=10000.0, layout="half", scaling="none", factor=1.0, orig_ctx=0,
+                 beta_fast=0.0, beta_slow=0.0, attn_factor=0.0):
+        self.ctx, self.dim = ctx, dim
+        if layout not in self.LAYOUTS or scaling not in self.SCALINGS:
+            raise AqError(f"rope: layout {layout!r}, scaling {scaling!r}", AQ_EINVAL)
+        cfg = AqRopeConfig(dim, self.LAYOUTS[layout], theta, self.SCALINGS[scaling], factor, orig_ctx, beta_fast,
+                           beta_slow, attn_factor)
+        h = C.c_void_p()
+        check(lib().aq_rope_new(ctx.h, C.byref(cfg), C.byref(h)))
+        self.h = h
+
+    def free(self):
+        if getattr(self, "h", None):
+            lib().aq_rope_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.free()
+
+
+def _ref(struct):
+    return None if struct is None else C.byref(struct)
+
+
+def rope_apply(rope: Rope, x, y, n_rows, n_heads, head_dim, pos, inverse=False, stream=None):
+    """y = x rotated by pos (aq_rope_apply), queued on `stream` (an integer hipStream_t; None: the context's own)."""
+    check(lib().aq_rope_apply(rope.h, _ref(x), _ref(y), n_rows, n_heads, head_dim, dev_ptr(pos), 1 if inverse else 0,
+                              stream))
+
+
+def paged_append(ctx: Context, kv, batch, k, v, rope=None, q=None, q_out=None, n_head=0, stream=None):
+    """New k, v rows into their pages, k (and q into q_out) rotated on the way (aq_paged_append), queued."""
+    check(lib().aq_paged_append(ctx.h, _ref(kv), _ref(batch), _ref(k), _ref(v), None if rope is None else rope.h,
+                                _ref(q), _ref(q_out), n_head, stream))
+
+
+def paged_attention_workspace(ctx: Context, kv, batch, n_head):
+    """Bytes of device memory that paged_attention needs for these arguments (aq_paged_attention_workspace)."""
+    n = C.c_size_t()
+    check(lib().aq_paged_attention_workspace(ctx.h, C.byref(kv), C.byref(batch), n_head, C.byref(n)))
+    return n.value
+
+
+def paged_attention(ctx: Context, kv, batch, n_head, q, out, scale, window=0, gate=None, workspace=None,
+                    workspace_bytes=None, stream=None):
+    """The new rows' attention over their pages (aq_paged_attention), queued."""
+    if workspace_bytes is None:
+        workspace_bytes = workspace.nbytes if isinstance(workspace, DeviceBuffer) else 0
+    check(lib().aq_paged_attention(ctx.h, _ref(kv), _ref(batch), n_head, _ref(q), _ref(out), scale, window, _ref(gate),
+                                   dev_ptr(workspace), workspace_bytes, stream))
 
 
 # ------------------------------------------------------------------------------------------------ GGUF files

@@ -1,0 +1,115 @@
+// paged.h — the paged K/V cache and the batch over it as the kernels see them, and the host checks the paged entry
+// points share (rope.hip: rotation and append; paged_attention.hip: attention).
+#pragma once
+
+#include "aq_common.h"
+
+namespace aq {
+
+// n / d and n % d for positions (n < 2^31): pages of a power of two by shifting, others by a 32-bit reciprocal:
+// m = ceil(2^(31 + k) / d) with 2^(k-1) < d <= 2^k exceeds 2^(31+k) / d by less than 1, so floor(n m / 2^(31+k)) is
+// exact for n < 2^31.
+struct FastDiv {
+    uint32_t d = 1, mul = 0, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div) {
+        uint32_t k = 0;
+        while ((1ull << k) < div) k++;
+        if ((1ull << k) == div) {
+            shift = k; // mul 0: a shift
+        } else {
+            mul = (uint32_t)(((1ull << (31 + k)) + div - 1) / div);
+            shift = k - 1;
+        }
+    }
+    __host__ __device__ uint32_t quot(uint32_t n) const {
+        return mul ? (uint32_t)(((uint64_t)n * mul) >> 32) >> shift : n >> shift;
+    }
+};
+
+// The cache: K and V rows at base + ((page * page_units + slot * slot_units) << unit_shift) bytes, then the head.
+// Offsets are counted in the largest power of two of bytes that divides both strides, so that 32 bits of it reach any
+// pool a device can hold.
+struct PagedKv {
+    const char *k = nullptr, *v = nullptr;
+    uint32_t n_pages = 0, page_units = 0, slot_units = 0, unit_shift = 0, head_bytes = 0;
+    FastDiv page_size;
+    int nkv = 0, hd = 0, type = 0;
+};
+
+struct PagedBatch {
+    const int32_t *row_start = nullptr, *kv_len = nullptr, *pages = nullptr;
+    uint32_t n_seq = 0, max_pages = 0, n_rows = 0;
+};
+
+// [rows][heads][head_dim] values with strides, in elements.
+struct HeadsView {
+    char *p = nullptr;
+    int64_t row = 0, head = 0;
+    int type = 0;
+};
+
+inline size_t type_bytes(int t) { return t == AQ_TYPE_F32 ? 4 : 2; }
+inline bool row_type(int t) { return t == AQ_TYPE_F32 || t == AQ_TYPE_F16 || t == AQ_TYPE_BF16; }
+
+// The host checks; each names the call in its message.
+int check_heads(const char *call, const char *what, const aq_heads *h, size_t n_rows, size_t n_heads, size_t head_dim);
+int check_paged(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, PagedKv *out, PagedBatch *bout);
+inline HeadsView heads_view(const aq_heads *h) {
+    HeadsView v;
+    v.p = (char *)h->data;
+    v.row = h->row_stride;
+    v.head = h->head_stride;
+    v.type = h->type;
+    return v;
+}
+// Whether every row of the view can be read and written 16 bytes at a time.
+bool heads_aligned(const aq_heads *h, size_t n_rows, size_t n_heads);
+
+// ------------------------------------------------------------------------------------------------ device side
+template <int T> struct RowType;
+template <> struct RowType<AQ_TYPE_F32> { using type = float; };
+template <> struct RowType<AQ_TYPE_F16> { using type = _Float16; };
+template <> struct RowType<AQ_TYPE_BF16> { using type = __bf16; };
+
+// Byte offset (in units) of a position's K / V row and whether it has one: a position past the table or on a page
+// outside 0..n_pages-1 has none.
+__device__ __forceinline__ bool paged_slot(const PagedKv &c, const int32_t *table, uint32_t max_pages, uint32_t pos,
+                                           uint32_t *units) {
+    const uint32_t col = c.page_size.quot(pos), slot = pos - col * c.page_size.d;
+    const uint32_t page = col < max_pages ? (uint32_t)table[col] : 0xFFFFFFFFu;
+    const bool ok = page < c.n_pages;
+    *units = ok ? page * c.page_units + slot * c.slot_units : 0u;
+    return ok;
+}
+
+// The sequence that row `row` belongs to (n_seq: none): the number of sequences that end at or before it, counted by
+// the whole wave.
+__device__ __forceinline__ uint32_t paged_seq_of(const PagedBatch &b, uint32_t row) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t seq = 0;
+    for (uint32_t s0 = 0; s0 < b.n_seq; s0 += 64) {
+        const uint32_t s = s0 + lane;
+        const bool before = s < b.n_seq && b.row_start[s + 1] <= (int32_t)row;
+        const uint32_t n = (uint32_t)__popcll(__ballot(before));
+        seq += n;
+        if (n < 64) break;
+    }
+    return seq;
+}
+
+// A sequence's rows within the batch's n_rows, whatever row_start holds, and its length.
+struct SeqRows {
+    int32_t first, n, len;
+};
+__device__ __forceinline__ SeqRows paged_seq(const PagedBatch &b, uint32_t s) {
+    const int32_t lo = b.row_start[s], hi = b.row_start[s + 1], len = b.kv_len[s];
+    SeqRows r;
+    r.first = lo < 0 ? 0 : lo;
+    const int32_t end = hi < (int32_t)b.n_rows ? hi : (int32_t)b.n_rows;
+    r.n = end > r.first ? end - r.first : 0;
+    r.len = len > 0 ? len : 0;
+    return r;
+}
+
+} // namespace aq
