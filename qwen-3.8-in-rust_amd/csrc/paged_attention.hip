@@ -1,5 +1,6 @@
 // paged_attention.hip — attention over a paged K/V cache (aq_paged_attention): the choice of kernel, the kernel for few
-// rows (single tokens, verify batches, and f32 rows of any number), the plan and the join of split sequences.
+// rows (single tokens, verify batches, and f32 rows of any number), the plan and the join of split sequences. Many
+// 16-bit rows take paged_chunk.hip.
 //
 // The kernel for few rows. Single tokens are bound by reading the cache: a wave takes 32 positions at a time straight
 // from the pages into registers, in the matrix cores' operand layout, with no LDS on the way:
@@ -57,71 +58,10 @@ __device__ __forceinline__ void pieces(const float *v, u4 *out) { // 8 values ->
     }
 }
 
-// Bits 15 and 31 of the result: the low and high 16-bit value of w is an infinity or a NaN (its exponent plus one carries).
-template <int CT>
-__device__ __forceinline__ unsigned odd_bits(unsigned w) {
-    return (w & 0x7FFF7FFFu) + (CT == AQ_TYPE_F16 ? 0x04000400u : 0x00800080u);
-}
-// All bits of such a value, none of others.
-template <int CT>
-__device__ __forceinline__ unsigned odd_mask(unsigned w) {
-    return ((odd_bits<CT>(w) & 0x80008000u) >> 15) * 0xFFFFu;
-}
+// An infinity or a NaN.
 __device__ __forceinline__ bool odd_f32(unsigned w) { return (w & 0x7F800000u) == 0x7F800000u; }
 
-template <int QT>
-__device__ __forceinline__ float load_one(const char *p, int64_t i) {
-    return (float)reinterpret_cast<const typename RowType<QT>::type *>(p)[i];
-}
-
-// N consecutive values of a row as f32, of which `have` exist (the others 0).
-template <int QT, int N>
-__device__ __forceinline__ void load_row(const char *row, int at, int have, bool wide, float *v) {
-    using E = typename RowType<QT>::type;
-    if (at >= have) {
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = 0.0f;
-    } else if (wide) {
-        constexpr int C = 16 / (int)sizeof(E) < N ? 16 / (int)sizeof(E) : N;
-        typedef E vec __attribute__((ext_vector_type(C)));
-#pragma unroll
-        for (int i = 0; i < N / C; i++) {
-            const vec x = *reinterpret_cast<const vec *>(row + (size_t)(at + i * C) * sizeof(E));
-#pragma unroll
-            for (int j = 0; j < C; j++) v[i * C + j] = (float)x[j];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = load_one<QT>(row, at + i);
-    }
-}
-
-// Four outputs of a row: times the gate, rounded, stored.
-template <int QT>
-__device__ __forceinline__ void store_out(const AttnPagedArgs &a, int64_t row, int head, int dim, float *v) {
-    using E = typename RowType<QT>::type;
-    if (a.gate.p) {
-        const char *gp = a.gate.p + (row * a.gate.row + (int64_t)head * a.gate.head + dim) * (int64_t)sizeof(E);
-        float g[4];
-        load_row<QT, 4>(gp, 0, 4, a.out_wide, g);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] *= 1.0f / (1.0f + expf(-g[i]));
-    }
-    E *o = (E *)a.out.p + row * a.out.row + (int64_t)head * a.out.head + dim;
-    typedef E vec __attribute__((ext_vector_type(4)));
-    if (a.out_wide) {
-        vec x;
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = (E)v[i];
-        *reinterpret_cast<vec *>(o) = x;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = (E)v[i];
-    }
-}
-
 constexpr int WAVES = 4, TILE = 32, UNIT = WAVES * TILE; // positions of a wave's tile and of a work-group's step
-constexpr int INLINE_SEQS = 1024;                        // sequences that a work-group divides by itself
 
 // What the few-row kernel keeps where, for one cache type, row type and padded head size.
 template <int CT, bool FQ, int D, int NR>
@@ -155,84 +95,14 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
-    const uint32_t nkv = (uint32_t)a.kv.nkv;
     const int hd = a.kv.hd, G = a.G;
 
-    // ---- this work-group's share of the line of units
-    uint32_t total, chunk, n_seg;
-    if (a.planned) {
-        total = a.plan[0];
-        chunk = a.plan[1];
-        n_seg = a.plan[2];
-    } else {
-        n_seg = a.b.n_seq;
-        uint32_t mine[INLINE_SEQS / 256], sum = 0;
-#pragma unroll
-        for (int i = 0; i < INLINE_SEQS / 256; i++) {
-            const uint32_t s = (uint32_t)tid * (INLINE_SEQS / 256) + i;
-            mine[i] = 0;
-            if (s < n_seg) {
-                const SeqRows sr = paged_seq(a.b, s);
-                if (sr.n > 0) {
-                    const UnitRange u = tile_units(sr, G, a.window, a.cap, 0, R, UNIT);
-                    mine[i] = u.hi - u.lo;
-                }
-            }
-            sum += mine[i];
-        }
-        uint32_t scan = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t v = __shfl_up(scan, d);
-            if (lane >= d) scan += v;
-        }
-        if (lane == 63) wsum[wave] = scan;
-        __syncthreads();
-        uint32_t before = scan - sum;
-        for (int w = 0; w < wave; w++) before += wsum[w];
-        if (tid == 0) pre[0] = 0;
-#pragma unroll
-        for (int i = 0; i < INLINE_SEQS / 256; i++) {
-            before += mine[i];
-            pre[tid * (INLINE_SEQS / 256) + i + 1] = before;
-        }
-        __syncthreads();
-        total = pre[n_seg] * nkv;
-        chunk = share_chunk(total, a.shares, a.min_chunk);
-        if (blockIdx.x == 0) { // for the join
-            if (tid == 0) {
-                a.plan[0] = total;
-                a.plan[1] = chunk;
-                a.plan[2] = n_seg;
-            }
-            for (uint32_t s = tid; s <= n_seg; s += 256) a.plan[PLAN_HEAD + s] = pre[s];
-        }
-    }
-    // neighbouring shares on one XCD: work-groups go round the 8 XCDs, and neighbours read the same pages' lines
-    const uint32_t per = a.shares / 8, w = a.shares % 8 ? blockIdx.x : (blockIdx.x % 8) * per + blockIdx.x / 8;
-    const uint64_t first = (uint64_t)w * chunk;
-    if (first >= total) return; // uniform
-    uint32_t u = (uint32_t)first;
-    const uint32_t end = min(total, u + chunk);
-    auto prefix = [&](uint32_t j) { return a.planned ? a.plan[PLAN_HEAD + j] : pre[j]; };
-    // the row tile that unit u lies in: the only one that begins at or before it and ends after it
-    for (uint32_t j = tid; j < n_seg; j += 256)
-        if (prefix(j) * nkv <= u && u < prefix(j + 1) * nkv) found = j;
-    __syncthreads();
-    uint32_t j = found;
-
-    while (u < end) { // uniform
-        uint32_t p0 = prefix(j), p1 = prefix(j + 1);
-        while (p1 * nkv <= u) { // row tiles without units
-            j++;
-            p0 = p1;
-            p1 = prefix(j + 1);
-        }
-        const uint32_t cnt = p1 - p0, rel = u - p0 * nkv, kvh = rel / cnt, t0 = rel - kvh * cnt;
-        const uint32_t t1 = min(cnt, t0 + (end - u));
-        u += t1 - t0;
-        const uint32_t seq = a.planned ? a.seg_seq[j] : j;
-        const int32_t r0 = a.planned ? (int32_t)a.seg_rt[j] * R : 0;
+    const Share sh = take_share(a, R, UNIT, pre, wsum, &found);
+    uint32_t u = sh.begin, j = sh.j;
+    while (u < sh.end) { // uniform
+        const Segment sg = next_segment(a, R, pre, sh, u, j);
+        const uint32_t kvh = sg.kvh, seq = sg.seq, t0 = sg.t0, t1 = sg.t1;
+        const int32_t r0 = sg.r0;
         const SeqRows sr = paged_seq(a.b, seq);
         const int32_t n_rows = sr.n * G, base = sr.len - sr.n;
         const UnitRange range = tile_units(sr, G, a.window, a.cap, r0, R, UNIT);
@@ -665,8 +535,8 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             for (int x = 0; x < WAVES; x++) mx = fmaxf(mx, ml[(x * R + 16 * nr + r) * 2]);
             mine[nr] = fast_exp2(m[nr] - (mx == -INFINITY ? 0.0f : mx));
         }
-        const bool cut = t1 - t0 < cnt;
-        const uint32_t slot = 2 * w + (t0 == 0 ? 1 : 0);
+        const bool cut = t1 - t0 < sg.cnt;
+        const uint32_t slot = 2 * sh.w + (t0 == 0 ? 1 : 0);
 #pragma unroll
         for (int pass = 0; pass < S::PASSES; pass++) {
             if (pass) __syncthreads();
@@ -870,6 +740,7 @@ int compute_units(int device) {
 
 // Which kernel, its row tile and padded head size, and how its work is split.
 struct Choice {
+    bool many = false; // paged_chunk.hip
     int R = 16, D = 64;
     uint32_t unit = UNIT, shares = 0, min_chunk = 1, n_seg = 0, cap = 0;
     bool planned = false, join = false;
@@ -911,7 +782,11 @@ int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uin
     const uint64_t rows = (uint64_t)b->max_rows * G;
     c->D = kv->head_dim <= 64 ? 64 : kv->head_dim <= 128 ? 128 : 256;
     c->cap = (uint32_t)std::min<uint64_t>((uint64_t)b->max_pages * kv->page_size, b->max_len);
-    c->R = rows <= 16 ? 16 : 32;
+    // 16-bit rows past what one pass of the few-row kernel holds
+    c->many = !f32_rows && rows > 32;
+    c->R = c->many ? CHUNK_ROWS : rows <= 16 ? 16 : 32;
+    c->unit = c->many ? chunk_keys(c->D) : UNIT;
+    c->min_chunk = c->many ? 256 / c->unit : 1;
     c->planned = rows > (uint64_t)c->R || b->n_seq > INLINE_SEQS;
     // row tiles: a whole one per R rows of all sequences together, and one begun per sequence
     const uint64_t n_seg = c->planned ? ((uint64_t)b->n_rows * G) / c->R + b->n_seq : b->n_seq;
@@ -1028,7 +903,9 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
         rc = launch_paged_plan(a, c.R, c.unit, st);
         if (rc) return rc;
     }
-    if (q->type == AQ_TYPE_F32) {
+    if (c.many) {
+        rc = launch_paged_chunk(a, c.D, st);
+    } else if (q->type == AQ_TYPE_F32) {
         if (kv->type == AQ_TYPE_F32) rc = few_pick<AQ_TYPE_F32, true>(a, c.D, c.R, st);
         else if (kv->type == AQ_TYPE_F16) rc = few_pick<AQ_TYPE_F16, true>(a, c.D, c.R, st);
         else rc = few_pick<AQ_TYPE_BF16, true>(a, c.D, c.R, st);

@@ -1,5 +1,5 @@
-// paged_attn.h — what the paged attention kernels (paged_attention.hip) share: the division of the work, the partial
-// results, their argument block.
+// paged_attn.h — what the two paged attention kernels (paged_attention.hip: few rows, pages streamed through registers;
+// paged_chunk.hip: many rows, tiles in the LDS) share: the division of the work, the partial results, the outputs.
 //
 // Rows. The G = n_head / n_head_kv query heads that share a K/V head, times a sequence's new tokens, are its rows over
 // that head's keys: row = token * G + head in the group. A segment is one row tile (R rows) of one sequence on one K/V
@@ -64,6 +64,179 @@ __device__ __forceinline__ uint32_t share_chunk(uint32_t total, uint32_t shares,
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// x, of which the compiler knows nothing more: what is computed from it stays where it is used, instead of waiting in a
+// register from before a loop.
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+constexpr int INLINE_SEQS = 1024; // sequences that a work-group of 256 divides by itself
+
+// A work-group's share of the line: its number, its units begin .. end - 1 (none: begin == end), the row tile that
+// begin lies in. pre (INLINE_SEQS + 1), wsum (4) and found are the work-group's.
+struct Share {
+    uint32_t w, begin, end, n_seg, j;
+};
+__device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint32_t tk, uint32_t *pre, uint32_t *wsum,
+                                            uint32_t *found) {
+    constexpr int PER = INLINE_SEQS / 256;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t nkv = (uint32_t)a.kv.nkv;
+    uint32_t total, chunk;
+    Share sh;
+    if (a.planned) {
+        total = a.plan[0];
+        chunk = a.plan[1];
+        sh.n_seg = a.plan[2];
+    } else {
+        sh.n_seg = a.b.n_seq;
+        uint32_t mine[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const uint32_t s = (uint32_t)tid * PER + i;
+            mine[i] = 0;
+            if (s < sh.n_seg) {
+                const SeqRows sr = paged_seq(a.b, s);
+                if (sr.n > 0) {
+                    const UnitRange u = tile_units(sr, a.G, a.window, a.cap, 0, R, tk);
+                    mine[i] = u.hi - u.lo;
+                }
+            }
+            sum += mine[i];
+        }
+        uint32_t scan = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t v = __shfl_up(scan, d);
+            if (lane >= d) scan += v;
+        }
+        if (lane == 63) wsum[wave] = scan;
+        __syncthreads();
+        uint32_t before = scan - sum;
+        for (int w = 0; w < wave; w++) before += wsum[w];
+        if (tid == 0) pre[0] = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            before += mine[i];
+            pre[tid * PER + i + 1] = before;
+        }
+        __syncthreads();
+        total = pre[sh.n_seg] * nkv;
+        chunk = share_chunk(total, a.shares, a.min_chunk);
+        if (blockIdx.x == 0) { // for the join
+            if (tid == 0) {
+                a.plan[0] = total;
+                a.plan[1] = chunk;
+                a.plan[2] = sh.n_seg;
+            }
+            for (uint32_t s = tid; s <= sh.n_seg; s += 256) a.plan[PLAN_HEAD + s] = pre[s];
+        }
+    }
+    // neighbouring shares on one XCD: work-groups go round the 8 XCDs, and neighbours read the same pages' lines
+    sh.w = a.shares % 8 ? blockIdx.x : (blockIdx.x % 8) * (a.shares / 8) + blockIdx.x / 8;
+    const uint64_t first = (uint64_t)sh.w * chunk;
+    if (first >= total) {
+        sh.begin = sh.end = sh.j = 0;
+        return sh;
+    }
+    sh.begin = (uint32_t)first;
+    sh.end = min(total, sh.begin + chunk);
+    // the only row tile that begins at or before it and ends after it
+    for (uint32_t j = tid; j < sh.n_seg; j += 256) {
+        const uint32_t p0 = a.planned ? a.plan[PLAN_HEAD + j] : pre[j], p1 = a.planned ? a.plan[PLAN_HEAD + j + 1] : pre[j + 1];
+        if (p0 * nkv <= sh.begin && sh.begin < p1 * nkv) *found = j;
+    }
+    __syncthreads();
+    sh.j = *found;
+    return sh;
+}
+
+// The next segment of a share, from unit u on: K/V head, the sequence, its first row, the units t0 .. t1 - 1 of the
+// segment's cnt that are the share's. Advances u and j.
+struct Segment {
+    uint32_t kvh, seq, t0, t1, cnt;
+    int32_t r0;
+};
+__device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, const uint32_t *pre, const Share &sh,
+                                                uint32_t &u, uint32_t &j) {
+    const uint32_t nkv = (uint32_t)a.kv.nkv;
+    const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : pre;
+    uint32_t p0 = line[j], p1 = line[j + 1];
+    while (p1 * nkv <= u) { // row tiles without units
+        j++;
+        p0 = p1;
+        p1 = line[j + 1];
+    }
+    Segment s;
+    s.cnt = p1 - p0;
+    const uint32_t rel = u - p0 * nkv;
+    s.kvh = rel / s.cnt;
+    s.t0 = rel - s.kvh * s.cnt;
+    s.t1 = min(s.cnt, s.t0 + (sh.end - u));
+    u += s.t1 - s.t0;
+    s.seq = a.planned ? a.seg_seq[j] : j;
+    s.r0 = a.planned ? (int32_t)a.seg_rt[j] * R : 0;
+    return s;
+}
+
+// N consecutive values of a row as f32, of which `have` exist (the others 0).
+template <int QT, int N>
+__device__ __forceinline__ void load_row(const char *row, int at, int have, bool wide, float *v) {
+    using E = typename RowType<QT>::type;
+    if (at >= have) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = 0.0f;
+    } else if (wide) {
+        constexpr int C = 16 / (int)sizeof(E) < N ? 16 / (int)sizeof(E) : N;
+        typedef E vec __attribute__((ext_vector_type(C)));
+#pragma unroll
+        for (int i = 0; i < N / C; i++) {
+            const vec x = *reinterpret_cast<const vec *>(row + (size_t)(at + i * C) * sizeof(E));
+#pragma unroll
+            for (int j = 0; j < C; j++) v[i * C + j] = (float)x[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = (float)reinterpret_cast<const E *>(row)[at + i];
+    }
+}
+
+// Four outputs of a row: times the gate, rounded, stored.
+template <int QT>
+__device__ __forceinline__ void store_out(const AttnPagedArgs &a, int64_t row, int head, int dim, float *v) {
+    using E = typename RowType<QT>::type;
+    if (a.gate.p) {
+        const char *gp = a.gate.p + (row * a.gate.row + (int64_t)head * a.gate.head + dim) * (int64_t)sizeof(E);
+        float g[4];
+        load_row<QT, 4>(gp, 0, 4, a.out_wide, g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] *= 1.0f / (1.0f + expf(-g[i]));
+    }
+    E *o = (E *)a.out.p + row * a.out.row + (int64_t)head * a.out.head + dim;
+    typedef E vec __attribute__((ext_vector_type(4)));
+    if (a.out_wide) {
+        vec x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = (E)v[i];
+        *reinterpret_cast<vec *>(o) = x;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = (E)v[i];
+    }
+}
+
+// Bits 15 and 31 of the result: the low and high 16-bit value of w is an infinity or a NaN (its exponent plus one carries).
+template <int CT>
+__device__ __forceinline__ unsigned odd_bits(unsigned w) {
+    return (w & 0x7FFF7FFFu) + (CT == AQ_TYPE_F16 ? 0x04000400u : 0x00800080u);
+}
+// All bits of such a value, none of others.
+template <int CT>
+__device__ __forceinline__ unsigned odd_mask(unsigned w) {
+    return ((odd_bits<CT>(w) & 0x80008000u) >> 15) * 0xFFFFu;
+}
+
 // Workspace layout, the same in the size query and in the launch.
 struct PagedSpace {
     size_t plan = 0, seg = 0, o = 0, ml = 0, bytes = 0;
@@ -79,6 +252,10 @@ inline PagedSpace paged_space(size_t shares, size_t n_seg, size_t R, size_t D) {
 }
 
 int launch_paged_plan(const AttnPagedArgs &a, int R, uint32_t tk, hipStream_t stream);
+int launch_paged_chunk(const AttnPagedArgs &a, int D, hipStream_t stream); // 16-bit rows and cache
 int launch_paged_combine(const AttnPagedArgs &a, int R, int D, hipStream_t stream);
+
+constexpr int CHUNK_ROWS = 128;                                   // paged_chunk.hip's row tile
+constexpr int chunk_keys(int D) { return D == 256 ? 32 : 64; } // and its unit
 
 } // namespace aq

@@ -1,0 +1,404 @@
+// paged_chunk.hip — attention of many 16-bit rows (prompt chunks, whole prompts) over a paged cache of their type: bound
+// by the matrix cores (4 D flops a row and position).
+//
+// A work-group's 128 rows lie on four waves of 32; the keys come in tiles of 64 (heads past 128: 32), K and V through
+// the LDS, the next tile loaded while this one is summed:
+//   S^T = K Q^T   32x32x16: A = K from the LDS, B = Q^T in registers for the whole segment. Lane (n, h) = (lane & 31,
+//                 lane >> 5) then holds row n's scores of positions 8 (i / 4) + 4 h + i % 4, so that a row's maximum and
+//                 sum are in two lanes: one exchange (v_permlane32_swap) per tile.
+//   O^T = V^T P^T the exponentials, rounded, are B's layout as they stand if k-slot (h, e) stands for position 8 (e / 4) +
+//                 4 h + e % 4; A = V^T comes from the row-major V tile by transposing LDS reads (ds_read_b64_tr_b16).
+// The maximum a row's exponentials are taken against moves only when it grows by more than 2^7 (the sums hold that), so
+// that outputs are rarely rescaled.
+//
+// Tiles are loaded straight into the LDS (16 bytes a lane, consecutive lanes consecutive addresses), each lane choosing
+// which 16 bytes of its row it fetches: the row's chunks are swapped by an exclusive or with the row's low bits, so that
+// neither kind of read meets a bank twice. Rows without a page come from a row of zeros.
+#include <atomic>
+#include <type_traits>
+
+#include "paged_attn.h"
+
+namespace aq {
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+__device__ const u4 zeros = {0, 0, 0, 0};
+
+template <int CT>
+__device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
+    if constexpr (CT == AQ_TYPE_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+template <int CT>
+__device__ __forceinline__ unsigned pack2(float x, float y) {
+    using E = typename RowType<CT>::type;
+    typedef E e2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, e2));
+}
+
+// The larger of x's two halves (lanes l and l + 32).
+__device__ __forceinline__ float both_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int D>
+struct ChunkShape {
+    static constexpr int RB = D * 2, CPR = D / 8;             // bytes and 16-byte chunks of a row
+    static constexpr int KEYS = chunk_keys(D), HALVES = KEYS / 32; // positions of a tile; 32 x 32 score tiles
+    static constexpr int TILE_BYTES = KEYS * RB;
+    static constexpr int LOADS = TILE_BYTES / (256 * 16);     // 16-byte loads per thread and tile, of K and of V
+    static constexpr int LDS = 4 * TILE_BYTES;                // two buffers of each
+    // which chunk of row r lies at place p: p ^ swizzle(r)
+    static __device__ __forceinline__ int swizzle(int r) { return D == 64 ? ((r >> 1) & 3) << 1 : (r & 7) << 1; }
+};
+
+#define AQ_LDS __attribute__((address_space(3)))
+#define AQ_GLB __attribute__((address_space(1)))
+
+template <int CT, int D>
+__global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
+    using S = ChunkShape<D>;
+    constexpr int R = CHUNK_ROWS, KEYS = S::KEYS, HALVES = S::HALVES, STEPS = D / 16, DB = D / 32;
+    constexpr float P_SHIFT = CT == AQ_TYPE_F16 ? 7.0f : 0.0f, GROW = 7.0f;
+    extern __shared__ __align__(16) char smem[];
+    __shared__ uint32_t pre[INLINE_SEQS + 1], wsum[4], found;
+    char *kbuf = smem, *vbuf = smem + 2 * S::TILE_BYTES;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hd = a.kv.hd, G = a.G;
+
+    // LDS addresses of this lane's reads of K (operand step 0) and V (dimensions 0 .. 31); the other steps by an exclusive
+    // or, rows and chunks from 16 on by constant offsets
+    const int n0 = lane & 31, h0 = lane >> 5, vi = lane & 15, vkey = 4 * h0 + vi / 4;
+    const int kaddr0 = n0 * S::RB + ((h0 ^ S::swizzle(n0)) << 4);
+    const int vaddr0 = vkey * S::RB + (((2 * ((lane >> 4) & 1) + (vi % 4) / 2) ^ S::swizzle(vkey)) << 4) + (vi % 2) * 8;
+
+    const Share sh = take_share(a, R, KEYS, pre, wsum, &found);
+    uint32_t u = sh.begin, j = sh.j;
+    while (u < sh.end) { // uniform
+        const Segment sg = next_segment(a, R, pre, sh, u, j);
+        const int n = here(n0), h = here(h0);
+        const SeqRows sr = paged_seq(a.b, sg.seq);
+        const int32_t n_rows = sr.n * G, base = sr.len - sr.n;
+        const UnitRange range = tile_units(sr, G, a.window, a.cap, sg.r0, R, KEYS);
+        const int32_t *table = a.b.pages + (size_t)sg.seq * a.b.max_pages;
+        const uint64_t head_off = (uint64_t)sg.kvh * a.kv.head_bytes;
+        const int32_t seg_last = (min(sg.r0 + R, n_rows) - 1) / G;
+        const int32_t kend = min(max(base + seg_last + 1, 0), (int32_t)a.cap); // positions from here on: nobody's
+
+        // this lane's row, and what the wave's rows see between them
+        const int32_t rr = sg.r0 + 32 * wave + n, tok = rr / G;
+        const bool have = rr < n_rows;
+        const int32_t hi = have ? base + tok + 1 : 0;
+        const int64_t lo64 = a.window ? (int64_t)base + tok + 1 - (int64_t)a.window : 0;
+        const int32_t lo = lo64 > 0 ? (int32_t)lo64 : 0;
+        const int32_t w0 = sg.r0 + 32 * wave, w1 = min(w0 + 32, n_rows) - 1;
+        const bool idle = w0 >= n_rows; // a wave without rows only loads
+        const int32_t tok0 = w0 / G, tok1 = idle ? tok0 : w1 / G;
+        const int32_t min_hi = base + tok0 + 1, max_hi = idle ? 0 : base + tok1 + 1;
+        const int64_t min_lo = a.window ? (int64_t)base + tok0 + 1 - (int64_t)a.window : INT64_MIN,
+                      max_lo = a.window ? (int64_t)base + tok1 + 1 - (int64_t)a.window : INT64_MIN;
+
+        constexpr uint64_t ALL = KEYS == 64 ? ~0ull : (1ull << (KEYS & 63)) - 1;
+        // where a tile's rows are: lane l has position l's; bit l of the result: it has a page
+        auto locate = [&](int32_t tile, uint32_t *units) {
+            const int32_t p = tile * KEYS + lane;
+            const bool ok = p < kend && lane < KEYS && paged_slot(a.kv, table, a.b.max_pages, (uint32_t)p, units);
+            if (!ok) *units = 0xFFFFFFFFu;
+            return (uint64_t)__ballot(ok);
+        };
+        const char *const kpool = a.kv.k + head_off, *const vpool = a.kv.v + head_off;
+        auto load_tile = [&](uint32_t units, uint64_t ok, int buf) {
+            const int ln = here(lane), last = hd / 8 - 1;
+            char *kd = kbuf + buf * S::TILE_BYTES + wave * S::LOADS * 1024, *vd = vbuf + (kd - kbuf);
+#pragma unroll
+            for (int i = 0; i < S::LOADS; i++) {
+                const int at = i * 64 + ln, row = wave * (S::LOADS * 64 / S::CPR) + at / S::CPR, place = at % S::CPR;
+                // past the head: the queries are 0 there, the outputs not stored
+                const uint32_t c = (uint32_t)min(place ^ S::swizzle(row), last);
+                const uint64_t off = ((uint64_t)(uint32_t)__shfl((int)units, row) << a.kv.unit_shift) + c * 16;
+                const char *kp = kpool + off, *vp = vpool + off;
+                if (ok != ALL) { // uniform
+                    const bool has = (ok >> row) & 1;
+                    kp = has ? kp : (const char *)&zeros;
+                    vp = has ? vp : (const char *)&zeros;
+                }
+                __builtin_amdgcn_global_load_lds((const AQ_GLB void *)kp, (AQ_LDS void *)(kd + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const AQ_GLB void *)vp, (AQ_LDS void *)(vd + i * 1024), 16, 0, 0);
+            }
+        };
+
+        // ---- queries
+        u4 q[STEPS];
+        {
+            const char *row = a.q.p + ((int64_t)(sr.first + tok) * a.q.row + (int64_t)((int)sg.kvh * G + (rr - tok * G)) * a.q.head) * 2;
+#pragma unroll
+            for (int s = 0; s < STEPS; s++) {
+                const int at = 16 * s + 8 * h;
+                u4 x = u4{0u, 0u, 0u, 0u};
+                if (have && at < hd) {
+                    if (a.q_wide) {
+                        x = *reinterpret_cast<const u4 *>(row + at * 2);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint16_t *y = reinterpret_cast<const uint16_t *>(row) + at + 2 * e;
+                            x[e] = y[0] | ((uint32_t)y[1] << 16);
+                        }
+                    }
+                }
+                q[s] = x;
+            }
+        }
+
+        f16v o[DB];
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[db][i] = 0.0f;
+        float mc = -INFINITY, l = 0.0f; // the maximum times scale_log2; this lane's part of the sum
+        bool big = false;               // some row's is past 2^20: products and difference are rounded apart
+
+        int32_t t = (int32_t)(range.lo + sg.t0);
+        const int32_t t_end = (int32_t)(range.lo + sg.t1);
+        uint32_t units, units_next = 0xFFFFFFFFu;
+        uint64_t ok = locate(t, &units), ok_next = 0;
+        __syncthreads(); // the segment before has read its tiles
+        load_tile(units, ok, 0);
+        if (t + 1 < t_end) ok_next = locate(t + 1, &units_next);
+        int buf = 0;
+        for (; t < t_end; t++) {
+            const int32_t kb = t * KEYS;
+            const char *kt = kbuf + buf * S::TILE_BYTES, *vt = vbuf + buf * S::TILE_BYTES;
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const uint64_t ok_now = ok;
+            if (t + 1 < t_end) {
+                load_tile(units_next, ok_next, buf ^ 1);
+                ok = ok_next;
+                if (t + 2 < t_end) ok_next = locate(t + 2, &units_next);
+            }
+            const bool work = kb < max_hi && (int64_t)kb + KEYS > min_lo; // uniform in the wave
+            const bool edge = kb + KEYS > min_hi || (int64_t)kb < max_lo || ok_now != ALL;
+            // One tile; CAREFUL: with what only tiles at an edge, with holes or with huge scores need. False: nothing done,
+            // the scores are huge.
+            auto sum_tile = [&](auto careful) __attribute__((always_inline)) {
+                constexpr bool CAREFUL = decltype(careful)::value;
+                f16v s[HALVES];
+                const int ka = here(kaddr0), va = here(vaddr0);
+#pragma unroll
+                for (int k = 0; k < HALVES; k++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[k][i] = 0.0f;
+#pragma unroll
+                for (int st = 0; st < STEPS; st++)
+#pragma unroll
+                    for (int k = 0; k < HALVES; k++) {
+                        const u4 x = *reinterpret_cast<const u4 *>(kt + (ka ^ (st % 8 * 32)) + 32 * k * S::RB + (st / 8) * 256);
+                        s[k] = mfma32<CT>(x, q[st], s[k]);
+                        if (st % (8 / HALVES) == 8 / HALVES - 1 && k == HALVES - 1) __builtin_amdgcn_sched_barrier(0);
+                    }
+                if (CAREFUL && edge) {
+                    const int hr = hi - kb - 4 * h, lr = lo - kb - 4 * h; // of position 0 of this lane's
+#pragma unroll
+                    for (int k = 0; k < HALVES; k++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int pos = 32 * k + 8 * (i / 4) + i % 4;
+                            s[k][i] = pos < hr && pos >= lr ? s[k][i] : -INFINITY;
+                        }
+                    if (ok_now != ALL) {
+                        const uint64_t mine = ok_now >> (4 * here(h));
+#pragma unroll
+                        for (int k = 0; k < HALVES; k++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                s[k][i] = (mine >> (32 * k + 8 * (i / 4) + i % 4)) & 1 ? s[k][i] : -INFINITY;
+                    }
+                }
+                float mt = s[0][0];
+#pragma unroll
+                for (int i = 1; i < 16 * HALVES; i++) mt = fmaxf(mt, s[i / 16][i % 16]);
+                mt = both_max(mt) * a.scale_log2;
+                if (!CAREFUL && __any(!(fabsf(mt) < 1048576.0f))) return false;
+                if (__any(mt > mc + GROW || (mc == -INFINITY && mt > mc))) {
+                    const float mn = fmaxf(mc, mt), mu = mn == -INFINITY ? 0.0f : mn;
+                    const float alpha = fast_exp2(mc - mu);
+                    l *= alpha;
+#pragma unroll
+                    for (int db = 0; db < DB; db++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[db][i] *= alpha;
+                    mc = mn;
+                    big = __any(!(fabsf(mc) < 1048576.0f) && mc != -INFINITY);
+                }
+                const float mu = mc == -INFINITY ? 0.0f : mc;
+                if (CAREFUL && big) {
+#pragma unroll
+                    for (int k = 0; k < HALVES; k++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) s[k][i] = fast_exp2((s[k][i] * a.scale_log2 - mu) + P_SHIFT);
+                } else {
+                    const float off = P_SHIFT - mu;
+#pragma unroll
+                    for (int k = 0; k < HALVES; k++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) s[k][i] = fast_exp2(fmaf(s[k][i], a.scale_log2, off));
+                }
+#pragma unroll
+                for (int k = 0; k < HALVES; k++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) l += s[k][i];
+                u4 p[2 * HALVES]; // of 16 positions each
+#pragma unroll
+                for (int kk = 0; kk < 2 * HALVES; kk++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        p[kk][e] = pack2<CT>(s[kk / 2][8 * (kk % 2) + 2 * e], s[kk / 2][8 * (kk % 2) + 2 * e + 1]);
+
+                auto v_operand = [&](int kk, int db) {
+                    u4 x;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const char *at = vt + (va ^ (db % 4 * 64)) + (16 * kk + 8 * e) * S::RB + (db / 4) * 256;
+                        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AQ_LDS s4 *)at);
+                        const u2 z = __builtin_bit_cast(u2, y);
+                        x[2 * e] = z[0];
+                        x[2 * e + 1] = z[1];
+                    }
+                    return x;
+                };
+                uint64_t odd = 0; // positions whose V row holds an infinity or a NaN
+                if (CAREFUL && edge && tok0 < tok1) {
+                    unsigned any = 0;
+                    const int ln = here(lane);
+#pragma unroll 4
+                    for (int c = 0; c < S::CPR; c++) {
+                        const u4 x = *reinterpret_cast<const u4 *>(vt + (ln % KEYS) * S::RB + ((c + ln) % S::CPR) * 16);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) any |= odd_bits<CT>(x[e]);
+                    }
+                    odd = __ballot(any & 0x80008000u) & ALL;
+                }
+                if (CAREFUL && odd) {
+                    // A position that only some rows see must not reach the others as a 0 times an infinity: such values
+                    // are added position by position, to the rows that see them, and left out of the product.
+#pragma unroll 1
+                    for (uint64_t rest = odd; rest; rest &= rest - 1) {
+                        const int pos = __builtin_ctzll(rest), e = 4 * (pos / 8 % 2) + pos % 4;
+                        u4 only = u4{0u, 0u, 0u, 0u};
+                        if (pos / 4 % 2 == h) only[e / 2] = e & 1 ? 0xFFFF0000u : 0x0000FFFFu;
+                        const bool sees = kb + pos < hi && kb + pos >= lo;
+#pragma unroll
+                        for (int kk = 0; kk < 2 * HALVES; kk++)
+                            if (pos / 16 == kk) { // uniform
+#pragma unroll
+                                for (int db = 0; db < DB; db++) {
+                                    u4 x = v_operand(kk, db) & only;
+#pragma unroll
+                                    for (int y = 0; y < 4; y++) x[y] &= odd_mask<CT>(x[y]);
+                                    const f16v r = mfma32<CT>(x, p[kk], o[db]);
+#pragma unroll
+                                    for (int i = 0; i < 16; i++) o[db][i] = sees ? r[i] : o[db][i];
+                                }
+                            }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 2 * HALVES; kk++)
+#pragma unroll
+                        for (int db = 0; db < DB; db++) {
+                            u4 x = v_operand(kk, db);
+#pragma unroll
+                            for (int y = 0; y < 4; y++) x[y] &= ~odd_mask<CT>(x[y]);
+                            o[db] = mfma32<CT>(x, p[kk], o[db]);
+                        }
+                } else {
+#pragma unroll
+                    for (int kk = 0; kk < 2 * HALVES; kk++)
+#pragma unroll
+                        for (int db = 0; db < DB; db++) {
+                            o[db] = mfma32<CT>(v_operand(kk, db), p[kk], o[db]);
+                            if (db % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                        }
+                }
+                return true;
+            };
+            if (work && (edge || big || !sum_tile(std::false_type{}))) sum_tile(std::true_type{});
+            buf ^= 1;
+        }
+
+        // ---- out: the whole segment's rows, or this share's part
+        {
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+            l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+        if (!have) continue; // no barrier below in this pass
+        const int hs = here(h);
+        const bool cut = sg.t1 - sg.t0 < sg.cnt;
+        float *part = a.part_o + ((size_t)(2 * sh.w + (sg.t0 == 0 ? 1 : 0)) * R + 32 * wave + n) * D;
+        if (cut && hs == 0) {
+            float *ml = a.part_ml + ((size_t)(2 * sh.w + (sg.t0 == 0 ? 1 : 0)) * R + 32 * wave + n) * 2;
+            ml[0] = mc;
+            ml[1] = l;
+        }
+        const float inv = cut ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int db = 0; db < DB; db++) {
+            const int d0 = here(4 * hs) + 32 * db;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (d0 + 8 * i >= hd) break;
+                float out[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) out[e] = inv == 0.0f ? 0.0f : o[db][4 * i + e] * inv;
+                if (cut) *reinterpret_cast<f4 *>(part + d0 + 8 * i) = f4{out[0], out[1], out[2], out[3]};
+                else store_out<CT>(a, sr.first + tok, (int)sg.kvh * G + (rr - tok * G), d0 + 8 * i, out);
+            }
+            asm volatile("" ::: "memory");
+        }
+    }
+}
+
+template <int CT, int D>
+int chunk_launch(const AttnPagedArgs &a, hipStream_t stream) {
+    using S = ChunkShape<D>;
+    static std::atomic<uint64_t> raised{0}; // bit d: done on device d
+    int dev = 0;
+    AQ_HIP(hipGetDevice(&dev));
+    if (!(raised.load() & (1ull << (dev & 63)))) {
+        AQ_HIP(hipFuncSetAttribute((const void *)chunk_kernel<CT, D>, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
+        raised.fetch_or(1ull << (dev & 63));
+    }
+    chunk_kernel<CT, D><<<a.shares, 256, S::LDS, stream>>>(a);
+    AQ_HIP(hipGetLastError());
+    return 0;
+}
+
+} // namespace
+
+int launch_paged_chunk(const AttnPagedArgs &a, int D, hipStream_t stream) {
+    if (a.kv.type == AQ_TYPE_F16) {
+        if (D == 64) return chunk_launch<AQ_TYPE_F16, 64>(a, stream);
+        if (D == 128) return chunk_launch<AQ_TYPE_F16, 128>(a, stream);
+        return chunk_launch<AQ_TYPE_F16, 256>(a, stream);
+    }
+    if (D == 64) return chunk_launch<AQ_TYPE_BF16, 64>(a, stream);
+    if (D == 128) return chunk_launch<AQ_TYPE_BF16, 128>(a, stream);
+    return chunk_launch<AQ_TYPE_BF16, 256>(a, stream);
+}
+
+} // namespace aq
