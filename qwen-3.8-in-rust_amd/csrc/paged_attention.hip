@@ -26,9 +26,14 @@ namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
+
+// Positions that a wave of the few-row kernel takes at once: 32, and 16 of a wide head, whose rows fill the registers.
+constexpr int few_tile(int CT, int D) { return CT != AQ_TYPE_F32 && D == 256 ? 16 : 32; }
 
 template <int CT>
 __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
@@ -38,86 +43,151 @@ __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
-// The sum of v over pieces: v as NP values of the type, each the rounding of what the ones before left.
-template <int CT, int NP>
-__device__ __forceinline__ void pieces(const float *v, u4 *out) { // 8 values -> NP operands
-    using E = typename RowType<CT>::type;
-    typedef E vec __attribute__((ext_vector_type(8)));
-    float rest[8];
+// O^T += V^T P^T over 32 positions (16-byte operands) or 16 (8-byte ones).
+template <int CT>
+__device__ __forceinline__ f4 mfma_pv(u4 a, u4 b, f4 c) {
+    return mfma16<CT>(a, b, c);
+}
+template <int CT>
+__device__ __forceinline__ f4 mfma_pv(u2 a, u2 b, f4 c) {
+    if constexpr (CT == AQ_TYPE_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4, a), __builtin_bit_cast(h4, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
+}
+
+// v as NP operands of the type: each the rounding of what the ones before left.
+template <int CT, int NP, typename V>
+__device__ __forceinline__ void pieces(const float *v, V *out) {
+    using T = typename RowType<CT>::type;
+    constexpr int N = sizeof(V) / 2;
+    typedef T vec __attribute__((ext_vector_type(N)));
+    float rest[N];
 #pragma unroll
-    for (int i = 0; i < 8; i++) rest[i] = v[i];
+    for (int i = 0; i < N; i++) rest[i] = v[i];
 #pragma unroll
     for (int p = 0; p < NP; p++) {
         vec x;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[i] = (E)rest[i];
+        for (int i = 0; i < N; i++) {
+            x[i] = (T)rest[i];
             if (p + 1 < NP) rest[i] -= (float)x[i];
         }
-        out[p] = __builtin_bit_cast(u4, x);
+        out[p] = __builtin_bit_cast(V, x);
     }
 }
 
 // An infinity or a NaN.
 __device__ __forceinline__ bool odd_f32(unsigned w) { return (w & 0x7F800000u) == 0x7F800000u; }
 
-constexpr int WAVES = 4, TILE = 32, UNIT = WAVES * TILE; // positions of a wave's tile and of a work-group's step
+constexpr int WAVES = 4;
 
-// What the few-row kernel keeps where, for one cache type, row type and padded head size.
-template <int CT, bool FQ, int D, int NR>
+// What the few-row kernel keeps where, for one cache type, row type, padded head size and rows (16 or 32). The rows lie
+// on a wave's NR accumulator tiles; 32 rows of a wide head would not fit its registers, so there two waves take 16 rows
+// each over the same positions (RG = 2: the second reads them from the cache the first filled).
+constexpr int few_groups(int CT, int D, int R) { return R == 32 && (D == 256 || (CT == AQ_TYPE_F32 && D == 128)) ? 2 : 1; }
+constexpr int few_unit(int CT, int D, int R) { return WAVES / few_groups(CT, D, R) * few_tile(CT, D); }
+template <int CT, bool FQ, int D, int ROWS>
 struct FewShape {
+    static constexpr int R = ROWS, RG = few_groups(CT, D, R), KW = WAVES / RG, NT = R / 16, NR = NT / RG;
     static constexpr bool F = CT == AQ_TYPE_F32;
     static constexpr int NP = !FQ || F ? 1 : (CT == AQ_TYPE_F16 ? 2 : 3); // pieces of q and of the probabilities
-    static constexpr int STEPS = F ? D / 16 : D / 32;                     // 16-byte K operands of a row per lane
-    static constexpr int VB = F || D == 64 ? 4 : 8;                       // dimensions of a V row per lane and chunk
+    static constexpr int TILE = few_tile(CT, D);  // positions of a wave's step
+    static constexpr int E = TILE / 4;                // of them a lane's: 16 (e / 4) + 4 g + e % 4
+    static constexpr int STEPS = F ? D / 16 : D / 32; // 16-byte K operands of a row per lane
+    static constexpr int VB = F || D == 64 ? 4 : 8;   // dimensions of a V row per lane and chunk
     static constexpr int CHUNKS = D / (16 * VB);
     static constexpr int ACC = CHUNKS * VB; // accumulators (4 values each) per row tile
-    static constexpr int R = 16 * NR;
-    static constexpr int PASSES = D / 64, CROW = 68; // the waves' outputs meet 64 dimensions at a time
-    static constexpr int QF = NR * STEPS * NP * 64;  // 16-byte operands of q
-    static constexpr int LDS = QF * 16 + WAVES * R * CROW * 4 + WAVES * R * 8;
-    static constexpr bool AHEAD = D <= 128 || NR == 1; // the next tile's K rows loaded while this one is summed
+    static constexpr int PASSES = D / 64, CROW = 68;  // the waves' outputs meet 64 dimensions at a time
+    static constexpr int QF = NT * STEPS * NP * 64 * 16, CB = KW * R * CROW * 4; // bytes of q; of the meeting
+    static constexpr int LDS = (QF > CB ? QF : CB) + KW * R * 8;
 };
 
-template <int CT, bool FQ, int D, int NR>
+// EXACT: the head fills D, so that a row's loads differ by constants only.
+template <int CT, bool FQ, int D, int R, bool EXACT>
 __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
-    using S = FewShape<CT, FQ, D, NR>;
+    using S = FewShape<CT, FQ, D, R>;
     constexpr bool F = S::F;
-    constexpr int QT = FQ ? AQ_TYPE_F32 : CT, NP = S::NP, STEPS = S::STEPS, CHUNKS = S::CHUNKS, VB = S::VB, R = S::R;
-    constexpr int ES = F ? 4 : 2;
+    constexpr int QT = FQ ? AQ_TYPE_F32 : CT, NP = S::NP, STEPS = S::STEPS, CHUNKS = S::CHUNKS, VB = S::VB;
+    constexpr int RG = S::RG, KW = S::KW, NT = S::NT, NR = S::NR;
+    constexpr int TILE = S::TILE, UNIT = KW * TILE, E = S::E, HT = TILE / 16, ES = F ? 4 : 2;
     // f16 probabilities are kept at 2^14 times their size (and so are the sums): their small ones stay normal numbers
     constexpr float P_SHIFT = CT == AQ_TYPE_F16 ? 14.0f : 0.0f;
     extern __shared__ __align__(16) char smem[];
     u4 *qf = reinterpret_cast<u4 *>(smem);
-    float *comb = reinterpret_cast<float *>(smem + S::QF * 16);        // [WAVES][R][CROW]
-    float *ml = reinterpret_cast<float *>(smem + S::QF * 16 + WAVES * R * S::CROW * 4); // [WAVES][R][2]
-    __shared__ uint32_t pre[INLINE_SEQS + 1], wsum[WAVES], qmax[R], found;
+    float *comb = reinterpret_cast<float *>(smem);                           // [KW][R][CROW], after the last tile
+    float *ml = reinterpret_cast<float *>(smem + S::LDS - KW * R * 8); // [KW][R][2]
+    __shared__ PlanLds plan;
+    __shared__ uint32_t qmax[R];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 15, g = lane >> 4;
-    const int hd = a.kv.hd, G = a.G;
+    const int r = lane & 15, g = lane >> 4, rg = wave % RG, kg = wave / RG; // which rows, which positions
+    const int hd = EXACT ? D : a.kv.hd, G = a.G;
 
-    const Share sh = take_share(a, R, UNIT, pre, wsum, &found);
+    const Share sh = take_share(a, R, UNIT, plan);
     uint32_t u = sh.begin, j = sh.j;
     while (u < sh.end) { // uniform
-        const Segment sg = next_segment(a, R, pre, sh, u, j);
-        const uint32_t kvh = sg.kvh, seq = sg.seq, t0 = sg.t0, t1 = sg.t1;
+        const Segment sg = next_segment(a, R, plan, sh, u, j);
+        const uint32_t kvh = sg.kvh;
         const int32_t r0 = sg.r0;
-        const SeqRows sr = paged_seq(a.b, seq);
+        const SeqRows sr = paged_seq(a.b, sg.seq);
         const int32_t n_rows = sr.n * G, base = sr.len - sr.n;
-        const UnitRange range = tile_units(sr, G, a.window, a.cap, r0, R, UNIT);
-        const int32_t tok0 = r0 / G, tok1 = (min(r0 + R, n_rows) - 1) / G;
+        const UnitRange range = tile_units(a, sr, r0, R, UNIT);
+        const int32_t tok0 = (int32_t)a.by_g.quot(r0), tok1 = (int32_t)a.by_g.quot(min(r0 + R, n_rows) - 1);
         const int32_t kend = min(max(base + tok1 + 1, 0), (int32_t)a.cap);
         const int32_t min_hi = base + tok0 + 1;
         const int64_t max_lo = a.window ? (int64_t)base + tok1 + 1 - (int64_t)a.window : INT64_MIN;
-        const int32_t *table = a.b.pages + (size_t)seq * a.b.max_pages;
+        const int32_t *table = a.b.pages + (size_t)sg.seq * a.b.max_pages;
         const uint64_t head_off = (uint64_t)kvh * a.kv.head_bytes;
+        const char *const kpool = a.kv.k + head_off, *const vpool = a.kv.v + head_off;
+
+        const int32_t last_tile = min((int32_t)((range.lo + sg.t1) * KW), (kend + TILE - 1) / TILE);
+        int32_t tile = (int32_t)(range.lo + sg.t0) * KW + kg;
+        // where the tile's rows are: lane l has position l % TILE's
+        auto locate = [&](int32_t t, uint32_t *units) {
+            const int32_t p = t * TILE + lane % TILE;
+            const bool ok = p < kend && paged_slot(a.kv, table, a.b.max_pages, (uint32_t)p, units);
+            if (!ok) *units = 0;
+            return (uint32_t)__ballot(ok) & (uint32_t)((1ull << TILE) - 1);
+        };
+        constexpr uint32_t ALL = (uint32_t)((1ull << TILE) - 1);
+        auto row_off = [&](uint32_t units, int pos) {
+            return (uint64_t)(uint32_t)__shfl((int)units, pos) << a.kv.unit_shift;
+        };
+        // operands s0 .. s0 + N - 1 of 16 rows of K; dimensions past the head repeat its last ones: q is 0 there
+        auto load_k = [&](uint32_t units, int t, int s0, auto &k) {
+            const char *p = kpool + (row_off(units, 16 * t + r) + (EXACT ? 16 * g : 0));
+            constexpr int N = sizeof(k) / 16;
+#pragma unroll
+            for (int s = 0; s < N; s++) {
+                const int at = EXACT ? 64 * (s0 + s) : min(64 * (s0 + s) + 16 * g, hd * ES - 16);
+                k[s] = *reinterpret_cast<const u4 *>(p + at);
+            }
+        };
+        using VV = typename std::conditional<VB * ES == 8, u2, u4>::type;
+        using VP = typename std::conditional<HT == 1, u2, u4>::type; // probabilities, V^T: E 16-bit values
+        constexpr int VW = VB * ES / 4; // dwords
+        // the row of this lane's e-th position: dimensions VB r .. of each chunk; past the head: outputs not stored
+        auto load_v = [&](uint32_t units, int e, VV *v, int stride) {
+            const char *p = vpool + (row_off(units, 16 * (e / 4) + 4 * g + e % 4) + (EXACT ? VB * ES * r : 0));
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c++) {
+                const int at = EXACT ? c * 16 * VB * ES : min(c * 16 * VB + VB * r, hd - VB) * ES;
+                v[c * stride] = *reinterpret_cast<const VV *>(p + at);
+            }
+        };
+
+        constexpr int KD = F && D == 256 ? STEPS / 2 : STEPS; // operands of a row in registers at once
+        constexpr int KH = F && D == 256 ? 1 : HT;
+        u4 k[KH][KD];
+        uint32_t units = 0, okm = 0;
+        if (tile < last_tile) okm = locate(tile, &units);
 
         // this lane's rows: the positions they see are lo .. hi - 1
         int32_t hi[NR], lo[NR];
 #pragma unroll
         for (int nr = 0; nr < NR; nr++) {
-            const int32_t rr = r0 + 16 * nr + r, tok = rr / G;
+            const int32_t rr = r0 + 16 * (rg * NR + nr) + r, tok = (int32_t)a.by_g.quot(rr);
             hi[nr] = rr < n_rows ? base + tok + 1 : 0;
             const int64_t l = a.window ? (int64_t)base + tok + 1 - (int64_t)a.window : 0;
             lo[nr] = l > 0 ? (int32_t)l : 0;
@@ -127,15 +197,18 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
         // ---- queries into the LDS, operand order; 16 rows x 16 units of 8 (4) dimensions at a time
         float rscale[NR]; // what this lane's rows' scores are multiplied by
         {
-            constexpr int QV = F ? 4 : 8, ALL = NR * (D / QV), UNITS = (ALL + 15) / 16; // 16 at a time
+            constexpr int QV = F ? 4 : 8, UN = NT * (D / QV), UNITS = (UN + 15) / 16;
+            const int th = here(tid), n = th & 15;
             float v[UNITS][QV];
-            if (tid < R) qmax[tid] = 0;
-            if constexpr (NP == 2) __syncthreads();
+            if constexpr (NP == 2) {
+                if (th < R) qmax[th] = 0;
+                __syncthreads();
+            }
 #pragma unroll
             for (int i = 0; i < UNITS; i++) {
-                const int unit = i * 16 + (tid >> 4), nr = unit / (D / QV), at = unit % (D / QV) * QV, n = tid & 15;
-                if (ALL % 16 && unit >= ALL) continue;
-                const int32_t rr = r0 + 16 * nr + n, tok = rr / G;
+                const int unit = i * 16 + (th >> 4), nr = unit / (D / QV), at = unit % (D / QV) * QV;
+                if (UN % 16 && unit >= UN) continue;
+                const int32_t rr = r0 + 16 * nr + n, tok = (int32_t)a.by_g.quot(rr);
                 const int head = (int)kvh * G + (rr - tok * G);
                 const char *row = a.q.p + ((int64_t)(sr.first + tok) * a.q.row + (int64_t)head * a.q.head) *
                                               (int64_t)sizeof(typename RowType<QT>::type);
@@ -152,8 +225,8 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             auto exponent = [&](int row) { return min(max(qmax[row] >> 23, 1u), 253u); };
 #pragma unroll
             for (int i = 0; i < UNITS; i++) {
-                const int unit = i * 16 + (tid >> 4), nr = unit / (D / QV), at = unit % (D / QV), n = tid & 15;
-                if (ALL % 16 && unit >= ALL) continue;
+                const int unit = i * 16 + (th >> 4), nr = unit / (D / QV), at = unit % (D / QV);
+                if (UN % 16 && unit >= UN) continue;
                 if constexpr (F) { // operand s = at / 4, lane (n, g = at % 4)
                     qf[(nr * STEPS + at / 4) * 64 + (at % 4) * 16 + n] =
                         u4{__float_as_uint(v[i][0]), __float_as_uint(v[i][1]), __float_as_uint(v[i][2]),
@@ -173,11 +246,17 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             }
 #pragma unroll
             for (int nr = 0; nr < NR; nr++)
-                rscale[nr] = NP == 2 ? a.scale_log2 * __uint_as_float(exponent(16 * nr + r) << 23) : a.scale_log2;
+                rscale[nr] = NP == 2 ? a.scale_log2 * __uint_as_float(exponent(16 * (rg * NR + nr) + r) << 23) : a.scale_log2;
+        }
+        if constexpr (KH == HT) {
+            if (tile < last_tile) {
+#pragma unroll
+                for (int t = 0; t < HT; t++) load_k(units, t, 0, k[t]);
+            }
         }
         __syncthreads();
 
-        // ---- the wave's tiles of 32 positions
+        // ---- the wave's tiles
         f4 o[NR][S::ACC];
         float m[NR], l[NR];
 #pragma unroll
@@ -187,198 +266,152 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
 #pragma unroll
             for (int i = 0; i < S::ACC; i++) o[nr][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        const int32_t last_tile = min((int32_t)((range.lo + t1) * WAVES), (kend + TILE - 1) / TILE);
-        int32_t tile = (int32_t)(range.lo + t0) * WAVES + wave;
-
-        // where the tile's rows are: lane (and lane + 32) holds position `lane & 31`'s
-        auto locate = [&](int32_t t, uint32_t *units) {
-            const int32_t p = t * TILE + (lane & 31);
-            const bool ok = p < kend && paged_slot(a.kv, table, a.b.max_pages, (uint32_t)p, units);
-            if (!ok) *units = 0;
-            return (uint32_t)__ballot(ok);
-        };
-        auto row_ptr = [&](const char *pool, uint32_t units, int pos) {
-            return pool + (((uint64_t)(uint32_t)__shfl((int)units, pos) << a.kv.unit_shift) + head_off);
-        };
-        auto load_k = [&](uint32_t units, int t, u4 *k) { // one 16-position half
-            const char *p = row_ptr(a.kv.k, units, 16 * t + r);
+        // The scores of one tile, in place: scaled, hidden ones taken out, then their exponentials against the running
+        // maximum, which the sums and outputs follow.
+        auto soften = [&](int nr, float *x, int32_t kb, uint32_t ok, bool edge) {
+            float mt = -INFINITY;
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                // dimensions past the head repeat its last ones: q is 0 there
-                const int at = min((F ? 16 : 32) * s + (F ? 4 : 8) * g, hd - (F ? 4 : 8));
-                k[s] = *reinterpret_cast<const u4 *>(p + at * ES);
+            for (int e = 0; e < E; e++) x[e] *= rscale[nr];
+            if (edge) {
+                const int gh = here(4 * g);
+                const int hr = hi[nr] - kb - gh, lr = lo[nr] - kb - gh; // of the lane's first position
+                const uint32_t mine = ok >> gh;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const int pos = 16 * (e / 4) + e % 4;
+                    x[e] = pos < hr && pos >= lr && ((mine >> pos) & 1) ? x[e] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) mt = fmaxf(mt, x[e]);
+            mt = fmaxf(mt, __shfl_xor(mt, 16));
+            mt = fmaxf(mt, __shfl_xor(mt, 32));
+            const float mn = fmaxf(m[nr], mt), mu = mn == -INFINITY ? 0.0f : mn;
+            if (__any(mn > m[nr])) {
+                const float alpha = fast_exp2(m[nr] - mu);
+                l[nr] *= alpha;
+#pragma unroll
+                for (int i = 0; i < S::ACC; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[nr][i][e] *= alpha;
+                m[nr] = mn;
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                x[e] = fast_exp2((x[e] - mu) + P_SHIFT);
+                l[nr] += x[e];
             }
         };
 
-        constexpr int KH = F ? 1 : 2; // 16-position halves of K in registers at once
-        u4 k[KH][STEPS];
-        uint32_t units = 0, okm = 0;
-        if (tile < last_tile) {
-            okm = locate(tile, &units);
-            if constexpr (S::AHEAD && !F) {
-#pragma unroll
-                for (int t = 0; t < 2; t++) load_k(units, t, k[t]);
-            }
-        }
-        for (; tile < last_tile; tile += WAVES) {
+        for (; tile < last_tile; tile += KW) {
             asm volatile("" ::: "memory"); // q's operands are read from the LDS each time, not kept in registers
             const int32_t kb = tile * TILE;
-            const uint32_t here = units, ok = okm;
-            // the next tile's page entries, ahead of its rows
-            if (tile + WAVES < last_tile) okm = locate(tile + WAVES, &units);
-            f4 s[NR][2];
+            const uint32_t now = units, ok = okm;
+            const bool edge = kb + TILE > min_hi || (int64_t)kb < max_lo || ok != ALL; // uniform
+            f4 s[NR][HT];
 #pragma unroll
             for (int nr = 0; nr < NR; nr++)
 #pragma unroll
-                for (int t = 0; t < 2; t++) s[nr][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-
-            // ---- V rows of 8 (f32: 4 per half) positions: lane (r, g) has dimensions VB r .. of chunk c
-            auto load_v = [&](int e, int c, auto *dst) {
-                const int pos = 16 * (e / 4) + 4 * g + e % 4;
-                const char *p = row_ptr(a.kv.v, here, pos);
-                const int at = min(c * 16 * VB + VB * r, hd - VB); // past the head: outputs that are not stored
-                if constexpr (VB * ES == 8) *dst = *reinterpret_cast<const u2 *>(p + at * ES);
-                else *dst = *reinterpret_cast<const u4 *>(p + at * ES);
-            };
+                for (int t = 0; t < HT; t++) s[nr][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
             if constexpr (!F) {
-                using VV = typename std::conditional<VB * ES == 8, u2, u4>::type;
-                constexpr int VW = VB * ES / 4; // dwords
-                if constexpr (!S::AHEAD) {
+                VV v[CHUNKS][E];
 #pragma unroll
-                    for (int t = 0; t < 2; t++) load_k(here, t, k[t]);
-                }
-                VV v[CHUNKS][8];
-#pragma unroll
-                for (int c = 0; c < (S::AHEAD ? CHUNKS : 1); c++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) load_v(e, c, &v[c][e]);
+                for (int e = 0; e < E; e++) load_v(now, e, &v[0][e], E);
+                if (tile + KW < last_tile) okm = locate(tile + KW, &units); // the next tile's page entries
+                const u4 *ql = qf + rg * NR * STEPS * NP * 64 + here(lane);
 #pragma unroll
                 for (int st = 0; st < STEPS; st++)
 #pragma unroll
                     for (int nr = 0; nr < NR; nr++)
 #pragma unroll
                         for (int p = 0; p < NP; p++) {
-                            const u4 q = qf[((nr * STEPS + st) * NP + p) * 64 + lane];
+                            const u4 q = ql[((nr * STEPS + st) * NP + p) * 64];
 #pragma unroll
-                            for (int t = 0; t < 2; t++) s[nr][t] = mfma16<CT>(k[t][st], q, s[nr][t]);
+                            for (int t = 0; t < HT; t++) s[nr][t] = mfma16<CT>(k[t][st], q, s[nr][t]);
+                            if (nr == NR - 1 && p == NP - 1 && st % 2 == 1) __builtin_amdgcn_sched_barrier(0);
                         }
                 if constexpr (NP > 1) { // an infinite key times the pieces of one number is a NaN: by the first piece alone
                     bool nan = false;
 #pragma unroll
                     for (int nr = 0; nr < NR; nr++)
 #pragma unroll
-                        for (int e = 0; e < 8; e++) nan |= s[nr][e / 4][e % 4] != s[nr][e / 4][e % 4];
+                        for (int e = 0; e < E; e++) nan |= s[nr][e / 4][e % 4] != s[nr][e / 4][e % 4];
                     if (__any(nan)) {
 #pragma unroll
                         for (int nr = 0; nr < NR; nr++)
 #pragma unroll
-                            for (int t = 0; t < 2; t++) {
+                            for (int t = 0; t < HT; t++) {
                                 f4 one = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                                 for (int st = 0; st < STEPS; st++)
-                                    one = mfma16<CT>(k[t][st], qf[(nr * STEPS + st) * NP * 64 + lane], one);
+                                    one = mfma16<CT>(k[t][st], ql[(nr * STEPS + st) * NP * 64], one);
 #pragma unroll
                                 for (int i = 0; i < 4; i++) s[nr][t][i] = s[nr][t][i] == s[nr][t][i] ? s[nr][t][i] : one[i];
                             }
                     }
                 }
-                if constexpr (S::AHEAD) {
-                    if (tile + WAVES < last_tile) {
+                if (tile + KW < last_tile) { // the next tile's K rows, while this one is summed
 #pragma unroll
-                        for (int t = 0; t < 2; t++) load_k(units, t, k[t]);
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 1; c < CHUNKS; c++)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) load_v(e, c, &v[c][e]);
+                    for (int t = 0; t < HT; t++) load_k(units, t, 0, k[t]);
                 }
-                const bool edge = kb + TILE > min_hi || (int64_t)kb < max_lo || ok != 0xFFFFFFFFu; // uniform
-                u4 pf[NR][NP];
+                VP pf[NR][NP];
 #pragma unroll
                 for (int nr = 0; nr < NR; nr++) {
-                    float x[8], mt = -INFINITY;
+                    float x[E];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int pos = 16 * (e / 4) + 4 * g + e % 4;
-                        x[e] = s[nr][e / 4][e % 4] * rscale[nr];
-                        if (edge && !(kb + pos < hi[nr] && kb + pos >= lo[nr] && ((ok >> pos) & 1))) x[e] = -INFINITY;
-                        mt = fmaxf(mt, x[e]);
-                    }
-                    mt = fmaxf(mt, __shfl_xor(mt, 16));
-                    mt = fmaxf(mt, __shfl_xor(mt, 32));
-                    const float mn = fmaxf(m[nr], mt), mu = mn == -INFINITY ? 0.0f : mn;
-                    if (__any(mn > m[nr])) {
-                        const float alpha = fast_exp2(m[nr] - mu);
-                        l[nr] *= alpha;
-#pragma unroll
-                        for (int i = 0; i < S::ACC; i++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[nr][i][e] *= alpha;
-                        m[nr] = mn;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[e] = fast_exp2((x[e] - mu) + P_SHIFT);
-                        l[nr] += x[e];
-                    }
+                    for (int e = 0; e < E; e++) x[e] = s[nr][e / 4][e % 4];
+                    soften(nr, x, kb, ok, edge);
                     pieces<CT, NP>(x, pf[nr]);
+                }
+                if (edge) { // rows of positions that no page holds are not numbers that may be multiplied by 0
+                    const uint32_t mine = ok >> here(4 * g);
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+#pragma unroll
+                        for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+                            for (int x = 0; x < VW; x++)
+                                v[c][e][x] = (mine >> (16 * (e / 4) + e % 4)) & 1 ? v[c][e][x] : 0u;
                 }
 #pragma unroll
                 for (int c = 0; c < CHUNKS; c++) {
                     auto product = [&](int jj) { // V^T operand of dimension jj of each lane's VB
-                        u4 t;
+                        VP t;
                         const unsigned sel = jj & 1 ? 0x07060302u : 0x05040100u;
 #pragma unroll
-                        for (int h = 0; h < 4; h++)
+                        for (int h = 0; h < E / 2; h++)
                             t[h] = __builtin_amdgcn_perm(v[c][2 * h + 1][jj / 2], v[c][2 * h][jj / 2], sel);
                         return t;
                     };
-                    if (edge) { // rows of positions that no page holds are not numbers that may be multiplied by 0
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-#pragma unroll
-                            for (int x = 0; x < VW; x++)
-                                v[c][e][x] = (ok >> (16 * (e / 4) + 4 * g + e % 4)) & 1 ? v[c][e][x] : 0u;
-                    }
                     if ((edge && tok0 < tok1) || NP > 1) {
                         // Nor are infinities and NaN of positions that only some of the rows see, and an infinity times
                         // the pieces of one number is a NaN: such values are added position by position, to the rows
                         // that see them, by the probability's first piece, and taken out of the product of the others.
                         unsigned any = 0;
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
+                        for (int e = 0; e < E; e++)
 #pragma unroll
                             for (int x = 0; x < VW; x++) any |= odd_bits<CT>(v[c][e][x]);
-                        uint32_t odd = 0;
                         if (__any(any & 0x80008000u)) {
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                unsigned bits = 0;
-#pragma unroll
-                                for (int x = 0; x < VW; x++) bits |= odd_bits<CT>(v[c][e][x]);
-                                const uint64_t b = __ballot(bits & 0x80008000u);
-#pragma unroll
-                                for (int gg = 0; gg < 4; gg++)
-                                    if ((b >> (16 * gg)) & 0xFFFFu) odd |= 1u << (16 * (e / 4) + 4 * gg + e % 4);
-                            }
-                        }
-                        if (odd) {
 #pragma unroll 1
-                            for (uint32_t rest = odd; rest; rest &= rest - 1) {
-                                const int pos = __ffs(rest) - 1, e = 4 * (pos / 16) + pos % 4; // its k-slot
-                                u4 only = u4{0u, 0u, 0u, 0u};
+                            for (int pos = 0; pos < TILE; pos++) {
+                                const int e = 4 * (pos / 16) + pos % 4; // its k-slot
+#pragma unroll
+                                for (int i = 0; i < E; i++) // nothing of the operands is kept from before the loop
+#pragma unroll
+                                    for (int x = 0; x < VW; x++) asm volatile("" : "+v"(v[c][i][x]));
+                                VP only = {};
                                 if (pos % 16 / 4 == g) only[e / 2] = e & 1 ? 0xFFFF0000u : 0x0000FFFFu;
 #pragma unroll
                                 for (int nr = 0; nr < NR; nr++) {
                                     const bool sees = kb + pos < hi[nr] && kb + pos >= lo[nr];
 #pragma unroll
                                     for (int jj = 0; jj < VB; jj++) {
-                                        u4 vt = product(jj) & only;
+                                        VP vt = product(jj) & only;
 #pragma unroll
-                                        for (int x = 0; x < 4; x++) vt[x] &= odd_mask<CT>(vt[x]);
-                                        const f4 t = mfma16<CT>(vt, pf[nr][0], o[nr][c * VB + jj]);
+                                        for (int x = 0; x < E / 2; x++) vt[x] &= odd_mask<CT>(vt[x]);
+                                        const f4 t = mfma_pv<CT>(vt, pf[nr][0], o[nr][c * VB + jj]);
 #pragma unroll
                                         for (int x = 0; x < 4; x++)
                                             o[nr][c * VB + jj][x] = sees ? t[x] : o[nr][c * VB + jj][x];
@@ -386,19 +419,20 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                                 }
                             }
 #pragma unroll
-                            for (int e = 0; e < 8; e++)
+                            for (int e = 0; e < E; e++)
 #pragma unroll
                                 for (int x = 0; x < VW; x++) v[c][e][x] &= ~odd_mask<CT>(v[c][e][x]);
                         }
                     }
 #pragma unroll
                     for (int jj = 0; jj < VB; jj++) {
-                        const u4 vt = product(jj);
+                        const VP vt = product(jj);
 #pragma unroll
                         for (int nr = 0; nr < NR; nr++)
 #pragma unroll
                             for (int p = 0; p < NP; p++)
-                                o[nr][c * VB + jj] = mfma16<CT>(vt, pf[nr][p], o[nr][c * VB + jj]);
+                                o[nr][c * VB + jj] = mfma_pv<CT>(vt, pf[nr][p], o[nr][c * VB + jj]);
+                        if (jj % 2 == 1) __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             } else {
@@ -406,75 +440,69 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                 auto mul = [](unsigned x, unsigned y, f4 c) {
                     return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x), __uint_as_float(y), c, 0, 0, 0);
                 };
-                u4 v[4][CHUNKS];
+                constexpr int VI = D == 64 ? 8 : 4; // V rows in registers at once
+                VV v[CHUNKS][VI];
+                const u4 *ql = qf + rg * NR * STEPS * NP * 64 + here(lane);
+                if constexpr (KH == HT) {
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    load_k(here, t, k[0]);
-                    if (t == 0) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int c = 0; c < CHUNKS; c++) load_v(i, c, &v[i][c]);
-                    }
-#pragma unroll
-                    for (int st = 0; st < STEPS; st++)
-#pragma unroll
-                        for (int nr = 0; nr < NR; nr++) {
-                            const u4 q = qf[(nr * STEPS + st) * 64 + lane];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) s[nr][t] = mul(k[0][st][i], q[i], s[nr][t]);
-                        }
+                    for (int i = 0; i < VI; i++) load_v(now, i, &v[0][i], VI);
+                    if (tile + KW < last_tile) okm = locate(tile + KW, &units); // the next tile's page entries
                 }
-                const bool edge = kb + TILE > min_hi || (int64_t)kb < max_lo || ok != 0xFFFFFFFFu; // uniform
-                float x[NR][8];
+#pragma unroll
+                for (int t = 0; t < HT; t++) {
+#pragma unroll
+                    for (int s0 = 0; s0 < STEPS; s0 += KD) {
+                        if constexpr (KH < HT) {
+                            load_k(now, t, s0, k[0]);
+                            if (t == HT - 1 && s0 + KD == STEPS) {
+#pragma unroll
+                                for (int i = 0; i < VI; i++) load_v(now, i, &v[0][i], VI);
+                            }
+                        }
+#pragma unroll
+                        for (int st = 0; st < KD; st++)
+#pragma unroll
+                            for (int nr = 0; nr < NR; nr++) {
+                                const u4 q = ql[(nr * STEPS + s0 + st) * 64];
+#pragma unroll
+                                for (int i = 0; i < 4; i++) s[nr][t] = mul(k[t % KH][st][i], q[i], s[nr][t]);
+                            }
+                    }
+                }
+                if constexpr (KH == HT) { // the next tile's K rows, while this one is summed
+                    if (tile + KW < last_tile) {
+#pragma unroll
+                        for (int t = 0; t < HT; t++) load_k(units, t, 0, k[t]);
+                    }
+                }
+                float x[NR][E];
 #pragma unroll
                 for (int nr = 0; nr < NR; nr++) {
-                    float mt = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int pos = 16 * (e / 4) + 4 * g + e % 4;
-                        x[nr][e] = s[nr][e / 4][e % 4] * rscale[nr];
-                        if (edge && !(kb + pos < hi[nr] && kb + pos >= lo[nr] && ((ok >> pos) & 1))) x[nr][e] = -INFINITY;
-                        mt = fmaxf(mt, x[nr][e]);
-                    }
-                    mt = fmaxf(mt, __shfl_xor(mt, 16));
-                    mt = fmaxf(mt, __shfl_xor(mt, 32));
-                    const float mn = fmaxf(m[nr], mt), mu = mn == -INFINITY ? 0.0f : mn;
-                    if (__any(mn > m[nr])) {
-                        const float alpha = fast_exp2(m[nr] - mu);
-                        l[nr] *= alpha;
-#pragma unroll
-                        for (int i = 0; i < S::ACC; i++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[nr][i][e] *= alpha;
-                        m[nr] = mn;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[nr][e] = fast_exp2(x[nr][e] - mu);
-                        l[nr] += x[nr][e];
-                    }
+                    for (int e = 0; e < E; e++) x[nr][e] = s[nr][e / 4][e % 4];
+                    soften(nr, x[nr], kb, ok, edge);
+                }
+                if constexpr (KH < HT) {
+                    if (tile + KW < last_tile) okm = locate(tile + KW, &units);
                 }
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    if (t == 1) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int c = 0; c < CHUNKS; c++) load_v(4 + i, c, &v[i][c]);
-                    }
+                for (int t = 0; t < HT; t++) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int pos0 = 16 * t + i; // + 4 g
-                        if (edge) {
-                            const bool keep = (ok >> (pos0 + 4 * g)) & 1;
+                        if (VI == 4 && i == 0 && t) {
+#pragma unroll
+                            for (int y = 0; y < 4; y++) load_v(now, 4 * t + y, &v[0][y], VI);
+                        }
+                        if (edge) { // as above
+                            const int pos0 = 16 * t + i; // + 4 g
+                            const bool keep = (ok >> (pos0 + here(4 * g))) & 1;
                             bool is_odd = false;
 #pragma unroll
                             for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
                                 for (int y = 0; y < 4; y++) {
-                                    v[i][c][y] = keep ? v[i][c][y] : 0u;
-                                    is_odd |= odd_f32(v[i][c][y]);
+                                    v[c][(4 * t + i) % VI][y] = keep ? v[c][(4 * t + i) % VI][y] : 0u;
+                                    is_odd |= odd_f32(v[c][(4 * t + i) % VI][y]);
                                 }
                             const uint64_t b = __ballot(is_odd);
                             if (b && tok0 < tok1) {
@@ -489,7 +517,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                                         for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
                                             for (int y = 0; y < 4; y++) {
-                                                const f4 n = mul(g == gg ? v[i][c][y] : 0u,
+                                                const f4 n = mul(g == gg ? v[c][(4 * t + i) % VI][y] : 0u,
                                                                  __float_as_uint(x[nr][4 * t + i]), o[nr][c * 4 + y]);
 #pragma unroll
                                                 for (int z = 0; z < 4; z++)
@@ -501,48 +529,69 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
 #pragma unroll
                                 for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
-                                    for (int y = 0; y < 4; y++) v[i][c][y] = out ? 0u : v[i][c][y];
+                                    for (int y = 0; y < 4; y++) v[c][(4 * t + i) % VI][y] = out ? 0u : v[c][(4 * t + i) % VI][y];
                             }
                         }
 #pragma unroll
-                        for (int nr = 0; nr < NR; nr++)
+                        for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
-                            for (int c = 0; c < CHUNKS; c++)
+                            for (int y = 0; y < 4; y++)
 #pragma unroll
-                                for (int y = 0; y < 4; y++)
-                                    o[nr][c * 4 + y] = mul(v[i][c][y], __float_as_uint(x[nr][4 * t + i]), o[nr][c * 4 + y]);
+                                for (int nr = 0; nr < NR; nr++)
+                                    o[nr][c * 4 + y] = mul(v[c][(4 * t + i) % VI][y], __float_as_uint(x[nr][4 * t + i]), o[nr][c * 4 + y]);
                     }
                 }
             }
         }
 
-        // ---- the four waves' rows joined: each scaled to the common maximum, then added, 64 dimensions a pass
+        // ---- the waves' rows joined: each scaled to the common maximum, then added, 64 dimensions a pass
 #pragma unroll
         for (int nr = 0; nr < NR; nr++) {
             l[nr] += __shfl_xor(l[nr], 16);
             l[nr] += __shfl_xor(l[nr], 32);
             if (g == 0) {
-                ml[(wave * R + 16 * nr + r) * 2] = m[nr];
-                ml[(wave * R + 16 * nr + r) * 2 + 1] = l[nr];
+                ml[(kg * R + 16 * (rg * NR + nr) + r) * 2] = m[nr];
+                ml[(kg * R + 16 * (rg * NR + nr) + r) * 2 + 1] = l[nr];
             }
         }
-        __syncthreads();
+        __syncthreads(); // every wave is past its tiles: q's place is the meeting's now
+        const int th = here(tid);
+        float *const cw = comb + (size_t)(kg * R + 16 * rg * NR + (th & 15)) * S::CROW + 16 * (th >> 4 & 3);
         float mine[NR];
 #pragma unroll
         for (int nr = 0; nr < NR; nr++) {
             float mx = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < WAVES; x++) mx = fmaxf(mx, ml[(x * R + 16 * nr + r) * 2]);
+            for (int x = 0; x < KW; x++) mx = fmaxf(mx, ml[(x * R + 16 * (rg * NR + nr) + (th & 15)) * 2]);
             mine[nr] = fast_exp2(m[nr] - (mx == -INFINITY ? 0.0f : mx));
         }
-        const bool cut = t1 - t0 < sg.cnt;
-        const uint32_t slot = 2 * sh.w + (t0 == 0 ? 1 : 0);
+        const bool cut = sg.t1 - sg.t0 < sg.cnt;
+        const uint32_t slot = 2 * sh.w + (sg.t0 == 0 ? 1 : 0);
+        // this thread's row (+ 16 it) and its values of a pass: the waves' sums, their maximum
+        const int row0 = th >> 4, v0 = (th & 15) * 4;
+        float lt[NT], mx[NT];
+#pragma unroll
+        for (int it = 0; it < NT; it++) {
+            const float *p = ml + (it * 16 + row0) * 2;
+            mx[it] = p[0];
+#pragma unroll
+            for (int x = 1; x < KW; x++) mx[it] = fmaxf(mx[it], p[x * R * 2]);
+            lt[it] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < KW; x++)
+                lt[it] += p[x * R * 2 + 1] * fast_exp2(p[x * R * 2] - (mx[it] == -INFINITY ? 0.0f : mx[it]));
+            if (cut && v0 == 0 && r0 + it * 16 + row0 < n_rows) {
+                float *d = a.part_ml + ((size_t)slot * R + it * 16 + row0) * 2;
+                d[0] = mx[it];
+                d[1] = lt[it];
+            }
+        }
 #pragma unroll
         for (int pass = 0; pass < S::PASSES; pass++) {
             if (pass) __syncthreads();
 #pragma unroll
             for (int nr = 0; nr < NR; nr++) {
-                float *c = comb + (size_t)(wave * R + 16 * nr + r) * S::CROW + 16 * g;
+                float *c = cw + 16 * nr * S::CROW;
                 if constexpr (VB == 4) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -565,37 +614,27 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                 }
             }
             __syncthreads();
+            const int dim = VB == 4 ? 64 * pass + v0
+                                    : 128 * (pass >> 1) + 8 * (4 * (v0 >> 4) + 2 * (pass & 1) + ((v0 >> 3) & 1)) + (v0 & 7);
 #pragma unroll
-            for (int it = 0; it < NR; it++) {
-                const int row = it * 16 + (tid >> 4), v0 = (tid & 15) * 4;
+            for (int it = 0; it < NT; it++) {
+                const int row = it * 16 + row0;
                 const int32_t rr = r0 + row;
-                const int dim = VB == 4 ? 64 * pass + v0
-                                        : 128 * (pass >> 1) + 8 * (4 * (v0 >> 4) + 2 * (pass & 1) + ((v0 >> 3) & 1)) + (v0 & 7);
                 if (rr >= n_rows || dim >= hd) continue;
                 f4 sum = *reinterpret_cast<const f4 *>(comb + (size_t)row * S::CROW + v0);
-                float mx = ml[row * 2];
 #pragma unroll
-                for (int x = 1; x < WAVES; x++) {
+                for (int x = 1; x < KW; x++) {
                     const f4 t = *reinterpret_cast<const f4 *>(comb + (size_t)(x * R + row) * S::CROW + v0);
 #pragma unroll
                     for (int y = 0; y < 4; y++) sum[y] += t[y];
-                    mx = fmaxf(mx, ml[(x * R + row) * 2]);
                 }
-                float lt = 0.0f;
-#pragma unroll
-                for (int x = 0; x < WAVES; x++)
-                    lt += ml[(x * R + row) * 2 + 1] * fast_exp2(ml[(x * R + row) * 2] - (mx == -INFINITY ? 0.0f : mx));
                 if (cut) {
                     *reinterpret_cast<f4 *>(a.part_o + ((size_t)slot * R + row) * D + dim) = sum;
-                    if (dim == 0) {
-                        a.part_ml[((size_t)slot * R + row) * 2] = mx;
-                        a.part_ml[((size_t)slot * R + row) * 2 + 1] = lt;
-                    }
                 } else {
-                    const int32_t tok = rr / G;
+                    const int32_t tok = (int32_t)a.by_g.quot(rr);
                     float out[4];
 #pragma unroll
-                    for (int y = 0; y < 4; y++) out[y] = lt == 0.0f ? 0.0f : sum[y] / lt;
+                    for (int y = 0; y < 4; y++) out[y] = lt[it] == 0.0f ? 0.0f : sum[y] / lt[it];
                     store_out<QT>(a, sr.first + tok, (int)kvh * G + (rr - tok * G), dim, out);
                 }
             }
@@ -604,84 +643,134 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------- the join
-// One work-group per row of a segment: a group of D / 4 threads takes every so many parts, each part's outputs times
-// 2^(its maximum - the running one); the groups meet in the LDS.
-template <int QT>
-__global__ void __launch_bounds__(256) join_kernel(AttnPagedArgs a, int R, int D) {
-    __shared__ f4 os[256];
-    __shared__ float ms[256], ls[256];
-    const uint32_t nkv = (uint32_t)a.kv.nkv, j = blockIdx.x / nkv, kvh = blockIdx.x % nkv;
-    const uint32_t chunk = a.plan[1];
-    if (j >= a.plan[2]) return;
-    const uint32_t p0 = a.plan[PLAN_HEAD + j], cnt = a.plan[PLAN_HEAD + j + 1] - p0;
-    if (cnt == 0) return;
-    const uint32_t s0 = p0 * nkv + kvh * cnt, w0 = s0 / chunk, w1 = (s0 + cnt - 1) / chunk;
+// The rows of one cut segment: segment blockIdx.x of all, or, BY_SHARE, the one that begins in share blockIdx.x and goes on
+// past it (where there are more segments than shares). Threads of a group of D / 4 have four dimensions each; ROWS groups
+// side by side take a row each, and GROUPS of them every so many parts of it, whose outputs, each times 2^(its maximum -
+// the running one), meet in the LDS.
+template <int QT, int THREADS, int D, int GROUPS, bool BY_SHARE>
+__global__ void __launch_bounds__(THREADS) join_kernel(AttnPagedArgs a, int R) {
+    constexpr int QUADS = D / 4, ROWS = THREADS / (QUADS * GROUPS);
+    __shared__ uint32_t found;
+    __shared__ f4 os[GROUPS > 1 ? THREADS : 1];
+    __shared__ float ms[GROUPS > 1 ? THREADS : 1], ls[GROUPS > 1 ? THREADS : 1];
+    const int tid = threadIdx.x;
+    const uint32_t nkv = (uint32_t)a.kv.nkv, total = a.plan[0], chunk = a.plan[1], n_seg = a.plan[2];
+    const uint32_t *line = a.plan + PLAN_HEAD;
+    uint32_t j, kvh, s0, cnt;
+    if constexpr (BY_SHARE) {
+        const uint64_t end64 = (uint64_t)(blockIdx.x + 1) * chunk;
+        if (end64 >= total) return; // the last share, or none
+        const uint32_t end = (uint32_t)end64;
+        if (tid == 0) found = 0xFFFFFFFFu;
+        __syncthreads();
+        for (uint32_t i = tid; i < n_seg; i += THREADS)
+            if (line[i] * nkv < end && end < line[i + 1] * nkv) found = i;
+        __syncthreads();
+        j = found;
+        if (j == 0xFFFFFFFFu) return; // a row tile's first K/V head begins there
+        const uint32_t p0 = line[j];
+        cnt = line[j + 1] - p0;
+        kvh = (end - p0 * nkv) / cnt;
+        s0 = p0 * nkv + kvh * cnt;
+        if (s0 == end || s0 / chunk != blockIdx.x) return; // begins there, or before this share
+    } else {
+        j = blockIdx.x / nkv;
+        kvh = blockIdx.x % nkv;
+        if (j >= n_seg) return;
+        cnt = line[j + 1] - line[j];
+        s0 = line[j] * nkv + kvh * cnt;
+    }
+    const uint32_t w0 = s0 / chunk, w1 = (s0 + cnt - 1) / chunk;
     if (w0 == w1) return; // one share had it all
-    const uint32_t seq = a.planned ? a.seg_seq[j] : j;
-    const int32_t r0 = a.planned ? (int32_t)a.seg_rt[j] * R : 0;
-    const SeqRows sr = paged_seq(a.b, seq);
-    const int row = blockIdx.y;
-    const int32_t rr = r0 + row;
-    if (rr >= sr.n * a.G) return;
-    const int tid = threadIdx.x, quads = D / 4, grp = tid / quads, groups = 256 / quads, dim = tid % quads * 4;
+    const SeqRows sr = paged_seq(a.b, a.seg_seq[j]);
+    const int row = (int)blockIdx.y * ROWS + tid / (QUADS * GROUPS), grp = tid / QUADS % GROUPS, dim = tid % QUADS * 4;
+    const int32_t rr = (int32_t)a.seg_rt[j] * R + row;
+    const bool have = row < R && rr < sr.n * a.G && dim < a.kv.hd;
     float m = -INFINITY, l = 0.0f;
     f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (have) {
 #pragma unroll 4
-    for (uint32_t w = w0 + grp; w <= w1; w += groups) {
-        const size_t at = (size_t)(2 * w + (w == w0 ? 1 : 0)) * R + row;
-        const float pm = a.part_ml[at * 2], pl = a.part_ml[at * 2 + 1];
-        const f4 po = dim < a.kv.hd ? *reinterpret_cast<const f4 *>(a.part_o + at * D + dim) : f4{0.0f, 0.0f, 0.0f, 0.0f};
-        const float mn = fmaxf(m, pm), mu = mn == -INFINITY ? 0.0f : mn;
-        const float x = fast_exp2(m - mu), y = fast_exp2(pm - mu);
-        m = mn;
-        l = l * x + pl * y;
+        for (uint32_t w = w0 + grp; w <= w1; w += GROUPS) {
+            const size_t at = (size_t)(2 * w + (w == w0 ? 1 : 0)) * R + row;
+            const float pm = a.part_ml[at * 2], pl = a.part_ml[at * 2 + 1];
+            const f4 po = *reinterpret_cast<const f4 *>(a.part_o + at * D + dim);
+            const float mn = fmaxf(m, pm), mu = mn == -INFINITY ? 0.0f : mn;
+            const float x = fast_exp2(m - mu), y = fast_exp2(pm - mu);
+            m = mn;
+            l = l * x + pl * y;
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = o[i] * x + po[i] * y;
+            for (int i = 0; i < 4; i++) o[i] = o[i] * x + po[i] * y;
+        }
     }
-    os[tid] = o;
-    ms[tid] = m;
-    ls[tid] = l;
-    __syncthreads();
-    if (grp || dim >= a.kv.hd) return;
-    float mx = m;
-    for (int x = 1; x < groups; x++) mx = fmaxf(mx, ms[x * quads + tid]);
-    const float mu = mx == -INFINITY ? 0.0f : mx;
-    const float x0 = fast_exp2(m - mu);
-    l *= x0;
+    if constexpr (GROUPS > 1) {
+        os[tid] = o;
+        ms[tid] = m;
+        ls[tid] = l;
+        __syncthreads();
+        if (grp) return;
+        float mx = m;
+#pragma unroll 4
+        for (int x = 1; x < GROUPS; x++) mx = fmaxf(mx, ms[x * QUADS + tid]);
+        const float mu = mx == -INFINITY ? 0.0f : mx, x0 = fast_exp2(m - mu);
+        l *= x0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] *= x0;
-    for (int x = 1; x < groups; x++) {
-        const float y = fast_exp2(ms[x * quads + tid] - mu);
-        l += ls[x * quads + tid] * y;
-        const f4 t = os[x * quads + tid];
+        for (int i = 0; i < 4; i++) o[i] *= x0;
+#pragma unroll 4
+        for (int x = 1; x < GROUPS; x++) {
+            const float y = fast_exp2(ms[x * QUADS + tid] - mu);
+            l += ls[x * QUADS + tid] * y;
+            const f4 t = os[x * QUADS + tid];
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] += t[i] * y;
+            for (int i = 0; i < 4; i++) o[i] += t[i] * y;
+        }
     }
+    if (!have) return;
     float out[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) out[i] = l == 0.0f ? 0.0f : o[i] / l;
-    const int32_t tok = rr / a.G;
+    const int32_t tok = (int32_t)a.by_g.quot(rr);
     store_out<QT>(a, sr.first + tok, (int)kvh * a.G + (rr - tok * a.G), dim, out);
 }
 
+// Few rows: a work-group per row, of 1024 threads where a row has many parts (a long context of one sequence has hundreds:
+// 24 rows of 63 parts of 256 dimensions take 5.1 us, with 256 threads 10.4). Many rows: 256 threads, a row per D / 4 of
+// them, its two to a few parts one after the other.
+template <int QT, int D>
+void join_launch(const AttnPagedArgs &a, int R, int rows, hipStream_t stream) {
+    const uint32_t segs = a.n_seg * (uint32_t)a.kv.nkv;
+    if (R > 32) {
+        constexpr int ROWS = 256 / (D / 4);
+        const uint32_t y = (uint32_t)((rows + ROWS - 1) / ROWS);
+        if (segs <= a.shares) join_kernel<QT, 256, D, 1, false><<<dim3(segs, y), 256, 0, stream>>>(a, R);
+        else join_kernel<QT, 256, D, 1, true><<<dim3(a.shares, y), 256, 0, stream>>>(a, R);
+    } else if (segs * 16 <= a.shares) {
+        join_kernel<QT, 1024, D, 1024 / (D / 4), false><<<dim3(segs, (uint32_t)rows), 1024, 0, stream>>>(a, R);
+    } else if (segs <= a.shares) {
+        join_kernel<QT, 256, D, 256 / (D / 4), false><<<dim3(segs, (uint32_t)rows), 256, 0, stream>>>(a, R);
+    } else {
+        join_kernel<QT, 256, D, 256 / (D / 4), true><<<dim3(a.shares, (uint32_t)rows), 256, 0, stream>>>(a, R);
+    }
+}
+template <int QT>
+void join_pick(const AttnPagedArgs &a, int R, int D, int rows, hipStream_t stream) {
+    if (D == 64) join_launch<QT, 64>(a, R, rows, stream);
+    else if (D == 128) join_launch<QT, 128>(a, R, rows, stream);
+    else join_launch<QT, 256>(a, R, rows, stream);
+}
+
 // ---------------------------------------------------------------------------------------------------- the plan
-// Row tiles of all sequences in order, and the prefix sums of their units; one work-group.
+// Of batches of more sequences or row tiles than a work-group divides by itself: all row tiles in order, and the prefix
+// sums of their units; one work-group.
 __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint32_t tk) {
-    __shared__ uint32_t wsum[16], carry;
+    __shared__ uint32_t wsum[16], carry, first[1024];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // the inclusive prefix sum of v over the work-group, plus what came before; uniform calls
     auto scan = [&](uint32_t v) {
-        uint32_t s = v;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t x = __shfl_up(s, d);
-            if (lane >= d) s += x;
-        }
+        uint32_t s = wave_scan(v);
         if (lane == 63) wsum[wave] = s;
         __syncthreads();
-        uint32_t before = carry;
-        for (int i = 0; i < wave; i++) before += wsum[i];
-        s += before;
+        for (int i = 0; i < wave; i++) s += wsum[i];
+        s += carry;
         __syncthreads();
         if (tid == 1023) carry = s;
         __syncthreads();
@@ -689,16 +778,24 @@ __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint
     };
     if (tid == 0) carry = 0;
     __syncthreads();
-    // row tiles: each sequence writes its own
+    // the row tiles of 1024 sequences at a time, each found by its number
     for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 1024) {
-        const uint32_t s = s0 + tid;
-        uint32_t n = 0;
-        if (s < a.b.n_seq) n = (uint32_t)(((int64_t)paged_seq(a.b, s).n * a.G + R - 1) / R);
-        const uint32_t at = scan(n) - n;
-        for (uint32_t i = 0; i < n && at + i < a.n_seg; i++) {
-            a.seg_seq[at + i] = s;
-            a.seg_rt[at + i] = i;
+        const uint32_t from = carry, n = min(seq_tiles(a, s0 + tid, R), a.n_seg);
+        first[tid] = scan(n) - n;
+        __syncthreads();
+        const uint32_t to = min(carry, a.n_seg);
+        for (uint32_t j = from + tid; j < to; j += 1024) {
+            uint32_t lo = 0, hi = min(1024u, a.b.n_seq - s0); // the last sequence that begins at or before j
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (first[mid] <= j) lo = mid;
+                else hi = mid;
+            }
+            a.seg_seq[j] = s0 + lo;
+            a.seg_rt[j] = j - first[lo];
         }
+        __syncthreads();
+        if (carry > a.n_seg) break; // sequences that overlap: not a batch
     }
     const uint32_t n_seg = min(carry, a.n_seg);
     __syncthreads();
@@ -707,11 +804,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint
     for (uint32_t j0 = 0; j0 < n_seg; j0 += 1024) {
         const uint32_t j = j0 + tid;
         uint32_t n = 0;
-        if (j < n_seg) {
-            const UnitRange u = tile_units(paged_seq(a.b, a.seg_seq[j]), a.G, a.window, a.cap,
-                                           (int32_t)a.seg_rt[j] * R, R, tk);
-            n = u.hi - u.lo;
-        }
+        if (j < n_seg) n = tile_count(a, a.seg_seq[j], a.seg_rt[j], R, tk); // its own, or ordered by the barriers above
         const uint32_t end = scan(n);
         if (j < n_seg) a.plan[PLAN_HEAD + j + 1] = end;
     }
@@ -742,15 +835,15 @@ int compute_units(int device) {
 struct Choice {
     bool many = false; // paged_chunk.hip
     int R = 16, D = 64;
-    uint32_t unit = UNIT, shares = 0, min_chunk = 1, n_seg = 0, cap = 0;
+    uint32_t unit = 0, shares = 0, min_chunk = 1, n_seg = 0, cap = 0;
     bool planned = false, join = false;
     PagedSpace space;
 };
 
-template <int CT, bool FQ, int D, int NR>
+template <int CT, bool FQ, int D, int R, bool EXACT>
 int few_launch(const AttnPagedArgs &a, hipStream_t stream) {
-    using S = FewShape<CT, FQ, D, NR>;
-    const auto kernel = few_rows_kernel<CT, FQ, D, NR>;
+    using S = FewShape<CT, FQ, D, R>;
+    const auto kernel = few_rows_kernel<CT, FQ, D, R, EXACT>;
     if constexpr (S::LDS > 56 * 1024) { // with the static arrays past the 64 KiB that need no asking
         static std::atomic<uint64_t> raised{0}; // bit d: done on device d
         int dev = 0;
@@ -764,16 +857,16 @@ int few_launch(const AttnPagedArgs &a, hipStream_t stream) {
     AQ_HIP(hipGetLastError());
     return 0;
 }
+template <int CT, bool FQ, int D>
+int few_rows(const AttnPagedArgs &a, int R, hipStream_t stream) {
+    if (a.kv.hd == D) return R == 16 ? few_launch<CT, FQ, D, 16, true>(a, stream) : few_launch<CT, FQ, D, 32, true>(a, stream);
+    return R == 16 ? few_launch<CT, FQ, D, 16, false>(a, stream) : few_launch<CT, FQ, D, 32, false>(a, stream);
+}
 template <int CT, bool FQ>
 int few_pick(const AttnPagedArgs &a, int D, int R, hipStream_t stream) {
-    if (R == 16) {
-        if (D == 64) return few_launch<CT, FQ, 64, 1>(a, stream);
-        if (D == 128) return few_launch<CT, FQ, 128, 1>(a, stream);
-        return few_launch<CT, FQ, 256, 1>(a, stream);
-    }
-    if (D == 64) return few_launch<CT, FQ, 64, 2>(a, stream);
-    if (D == 128) return few_launch<CT, FQ, 128, 2>(a, stream);
-    return few_launch<CT, FQ, 256, 2>(a, stream);
+    if (D == 64) return few_rows<CT, FQ, 64>(a, R, stream);
+    if (D == 128) return few_rows<CT, FQ, 128>(a, R, stream);
+    return few_rows<CT, FQ, 256>(a, R, stream);
 }
 
 int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uint32_t n_head, bool f32_rows, int device,
@@ -785,17 +878,18 @@ int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uin
     // 16-bit rows past what one pass of the few-row kernel holds
     c->many = !f32_rows && rows > 32;
     c->R = c->many ? CHUNK_ROWS : rows <= 16 ? 16 : 32;
-    c->unit = c->many ? chunk_keys(c->D) : UNIT;
+    c->unit = c->many ? chunk_keys(c->D) : few_unit(kv->type, c->D, c->R);
     c->min_chunk = c->many ? 256 / c->unit : 1;
-    c->planned = rows > (uint64_t)c->R || b->n_seq > INLINE_SEQS;
     // row tiles: a whole one per R rows of all sequences together, and one begun per sequence
-    const uint64_t n_seg = c->planned ? ((uint64_t)b->n_rows * G) / c->R + b->n_seq : b->n_seq;
-    const int cu = compute_units(device);
-    c->shares = (uint32_t)cu * 2;
-    const uint64_t per = (c->cap + c->unit - 1) / c->unit + 1;
+    const uint64_t n_seg = std::min<uint64_t>((uint64_t)b->n_rows * G / c->R + b->n_seq, (uint64_t)b->n_rows * G);
+    c->planned = n_seg > INLINE_TILES || b->n_seq > INLINE_TILES;
+    const uint64_t per = (c->cap + c->unit - 1) / c->unit + 1; // units of a segment at most (a window may begin inside one)
     if ((double)n_seg * (double)per * kv->n_head_kv >= 2147483648.0 || n_seg * kv->n_head_kv >= (1u << 31))
         return fail(AQ_EUNSUP, std::string(call) + ": batch of more than 2^31 units of work");
     c->n_seg = (uint32_t)n_seg;
+    // two work-groups per CU, and no more than there can be units
+    const uint64_t units = n_seg * kv->n_head_kv * per, shares = std::min<uint64_t>((uint64_t)compute_units(device) * 2, units);
+    c->shares = (uint32_t)(shares > 8 ? (shares + 7) / 8 * 8 : std::max<uint64_t>(shares, 1));
     c->join = c->cap > c->unit; // else no segment has a second unit
     c->space = paged_space(c->shares, c->n_seg, (size_t)c->R, (size_t)c->D);
     return 0;
@@ -821,12 +915,11 @@ int launch_paged_plan(const AttnPagedArgs &a, int R, uint32_t tk, hipStream_t st
     return 0;
 }
 
-int launch_paged_combine(const AttnPagedArgs &a, int R, int D, hipStream_t stream) {
-    const dim3 grid(a.n_seg * (uint32_t)a.kv.nkv, (uint32_t)R);
+int launch_paged_combine(const AttnPagedArgs &a, int R, int D, int rows, hipStream_t stream) {
     switch (a.q.type) {
-    case AQ_TYPE_F32: join_kernel<AQ_TYPE_F32><<<grid, 256, 0, stream>>>(a, R, D); break;
-    case AQ_TYPE_F16: join_kernel<AQ_TYPE_F16><<<grid, 256, 0, stream>>>(a, R, D); break;
-    default: join_kernel<AQ_TYPE_BF16><<<grid, 256, 0, stream>>>(a, R, D); break;
+    case AQ_TYPE_F32: join_pick<AQ_TYPE_F32>(a, R, D, rows, stream); break;
+    case AQ_TYPE_F16: join_pick<AQ_TYPE_F16>(a, R, D, rows, stream); break;
+    default: join_pick<AQ_TYPE_BF16>(a, R, D, rows, stream); break;
     }
     AQ_HIP(hipGetLastError());
     return 0;
@@ -882,6 +975,7 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
     if (gate) a.gate = heads_view(gate);
     a.n_head = (int)n_head;
     a.G = (int)(n_head / kv->n_head_kv);
+    a.by_g = FastDiv((uint32_t)a.G);
     a.window = window;
     a.cap = c.cap;
     a.scale_log2 = scale * 1.44269504088896340736f;
@@ -915,7 +1009,7 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
         rc = few_pick<AQ_TYPE_BF16, false>(a, c.D, c.R, st);
     }
     if (rc || !c.join) return rc;
-    return launch_paged_combine(a, c.R, c.D, st);
+    return launch_paged_combine(a, c.R, c.D, (int)std::min<uint64_t>((uint64_t)c.R, (uint64_t)batch->max_rows * a.G), st);
 }
 
 } // extern "C"

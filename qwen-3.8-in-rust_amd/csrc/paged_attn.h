@@ -23,16 +23,17 @@ struct AttnPagedArgs {
     PagedBatch b;
     HeadsView q, out, gate;  // gate.p null: none
     int n_head, G;
+    FastDiv by_g; // rows to tokens
     uint32_t window; // 0: all
     uint32_t cap;    // positions from here on are not attended: the table's reach, or max_len
     float scale_log2;          // scale * log2(e)
     uint32_t q_wide, out_wide; // 16-byte loads of q; 4-value stores of out and loads of gate
     uint32_t shares, min_chunk; // work-groups; least units of a share
-    uint32_t n_seg;   // row tiles of all sequences at most (one per sequence where planned is 0)
-    uint32_t planned; // 1: a plan launch has filled plan, seg_seq, seg_rt; 0: one row tile per sequence
+    uint32_t n_seg;   // row tiles of all sequences at most
+    uint32_t planned; // 1: a plan launch has filled plan, seg_seq, seg_rt; 0: the work-groups divide by themselves
     // workspace
     uint32_t *plan;    // [0] total units (of all K/V heads), [1] chunk, [2] row tiles; then prefix sums of their units
-    uint32_t *seg_seq; // of each row tile: its sequence and its index there (kernels with a plan launch)
+    uint32_t *seg_seq; // of each row tile: its sequence and its index there
     uint32_t *seg_rt;
     float *part_o;  // [2 * shares][R][D]
     float *part_ml; // [2 * shares][R][2]
@@ -44,12 +45,11 @@ constexpr uint32_t PLAN_HEAD = 4;
 struct UnitRange {
     uint32_t lo, hi;
 };
-__device__ __forceinline__ UnitRange tile_units(const SeqRows &sr, int G, uint32_t window, uint32_t cap, int32_t r0,
-                                                int32_t R, uint32_t tk) {
-    const int32_t last = min(r0 + R, sr.n * G) - 1;
-    const int32_t t0 = r0 / G, t1 = last / G, base = sr.len - sr.n; // row tokens' positions are base + token
-    const int32_t end = min(max(base + t1 + 1, 0), (int32_t)cap);
-    const int64_t begin = window ? max((int64_t)base + t0 + 1 - (int64_t)window, (int64_t)0) : 0;
+__device__ __forceinline__ UnitRange tile_units(const AttnPagedArgs &a, const SeqRows &sr, int32_t r0, int32_t R, uint32_t tk) {
+    const int32_t last = min(r0 + R, sr.n * a.G) - 1;
+    const int32_t t0 = (int32_t)a.by_g.quot(r0), t1 = (int32_t)a.by_g.quot(last), base = sr.len - sr.n; // row tokens' positions are base + token
+    const int32_t end = min(max(base + t1 + 1, 0), (int32_t)a.cap);
+    const int64_t begin = a.window ? max((int64_t)base + t0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
     UnitRange u;
     u.lo = (uint32_t)begin / tk;
     u.hi = ((uint32_t)end + tk - 1) / tk;
@@ -71,84 +71,146 @@ __device__ __forceinline__ int here(int x) {
     return x;
 }
 
-constexpr int INLINE_SEQS = 1024; // sequences that a work-group of 256 divides by itself
+constexpr int INLINE_TILES = 1024; // sequences, and row tiles, that a work-group of 256 divides by itself
+
+// The plan in a work-group's LDS: of each row tile its sequence, of each sequence its first row tile, and the prefix sums
+// of the row tiles' units.
+struct PlanLds {
+    uint32_t pre[INLINE_TILES + 1], first[INLINE_TILES + 1], seq[INLINE_TILES], wsum[4], found;
+};
 
 // A work-group's share of the line: its number, its units begin .. end - 1 (none: begin == end), the row tile that
-// begin lies in. pre (INLINE_SEQS + 1), wsum (4) and found are the work-group's.
+// begin lies in.
 struct Share {
-    uint32_t w, begin, end, n_seg, j;
+    uint32_t w, begin, end, j;
 };
-__device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint32_t tk, uint32_t *pre, uint32_t *wsum,
-                                            uint32_t *found) {
-    constexpr int PER = INLINE_SEQS / 256;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+
+// Inclusive prefix sums over a wave, and over a work-group of 256 (wsum: 4 words; two barriers).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lanes = 64) { // the first `lanes` lanes'
+    const int lane = threadIdx.x & 63;
+    for (int d = 1; d < lanes; d *= 2) {
+        const uint32_t x = __shfl_up(v, d);
+        if (lane >= d) v += x;
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t *wsum) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v = wave_scan(v);
+    __syncthreads(); // the last call's sums are read
+    if (lane == 63) wsum[wave] = v;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) v += wsum[w];
+    return v;
+}
+
+__device__ __forceinline__ uint32_t seq_tiles(const AttnPagedArgs &a, uint32_t s, int R) {
+    return s < a.b.n_seq ? (uint32_t)((paged_seq(a.b, s).n * a.G + R - 1) / R) : 0u;
+}
+__device__ __forceinline__ uint32_t tile_count(const AttnPagedArgs &a, uint32_t s, uint32_t rt, int R, uint32_t tk) {
+    const UnitRange u = tile_units(a, paged_seq(a.b, s), (int32_t)rt * R, R, tk);
+    return u.hi - u.lo;
+}
+
+__device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint32_t tk, PlanLds &lds) {
+    const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t nkv = (uint32_t)a.kv.nkv;
-    uint32_t total, chunk;
     Share sh;
+    // neighbouring shares on one XCD: work-groups go round the 8 XCDs, and neighbours read the same pages' lines
+    sh.w = a.shares % 8 ? blockIdx.x : (blockIdx.x % 8) * (a.shares / 8) + blockIdx.x / 8;
+    sh.begin = sh.end = sh.j = 0;
+    uint32_t total, chunk, n_seg;
+    bool one_wave = false;
     if (a.planned) {
         total = a.plan[0];
         chunk = a.plan[1];
-        sh.n_seg = a.plan[2];
+        n_seg = a.plan[2];
     } else {
-        sh.n_seg = a.b.n_seq;
-        uint32_t mine[PER], sum = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const uint32_t s = (uint32_t)tid * PER + i;
-            mine[i] = 0;
-            if (s < sh.n_seg) {
-                const SeqRows sr = paged_seq(a.b, s);
-                if (sr.n > 0) {
-                    const UnitRange u = tile_units(sr, a.G, a.window, a.cap, 0, R, tk);
-                    mine[i] = u.hi - u.lo;
-                }
+        // Few: every wave for itself, without a barrier (all write the same words).
+        uint32_t cnt = 0, incl = 0;
+        if (a.b.n_seq <= 64) {
+            cnt = min(seq_tiles(a, lane, R), 65u);
+            incl = wave_scan(cnt, (int)a.b.n_seq);
+            n_seg = __builtin_amdgcn_readlane(incl, a.b.n_seq - 1);
+            one_wave = n_seg <= min(64u, a.n_seg);
+        }
+        if (one_wave) {
+            lds.first[lane] = incl - cnt;
+            for (uint32_t i = 0; i < cnt; i++) lds.seq[incl - cnt + i] = lane;
+            __builtin_amdgcn_wave_barrier();
+            uint32_t units = 0;
+            if ((uint32_t)lane < n_seg) {
+                const uint32_t s = lds.seq[lane];
+                units = tile_count(a, s, lane - lds.first[s], R, tk);
             }
-            sum += mine[i];
-        }
-        uint32_t scan = sum;
+            const uint32_t sum = wave_scan(units, (int)n_seg);
+            if (lane == 0) lds.pre[0] = 0;
+            lds.pre[lane + 1] = sum;
+            total = n_seg ? (uint32_t)__builtin_amdgcn_readlane(sum, n_seg - 1) * nkv : 0u;
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            constexpr int PER = INLINE_TILES / 256;
+            uint32_t mine[PER], sum = 0;
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t v = __shfl_up(scan, d);
-            if (lane >= d) scan += v;
-        }
-        if (lane == 63) wsum[wave] = scan;
-        __syncthreads();
-        uint32_t before = scan - sum;
-        for (int w = 0; w < wave; w++) before += wsum[w];
-        if (tid == 0) pre[0] = 0;
+            for (int i = 0; i < PER; i++) sum += mine[i] = min(seq_tiles(a, tid * PER + i, R), (uint32_t)INLINE_TILES);
+            uint32_t at = group_scan(sum, lds.wsum) - sum;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            before += mine[i];
-            pre[tid * PER + i + 1] = before;
+            for (int i = 0; i < PER; i++) {
+                lds.first[tid * PER + i] = at;
+                for (uint32_t k = 0; k < mine[i] && at + k < (uint32_t)INLINE_TILES; k++) lds.seq[at + k] = tid * PER + i;
+                at += mine[i];
+            }
+            if (tid == 255) lds.first[INLINE_TILES] = at;
+            __syncthreads();
+            n_seg = min(min(lds.first[INLINE_TILES], (uint32_t)INLINE_TILES), a.n_seg);
+            sum = 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const uint32_t j = tid * PER + i;
+                mine[i] = 0;
+                if (j < n_seg) mine[i] = tile_count(a, lds.seq[j], j - lds.first[lds.seq[j]], R, tk);
+                sum += mine[i];
+            }
+            at = group_scan(sum, lds.wsum) - sum;
+            if (tid == 0) lds.pre[0] = 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                at += mine[i];
+                lds.pre[tid * PER + i + 1] = at;
+            }
+            __syncthreads();
+            total = lds.pre[n_seg] * nkv;
         }
-        __syncthreads();
-        total = pre[sh.n_seg] * nkv;
         chunk = share_chunk(total, a.shares, a.min_chunk);
         if (blockIdx.x == 0) { // for the join
             if (tid == 0) {
                 a.plan[0] = total;
                 a.plan[1] = chunk;
-                a.plan[2] = sh.n_seg;
+                a.plan[2] = n_seg;
+                a.plan[PLAN_HEAD] = 0;
             }
-            for (uint32_t s = tid; s <= sh.n_seg; s += 256) a.plan[PLAN_HEAD + s] = pre[s];
+            for (uint32_t j = tid; j < n_seg; j += 256) {
+                a.plan[PLAN_HEAD + j + 1] = lds.pre[j + 1];
+                a.seg_seq[j] = lds.seq[j];
+                a.seg_rt[j] = j - lds.first[lds.seq[j]];
+            }
         }
     }
-    // neighbouring shares on one XCD: work-groups go round the 8 XCDs, and neighbours read the same pages' lines
-    sh.w = a.shares % 8 ? blockIdx.x : (blockIdx.x % 8) * (a.shares / 8) + blockIdx.x / 8;
     const uint64_t first = (uint64_t)sh.w * chunk;
-    if (first >= total) {
-        sh.begin = sh.end = sh.j = 0;
-        return sh;
-    }
+    if (first >= total) return sh;
     sh.begin = (uint32_t)first;
     sh.end = min(total, sh.begin + chunk);
-    // the only row tile that begins at or before it and ends after it
-    for (uint32_t j = tid; j < sh.n_seg; j += 256) {
-        const uint32_t p0 = a.planned ? a.plan[PLAN_HEAD + j] : pre[j], p1 = a.planned ? a.plan[PLAN_HEAD + j + 1] : pre[j + 1];
-        if (p0 * nkv <= sh.begin && sh.begin < p1 * nkv) *found = j;
+    // the row tile that the share begins in: the only one that begins at or before it and ends after it
+    if (one_wave) {
+        const bool in = (uint32_t)lane < n_seg && lds.pre[lane] * nkv <= sh.begin && sh.begin < lds.pre[lane + 1] * nkv;
+        sh.j = (uint32_t)__builtin_ctzll(__ballot(in));
+    } else {
+        const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : lds.pre;
+        for (uint32_t j = tid; j < n_seg; j += 256)
+            if (line[j] * nkv <= sh.begin && sh.begin < line[j + 1] * nkv) lds.found = j;
+        __syncthreads();
+        sh.j = lds.found;
     }
-    __syncthreads();
-    sh.j = *found;
     return sh;
 }
 
@@ -158,12 +220,12 @@ struct Segment {
     uint32_t kvh, seq, t0, t1, cnt;
     int32_t r0;
 };
-__device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, const uint32_t *pre, const Share &sh,
+__device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, const PlanLds &lds, const Share &sh,
                                                 uint32_t &u, uint32_t &j) {
     const uint32_t nkv = (uint32_t)a.kv.nkv;
-    const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : pre;
+    const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : lds.pre;
     uint32_t p0 = line[j], p1 = line[j + 1];
-    while (p1 * nkv <= u) { // row tiles without units
+    if (p1 * nkv <= u) { // every row tile has units
         j++;
         p0 = p1;
         p1 = line[j + 1];
@@ -175,8 +237,8 @@ __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, c
     s.t0 = rel - s.kvh * s.cnt;
     s.t1 = min(s.cnt, s.t0 + (sh.end - u));
     u += s.t1 - s.t0;
-    s.seq = a.planned ? a.seg_seq[j] : j;
-    s.r0 = a.planned ? (int32_t)a.seg_rt[j] * R : 0;
+    s.seq = a.planned ? a.seg_seq[j] : lds.seq[j];
+    s.r0 = (int32_t)(a.planned ? a.seg_rt[j] : j - lds.first[s.seq]) * R;
     return s;
 }
 
@@ -253,7 +315,7 @@ inline PagedSpace paged_space(size_t shares, size_t n_seg, size_t R, size_t D) {
 
 int launch_paged_plan(const AttnPagedArgs &a, int R, uint32_t tk, hipStream_t stream);
 int launch_paged_chunk(const AttnPagedArgs &a, int D, hipStream_t stream); // 16-bit rows and cache
-int launch_paged_combine(const AttnPagedArgs &a, int R, int D, hipStream_t stream);
+int launch_paged_combine(const AttnPagedArgs &a, int R, int D, int rows, hipStream_t stream);
 
 constexpr int CHUNK_ROWS = 128;                                   // paged_chunk.hip's row tile
 constexpr int chunk_keys(int D) { return D == 256 ? 32 : 64; } // and its unit

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
     constexpr int R = CHUNK_ROWS, KEYS = S::KEYS, HALVES = S::HALVES, STEPS = D / 16, DB = D / 32;
     constexpr float P_SHIFT = CT == AQ_TYPE_F16 ? 7.0f : 0.0f, GROW = 7.0f;
     extern __shared__ __align__(16) char smem[];
-    __shared__ uint32_t pre[INLINE_SEQS + 1], wsum[4], found;
+    __shared__ PlanLds plan;
     char *kbuf = smem, *vbuf = smem + 2 * S::TILE_BYTES;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -86,28 +86,28 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
     const int kaddr0 = n0 * S::RB + ((h0 ^ S::swizzle(n0)) << 4);
     const int vaddr0 = vkey * S::RB + (((2 * ((lane >> 4) & 1) + (vi % 4) / 2) ^ S::swizzle(vkey)) << 4) + (vi % 2) * 8;
 
-    const Share sh = take_share(a, R, KEYS, pre, wsum, &found);
+    const Share sh = take_share(a, R, KEYS, plan);
     uint32_t u = sh.begin, j = sh.j;
     while (u < sh.end) { // uniform
-        const Segment sg = next_segment(a, R, pre, sh, u, j);
+        const Segment sg = next_segment(a, R, plan, sh, u, j);
         const int n = here(n0), h = here(h0);
         const SeqRows sr = paged_seq(a.b, sg.seq);
         const int32_t n_rows = sr.n * G, base = sr.len - sr.n;
-        const UnitRange range = tile_units(sr, G, a.window, a.cap, sg.r0, R, KEYS);
+        const UnitRange range = tile_units(a, sr, sg.r0, R, KEYS);
         const int32_t *table = a.b.pages + (size_t)sg.seq * a.b.max_pages;
         const uint64_t head_off = (uint64_t)sg.kvh * a.kv.head_bytes;
-        const int32_t seg_last = (min(sg.r0 + R, n_rows) - 1) / G;
+        const int32_t seg_last = (int32_t)a.by_g.quot(min(sg.r0 + R, n_rows) - 1);
         const int32_t kend = min(max(base + seg_last + 1, 0), (int32_t)a.cap); // positions from here on: nobody's
 
         // this lane's row, and what the wave's rows see between them
-        const int32_t rr = sg.r0 + 32 * wave + n, tok = rr / G;
+        const int32_t rr = sg.r0 + 32 * wave + n, tok = (int32_t)a.by_g.quot(rr);
         const bool have = rr < n_rows;
         const int32_t hi = have ? base + tok + 1 : 0;
         const int64_t lo64 = a.window ? (int64_t)base + tok + 1 - (int64_t)a.window : 0;
         const int32_t lo = lo64 > 0 ? (int32_t)lo64 : 0;
         const int32_t w0 = sg.r0 + 32 * wave, w1 = min(w0 + 32, n_rows) - 1;
         const bool idle = w0 >= n_rows; // a wave without rows only loads
-        const int32_t tok0 = w0 / G, tok1 = idle ? tok0 : w1 / G;
+        const int32_t tok0 = (int32_t)a.by_g.quot(w0), tok1 = idle ? tok0 : (int32_t)a.by_g.quot(w1);
         const int32_t min_hi = base + tok0 + 1, max_hi = idle ? 0 : base + tok1 + 1;
         const int64_t min_lo = a.window ? (int64_t)base + tok0 + 1 - (int64_t)a.window : INT64_MIN,
                       max_lo = a.window ? (int64_t)base + tok1 + 1 - (int64_t)a.window : INT64_MIN;

@@ -175,7 +175,8 @@ def test_attention(ctx):
     need = aq.paged_attention_workspace(ctx, good_kv(), good_batch(), 4)
     assert need > 0
     go(f"{need} needed", size=need - 1)
-    go("2^31 units", batch=good_batch(n_seq=1 << 23, max_pages=1 << 23, max_len=(1 << 27) - 1), code=aq.AQ_EUNSUP)
+    go("2^31 units", batch=good_batch(n_seq=1 << 23, n_rows=1 << 23, max_pages=1 << 23, max_len=(1 << 27) - 1),
+       code=aq.AQ_EUNSUP)
     aq.paged_attention(ctx, good_kv(), good_batch(n_rows=0), 4, rows(heads=4), rows(heads=4), 0.1)  # nothing to do
     assert aq.lib().aq_paged_attention(None, *[None] * 2, 4, None, None, 0.1, 0, None, None, 0, None) == aq.AQ_EINVAL
     assert aq.lib().aq_paged_attention_workspace(ctx.h, C.byref(good_kv()), C.byref(good_batch()), 4, None) == aq.AQ_EINVAL
