@@ -6,25 +6,16 @@
 
 namespace aq {
 
-// n / d and n % d for positions (n < 2^31): pages of a power of two by shifting, others by a 32-bit reciprocal:
-// m = ceil(2^(31 + k) / d) with 2^(k-1) < d <= 2^k exceeds 2^(31+k) / d by less than 1, so floor(n m / 2^(31+k)) is
-// exact for n < 2^31.
+// n / d for n < 2^31: m = ceil(2^(31 + k) / d) with 2^(k-1) < d <= 2^k exceeds 2^(31+k) / d by less than 1, so
+// floor(n m / 2^(31+k)) is exact.
 struct FastDiv {
-    uint32_t d = 1, mul = 0, shift = 0;
+    uint32_t d = 1, mul = 1u << 31, shift = 0;
     FastDiv() = default;
     explicit FastDiv(uint32_t div) : d(div) {
-        uint32_t k = 0;
-        while ((1ull << k) < div) k++;
-        if ((1ull << k) == div) {
-            shift = k; // mul 0: a shift
-        } else {
-            mul = (uint32_t)(((1ull << (31 + k)) + div - 1) / div);
-            shift = k - 1;
-        }
+        while ((1ull << shift) < div) shift++;
+        mul = (uint32_t)(((1ull << (31 + shift)) + div - 1) / div);
     }
-    __host__ __device__ uint32_t quot(uint32_t n) const {
-        return mul ? (uint32_t)(((uint64_t)n * mul) >> 32) >> shift : n >> shift;
-    }
+    __host__ __device__ uint32_t quot(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> 31) >> shift; }
 };
 
 // The cache: K and V rows at base + ((page * page_units + slot * slot_units) << unit_shift) bytes, then the head.

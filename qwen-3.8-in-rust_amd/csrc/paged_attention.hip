@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
     uint32_t u = sh.begin, j = sh.j;
     while (u < sh.end) { // uniform
         const Segment sg = next_segment(a, R, plan, sh, u, j);
+        if (sg.t1 <= sg.t0) continue;
         const uint32_t kvh = sg.kvh;
         const int32_t r0 = sg.r0;
         const SeqRows sr = paged_seq(a.b, sg.seq);
@@ -565,8 +566,8 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             for (int x = 0; x < KW; x++) mx = fmaxf(mx, ml[(x * R + 16 * (rg * NR + nr) + (th & 15)) * 2]);
             mine[nr] = fast_exp2(m[nr] - (mx == -INFINITY ? 0.0f : mx));
         }
-        const bool cut = sg.t1 - sg.t0 < sg.cnt;
-        const uint32_t slot = 2 * sh.w + (sg.t0 == 0 ? 1 : 0);
+        const bool cut = is_cut(sg);
+        const uint32_t slot = part_slot(sg, sh);
         // this thread's row (+ 16 it) and its values of a pass: the waves' sums, their maximum
         const int row0 = th >> 4, v0 = (th & 15) * 4;
         float lt[NT], mx[NT];
@@ -668,17 +669,18 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnPagedArgs a, int R) {
         __syncthreads();
         j = found;
         if (j == 0xFFFFFFFFu) return; // a row tile's first K/V head begins there
-        const uint32_t p0 = line[j];
-        cnt = line[j + 1] - p0;
-        kvh = (end - p0 * nkv) / cnt;
-        s0 = p0 * nkv + kvh * cnt;
-        if (s0 == end || s0 / chunk != blockIdx.x) return; // begins there, or before this share
+        const uint32_t p0 = line[j], places = line[j + 1] - p0;
+        kvh = (end - p0 * nkv) / places;
+        s0 = p0 * nkv + kvh * places + a.lead; // the first unit's place
+        cnt = places - a.lead;
+        if (s0 >= end || s0 / chunk != blockIdx.x) return; // begins there, or before this share
     } else {
         j = blockIdx.x / nkv;
         kvh = blockIdx.x % nkv;
         if (j >= n_seg) return;
-        cnt = line[j + 1] - line[j];
-        s0 = line[j] * nkv + kvh * cnt;
+        const uint32_t p0 = line[j], places = line[j + 1] - p0;
+        s0 = p0 * nkv + kvh * places + a.lead;
+        cnt = places - a.lead;
     }
     const uint32_t w0 = s0 / chunk, w1 = (s0 + cnt - 1) / chunk;
     if (w0 == w1) return; // one share had it all
@@ -835,7 +837,7 @@ int compute_units(int device) {
 struct Choice {
     bool many = false; // paged_chunk.hip
     int R = 16, D = 64;
-    uint32_t unit = 0, shares = 0, min_chunk = 1, n_seg = 0, cap = 0;
+    uint32_t unit = 0, shares = 0, min_chunk = 1, lead = 0, n_seg = 0, cap = 0;
     bool planned = false, join = false;
     PagedSpace space;
 };
@@ -880,10 +882,12 @@ int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uin
     c->R = c->many ? CHUNK_ROWS : rows <= 16 ? 16 : 32;
     c->unit = c->many ? chunk_keys(c->D) : few_unit(kv->type, c->D, c->R);
     c->min_chunk = c->many ? 256 / c->unit : 1;
+    c->lead = c->many ? 192 / c->unit : 0;
     // row tiles: a whole one per R rows of all sequences together, and one begun per sequence
     const uint64_t n_seg = std::min<uint64_t>((uint64_t)b->n_rows * G / c->R + b->n_seq, (uint64_t)b->n_rows * G);
     c->planned = n_seg > INLINE_TILES || b->n_seq > INLINE_TILES;
-    const uint64_t per = (c->cap + c->unit - 1) / c->unit + 1; // units of a segment at most (a window may begin inside one)
+    // places of a segment at most (a window may begin inside a unit)
+    const uint64_t per = (c->cap + c->unit - 1) / c->unit + 1 + c->lead;
     if ((double)n_seg * (double)per * kv->n_head_kv >= 2147483648.0 || n_seg * kv->n_head_kv >= (1u << 31))
         return fail(AQ_EUNSUP, std::string(call) + ": batch of more than 2^31 units of work");
     c->n_seg = (uint32_t)n_seg;
@@ -983,6 +987,7 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
     a.out_wide = heads_aligned(out, rows, n_head) && (!gate || heads_aligned(gate, rows, n_head));
     a.shares = c.shares;
     a.min_chunk = c.min_chunk;
+    a.lead = c.lead;
     a.n_seg = c.n_seg;
     a.planned = c.planned;
     char *ws = (char *)workspace;

@@ -6,8 +6,9 @@
 // head; its keys are counted in units of TK positions from position 0, and only the units that some row of the tile
 // sees are work.
 //
-// Split. All segments' units in order (sequence, row tile, K/V head, key unit) form one line of `total` units, cut into
-// work-group shares of `chunk` units each, however long or short the sequences are. A share that holds a whole segment
+// Split. All segments' units in order (sequence, row tile, K/V head, key unit), each segment's with `lead` places before
+// them for what a segment costs besides its units, form one line of `total` places, cut into work-group shares of `chunk`
+// places each, however long or short the sequences are. A share that holds a whole segment
 // writes its output; where a segment is cut, each share writes its part (row maxima, sums and unnormalised outputs, in
 // f32) to the workspace, slot 2w for the segment that began before share w, slot 2w + 1 for the one that goes on after
 // it, and a second launch joins the parts in order. Which share has which part follows from the lengths alone, so the
@@ -28,11 +29,11 @@ struct AttnPagedArgs {
     uint32_t cap;    // positions from here on are not attended: the table's reach, or max_len
     float scale_log2;          // scale * log2(e)
     uint32_t q_wide, out_wide; // 16-byte loads of q; 4-value stores of out and loads of gate
-    uint32_t shares, min_chunk; // work-groups; least units of a share
+    uint32_t shares, min_chunk, lead; // work-groups; least places of a share; places before a segment's units
     uint32_t n_seg;   // row tiles of all sequences at most
     uint32_t planned; // 1: a plan launch has filled plan, seg_seq, seg_rt; 0: the work-groups divide by themselves
     // workspace
-    uint32_t *plan;    // [0] total units (of all K/V heads), [1] chunk, [2] row tiles; then prefix sums of their units
+    uint32_t *plan;    // [0] total places (of all K/V heads), [1] chunk, [2] row tiles; then prefix sums of their places
     uint32_t *seg_seq; // of each row tile: its sequence and its index there
     uint32_t *seg_rt;
     float *part_o;  // [2 * shares][R][D]
@@ -71,15 +72,18 @@ __device__ __forceinline__ int here(int x) {
     return x;
 }
 
+// x, which all lanes have: in a scalar register.
+__device__ __forceinline__ uint32_t same(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+
 constexpr int INLINE_TILES = 1024; // sequences, and row tiles, that a work-group of 256 divides by itself
 
 // The plan in a work-group's LDS: of each row tile its sequence, of each sequence its first row tile, and the prefix sums
-// of the row tiles' units.
+// of the row tiles' places.
 struct PlanLds {
     uint32_t pre[INLINE_TILES + 1], first[INLINE_TILES + 1], seq[INLINE_TILES], wsum[4], found;
 };
 
-// A work-group's share of the line: its number, its units begin .. end - 1 (none: begin == end), the row tile that
+// A work-group's share of the line: its number, its places begin .. end - 1 (none: begin == end), the row tile that
 // begin lies in.
 struct Share {
     uint32_t w, begin, end, j;
@@ -109,7 +113,7 @@ __device__ __forceinline__ uint32_t seq_tiles(const AttnPagedArgs &a, uint32_t s
 }
 __device__ __forceinline__ uint32_t tile_count(const AttnPagedArgs &a, uint32_t s, uint32_t rt, int R, uint32_t tk) {
     const UnitRange u = tile_units(a, paged_seq(a.b, s), (int32_t)rt * R, R, tk);
-    return u.hi - u.lo;
+    return u.hi - u.lo + a.lead;
 }
 
 __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint32_t tk, PlanLds &lds) {
@@ -179,7 +183,8 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
                 lds.pre[tid * PER + i + 1] = at;
             }
             __syncthreads();
-            total = lds.pre[n_seg] * nkv;
+            n_seg = same(n_seg);
+            total = same(lds.pre[n_seg]) * nkv;
         }
         chunk = share_chunk(total, a.shares, a.min_chunk);
         if (blockIdx.x == 0) { // for the join
@@ -209,38 +214,42 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
         for (uint32_t j = tid; j < n_seg; j += 256)
             if (line[j] * nkv <= sh.begin && sh.begin < line[j + 1] * nkv) lds.found = j;
         __syncthreads();
-        sh.j = lds.found;
+        sh.j = same(lds.found);
     }
     return sh;
 }
 
-// The next segment of a share, from unit u on: K/V head, the sequence, its first row, the units t0 .. t1 - 1 of the
-// segment's cnt that are the share's. Advances u and j.
+// The next segment of a share, from place u on: K/V head, the sequence, its first row, the units t0 .. t1 - 1 of the
+// segment's cnt that are the share's (none: t1 <= t0). Advances u and j. All uniform.
 struct Segment {
-    uint32_t kvh, seq, t0, t1, cnt;
-    int32_t r0;
+    uint32_t kvh, seq, cnt;
+    int32_t t0, t1, r0;
 };
 __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, const PlanLds &lds, const Share &sh,
                                                 uint32_t &u, uint32_t &j) {
     const uint32_t nkv = (uint32_t)a.kv.nkv;
     const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : lds.pre;
-    uint32_t p0 = line[j], p1 = line[j + 1];
+    uint32_t p0 = same(line[j]), p1 = same(line[j + 1]);
     if (p1 * nkv <= u) { // every row tile has units
         j++;
         p0 = p1;
-        p1 = line[j + 1];
+        p1 = same(line[j + 1]);
     }
     Segment s;
-    s.cnt = p1 - p0;
-    const uint32_t rel = u - p0 * nkv;
-    s.kvh = rel / s.cnt;
-    s.t0 = rel - s.kvh * s.cnt;
-    s.t1 = min(s.cnt, s.t0 + (sh.end - u));
-    u += s.t1 - s.t0;
-    s.seq = a.planned ? a.seg_seq[j] : lds.seq[j];
-    s.r0 = (int32_t)(a.planned ? a.seg_rt[j] : j - lds.first[s.seq]) * R;
+    const uint32_t places = p1 - p0, rel = u - p0 * nkv;
+    s.kvh = rel / places;
+    const uint32_t from = rel - s.kvh * places, to = min(places, from + (sh.end - u));
+    s.cnt = places - a.lead;
+    s.t0 = max((int32_t)(from - a.lead), 0);
+    s.t1 = (int32_t)(to - a.lead);
+    u += to - from;
+    s.seq = same(a.planned ? a.seg_seq[j] : lds.seq[j]);
+    s.r0 = (int32_t)same(a.planned ? a.seg_rt[j] : j - lds.first[s.seq]) * R;
     return s;
 }
+// Whether other shares have units of it too, and then the slot of this share's part.
+__device__ __forceinline__ bool is_cut(const Segment &s) { return s.t1 - s.t0 < (int32_t)s.cnt; }
+__device__ __forceinline__ uint32_t part_slot(const Segment &s, const Share &sh) { return 2 * sh.w + (s.t0 == 0 ? 1 : 0); }
 
 // N consecutive values of a row as f32, of which `have` exist (the others 0).
 template <int QT, int N>

@@ -61,8 +61,9 @@ struct ChunkShape {
     static constexpr int TILE_BYTES = KEYS * RB;
     static constexpr int LOADS = TILE_BYTES / (256 * 16);     // 16-byte loads per thread and tile, of K and of V
     static constexpr int LDS = 4 * TILE_BYTES;                // two buffers of each
-    // which chunk of row r lies at place p: p ^ swizzle(r)
-    static __device__ __forceinline__ int swizzle(int r) { return D == 64 ? ((r >> 1) & 3) << 1 : (r & 7) << 1; }
+    // which chunk of row r lies at place p: p ^ swizzle(r). Eight neighbouring rows have all eight values (K operands: 16
+    // bytes of each of eight rows a clock), four have their upper bits apart (V: 32 bytes of each of four rows).
+    static __device__ __forceinline__ uint32_t swizzle(uint32_t r) { return (r & 3) << 1 | (r >> 2 & 1); }
 };
 
 #define AQ_LDS __attribute__((address_space(3)))
@@ -83,13 +84,14 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
     // LDS addresses of this lane's reads of K (operand step 0) and V (dimensions 0 .. 31); the other steps by an exclusive
     // or, rows and chunks from 16 on by constant offsets
     const int n0 = lane & 31, h0 = lane >> 5, vi = lane & 15, vkey = 4 * h0 + vi / 4;
-    const int kaddr0 = n0 * S::RB + ((h0 ^ S::swizzle(n0)) << 4);
-    const int vaddr0 = vkey * S::RB + (((2 * ((lane >> 4) & 1) + (vi % 4) / 2) ^ S::swizzle(vkey)) << 4) + (vi % 2) * 8;
+    const int kaddr0 = n0 * S::RB + (int)((h0 ^ S::swizzle(n0)) << 4);
+    const int vaddr0 = vkey * S::RB + (int)(((2 * ((lane >> 4) & 1) + (vi % 4) / 2) ^ S::swizzle(vkey)) << 4) + (vi % 2) * 8;
 
     const Share sh = take_share(a, R, KEYS, plan);
     uint32_t u = sh.begin, j = sh.j;
     while (u < sh.end) { // uniform
         const Segment sg = next_segment(a, R, plan, sh, u, j);
+        if (sg.t1 <= sg.t0) continue;
         const int n = here(n0), h = here(h0);
         const SeqRows sr = paged_seq(a.b, sg.seq);
         const int32_t n_rows = sr.n * G, base = sr.len - sr.n;
@@ -122,17 +124,20 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
         };
         const char *const kpool = a.kv.k + head_off, *const vpool = a.kv.v + head_off;
         auto load_tile = [&](uint32_t units, uint64_t ok, int buf) {
-            const int ln = here(lane), last = hd / 8 - 1;
+            constexpr uint32_t RPI = 64 / S::CPR; // rows of one wave's load
+            const uint32_t ln = (uint32_t)here(lane), rl = ln / S::CPR, place = ln % S::CPR;
+            const uint32_t last = (uint32_t)hd / 8 - 1, row0 = wave * S::LOADS * RPI + rl;
             char *kd = kbuf + buf * S::TILE_BYTES + wave * S::LOADS * 1024, *vd = vbuf + (kd - kbuf);
 #pragma unroll
-            for (int i = 0; i < S::LOADS; i++) {
-                const int at = i * 64 + ln, row = wave * (S::LOADS * 64 / S::CPR) + at / S::CPR, place = at % S::CPR;
-                // past the head: the queries are 0 there, the outputs not stored
-                const uint32_t c = (uint32_t)min(place ^ S::swizzle(row), last);
-                const uint64_t off = ((uint64_t)(uint32_t)__shfl((int)units, row) << a.kv.unit_shift) + c * 16;
+            for (uint32_t i = 0; i < S::LOADS; i++) {
+                // the row's low three bits: rl and, above them, i's
+                uint32_t c = place ^ S::swizzle((i * RPI & 7) + rl);
+                if (D != hd) c = min(c, last); // past the head: the queries are 0 there, the outputs not stored
+                const uint32_t un = (uint32_t)__builtin_amdgcn_ds_bpermute((int)((row0 + i * RPI) * 4), (int)units);
+                const uint64_t off = ((uint64_t)un << a.kv.unit_shift) + c * 16;
                 const char *kp = kpool + off, *vp = vpool + off;
                 if (ok != ALL) { // uniform
-                    const bool has = (ok >> row) & 1;
+                    const bool has = (ok >> (row0 + i * RPI)) & 1;
                     kp = has ? kp : (const char *)&zeros;
                     vp = has ? vp : (const char *)&zeros;
                 }
@@ -282,8 +287,21 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                     }
                     return x;
                 };
-                uint64_t odd = 0; // positions whose V row holds an infinity or a NaN
-                if (CAREFUL && edge && tok0 < tok1) {
+#pragma unroll
+                for (int kk = 0; kk < 2 * HALVES; kk++)
+#pragma unroll
+                    for (int db = 0; db < DB; db++) {
+                        u4 x = v_operand(kk, db);
+                        if (CAREFUL) {
+#pragma unroll
+                            for (int y = 0; y < 4; y++) x[y] &= ~odd_mask<CT>(x[y]);
+                        }
+                        o[db] = mfma32<CT>(x, p[kk], o[db]);
+                        if (CAREFUL || db % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+                if (CAREFUL) {
+                    // A position that only some rows see must not reach the others as a 0 times an infinity or a NaN: such
+                    // values were left out above, and are added here to the rows that see them.
                     unsigned any = 0;
                     const int ln = here(lane);
 #pragma unroll 4
@@ -292,48 +310,31 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) any |= odd_bits<CT>(x[e]);
                     }
-                    odd = __ballot(any & 0x80008000u) & ALL;
-                }
-                if (CAREFUL && odd) {
-                    // A position that only some rows see must not reach the others as a 0 times an infinity: such values
-                    // are added position by position, to the rows that see them, and left out of the product.
 #pragma unroll 1
-                    for (uint64_t rest = odd; rest; rest &= rest - 1) {
-                        const int pos = __builtin_ctzll(rest), e = 4 * (pos / 8 % 2) + pos % 4;
-                        u4 only = u4{0u, 0u, 0u, 0u};
-                        if (pos / 4 % 2 == h) only[e / 2] = e & 1 ? 0xFFFF0000u : 0x0000FFFFu;
-                        const bool sees = kb + pos < hi && kb + pos >= lo;
+                    for (uint64_t rest = __ballot(any & 0x80008000u) & ALL; rest; rest &= rest - 1) {
+                        const int pos = __builtin_ctzll(rest);
+                        unsigned w = 0; // the word of p that has the position's, in the lanes of its half
 #pragma unroll
                         for (int kk = 0; kk < 2 * HALVES; kk++)
-                            if (pos / 16 == kk) { // uniform
 #pragma unroll
-                                for (int db = 0; db < DB; db++) {
-                                    u4 x = v_operand(kk, db) & only;
+                            for (int e = 0; e < 4; e++) w = pos / 16 * 4 + pos / 8 % 2 * 2 + pos % 4 / 2 == 4 * kk + e ? p[kk][e] : w;
+                        w = (unsigned)__shfl((int)w, here(n) + 32 * (pos / 4 % 2));
+                        using T = typename RowType<CT>::type;
+                        const float pv = (float)__builtin_bit_cast(T, (uint16_t)(pos & 1 ? w >> 16 : w));
+                        const bool sees = kb + pos < hi && kb + pos >= lo;
+                        const char *row = vt + pos * S::RB + here(8 * h);
 #pragma unroll
-                                    for (int y = 0; y < 4; y++) x[y] &= odd_mask<CT>(x[y]);
-                                    const f16v r = mfma32<CT>(x, p[kk], o[db]);
+                        for (int db = 0; db < DB; db++)
 #pragma unroll
-                                    for (int i = 0; i < 16; i++) o[db][i] = sees ? r[i] : o[db][i];
+                            for (int i = 0; i < 4; i++) { // dimensions 32 db + 8 i + 4 h ..
+                                const u2 v = *reinterpret_cast<const u2 *>(row + ((4 * db + i) ^ (int)S::swizzle(pos)) * 16);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const uint16_t x = (uint16_t)(e & 1 ? v[e / 2] >> 16 : v[e / 2]);
+                                    if (sees && (odd_bits<CT>(x) & 0x8000u)) o[db][4 * i + e] += pv * (float)__builtin_bit_cast(T, x);
                                 }
                             }
                     }
-#pragma unroll
-                    for (int kk = 0; kk < 2 * HALVES; kk++)
-#pragma unroll
-                        for (int db = 0; db < DB; db++) {
-                            u4 x = v_operand(kk, db);
-#pragma unroll
-                            for (int y = 0; y < 4; y++) x[y] &= ~odd_mask<CT>(x[y]);
-                            o[db] = mfma32<CT>(x, p[kk], o[db]);
-                        }
-                } else {
-#pragma unroll
-                    for (int kk = 0; kk < 2 * HALVES; kk++)
-#pragma unroll
-                        for (int db = 0; db < DB; db++) {
-                            o[db] = mfma32<CT>(v_operand(kk, db), p[kk], o[db]);
-                            if (db % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                        }
                 }
                 return true;
             };
@@ -348,10 +349,11 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
         }
         if (!have) continue; // no barrier below in this pass
         const int hs = here(h);
-        const bool cut = sg.t1 - sg.t0 < sg.cnt;
-        float *part = a.part_o + ((size_t)(2 * sh.w + (sg.t0 == 0 ? 1 : 0)) * R + 32 * wave + n) * D;
+        const bool cut = is_cut(sg);
+        const uint32_t slot = part_slot(sg, sh);
+        float *part = a.part_o + ((size_t)slot * R + 32 * wave + n) * D;
         if (cut && hs == 0) {
-            float *ml = a.part_ml + ((size_t)(2 * sh.w + (sg.t0 == 0 ? 1 : 0)) * R + 32 * wave + n) * 2;
+            float *ml = a.part_ml + ((size_t)slot * R + 32 * wave + n) * 2;
             ml[0] = mc;
             ml[1] = l;
         }
