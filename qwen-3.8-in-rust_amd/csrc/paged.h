@@ -64,14 +64,20 @@ template <> struct RowType<AQ_TYPE_F16> { using type = _Float16; };
 template <> struct RowType<AQ_TYPE_BF16> { using type = __bf16; };
 
 // Byte offset (in units) of a position's K / V row and whether it has one: a position past the table or on a page
-// outside 0..n_pages-1 has none.
+// outside 0..n_pages-1 has none. In two steps, so that the page's load need not be waited for at once.
+__device__ __forceinline__ uint32_t paged_entry(const PagedKv &c, const int32_t *table, uint32_t max_pages, uint32_t pos) {
+    const uint32_t col = c.page_size.quot(pos);
+    return col < max_pages ? (uint32_t)table[col] : 0xFFFFFFFFu;
+}
+__device__ __forceinline__ bool paged_units(const PagedKv &c, uint32_t entry, uint32_t pos, uint32_t *units) {
+    const uint32_t slot = pos - c.page_size.quot(pos) * c.page_size.d;
+    const bool ok = entry < c.n_pages;
+    *units = ok ? entry * c.page_units + slot * c.slot_units : 0u;
+    return ok;
+}
 __device__ __forceinline__ bool paged_slot(const PagedKv &c, const int32_t *table, uint32_t max_pages, uint32_t pos,
                                            uint32_t *units) {
-    const uint32_t col = c.page_size.quot(pos), slot = pos - col * c.page_size.d;
-    const uint32_t page = col < max_pages ? (uint32_t)table[col] : 0xFFFFFFFFu;
-    const bool ok = page < c.n_pages;
-    *units = ok ? page * c.page_units + slot * c.slot_units : 0u;
-    return ok;
+    return paged_units(c, paged_entry(c, table, max_pages, pos), pos, units);
 }
 
 // The sequence that row `row` belongs to (n_seq: none): the number of sequences that end at or before it, counted by

@@ -144,11 +144,13 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
 
         const int32_t last_tile = min((int32_t)((range.lo + sg.t1) * KW), (kend + TILE - 1) / TILE);
         int32_t tile = (int32_t)(range.lo + sg.t0) * KW + kg;
-        // where the tile's rows are: lane l has position l % TILE's
-        auto locate = [&](int32_t t, uint32_t *units) {
+        // where a tile's rows are: lane l has position l % TILE's page entry, then its place; bit l: it has a page
+        auto entry = [&](int32_t t) {
             const int32_t p = t * TILE + lane % TILE;
-            const bool ok = p < kend && paged_slot(a.kv, table, a.b.max_pages, (uint32_t)p, units);
-            if (!ok) *units = 0;
+            return t < last_tile && p < kend ? paged_entry(a.kv, table, a.b.max_pages, (uint32_t)p) : 0xFFFFFFFFu;
+        };
+        auto locate = [&](int32_t t, uint32_t e, uint32_t *units) {
+            const bool ok = paged_units(a.kv, e, (uint32_t)(t * TILE + lane % TILE), units);
             return (uint32_t)__ballot(ok) & (uint32_t)((1ull << TILE) - 1);
         };
         constexpr uint32_t ALL = (uint32_t)((1ull << TILE) - 1);
@@ -182,7 +184,11 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
         constexpr int KH = F && D == 256 ? 1 : HT;
         u4 k[KH][KD];
         uint32_t units = 0, okm = 0;
-        if (tile < last_tile) okm = locate(tile, &units);
+        uint32_t next = entry(tile); // page entries of the tile after this one, on their way for a tile's time
+        if (tile < last_tile) {
+            okm = locate(tile, next, &units);
+            next = entry(tile + KW);
+        }
 
         // this lane's rows: the positions they see are lo .. hi - 1
         int32_t hi[NR], lo[NR];
@@ -317,9 +323,10 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
 
             if constexpr (!F) {
                 VV v[CHUNKS][E];
+                okm = locate(tile + KW, next, &units);
+                next = entry(tile + 2 * KW);
 #pragma unroll
                 for (int e = 0; e < E; e++) load_v(now, e, &v[0][e], E);
-                if (tile + KW < last_tile) okm = locate(tile + KW, &units); // the next tile's page entries
                 const u4 *ql = qf + rg * NR * STEPS * NP * 64 + here(lane);
 #pragma unroll
                 for (int st = 0; st < STEPS; st++)
@@ -442,12 +449,13 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                     return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x), __uint_as_float(y), c, 0, 0, 0);
                 };
                 constexpr int VI = D == 64 ? 8 : 4; // V rows in registers at once
+                okm = locate(tile + KW, next, &units);
+                next = entry(tile + 2 * KW);
                 VV v[CHUNKS][VI];
                 const u4 *ql = qf + rg * NR * STEPS * NP * 64 + here(lane);
                 if constexpr (KH == HT) {
 #pragma unroll
                     for (int i = 0; i < VI; i++) load_v(now, i, &v[0][i], VI);
-                    if (tile + KW < last_tile) okm = locate(tile + KW, &units); // the next tile's page entries
                 }
 #pragma unroll
                 for (int t = 0; t < HT; t++) {
@@ -482,9 +490,6 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
 #pragma unroll
                     for (int e = 0; e < E; e++) x[nr][e] = s[nr][e / 4][e % 4];
                     soften(nr, x[nr], kb, ok, edge);
-                }
-                if constexpr (KH < HT) {
-                    if (tile + KW < last_tile) okm = locate(tile + KW, &units);
                 }
 #pragma unroll
                 for (int t = 0; t < HT; t++) {

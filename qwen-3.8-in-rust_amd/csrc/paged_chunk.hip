@@ -61,9 +61,12 @@ struct ChunkShape {
     static constexpr int TILE_BYTES = KEYS * RB;
     static constexpr int LOADS = TILE_BYTES / (256 * 16);     // 16-byte loads per thread and tile, of K and of V
     static constexpr int LDS = 4 * TILE_BYTES;                // two buffers of each
-    // which chunk of row r lies at place p: p ^ swizzle(r). Eight neighbouring rows have all eight values (K operands: 16
-    // bytes of each of eight rows a clock), four have their upper bits apart (V: 32 bytes of each of four rows).
-    static __device__ __forceinline__ uint32_t swizzle(uint32_t r) { return (r & 3) << 1 | (r >> 2 & 1); }
+    // Which chunk of row r lies at place p: p ^ swizzle(r). A clock serves 256 bytes: of K 16 bytes of 16 rows, which all
+    // have another value; of V 64 bytes of four rows, whose values differ above those four chunks. Linear: swizzle(x ^ y) =
+    // swizzle(x) ^ swizzle(y).
+    static __host__ __device__ constexpr uint32_t swizzle(uint32_t r) {
+        return D == 64 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3);
+    }
 };
 
 #define AQ_LDS __attribute__((address_space(3)))
@@ -115,28 +118,33 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                       max_lo = a.window ? (int64_t)base + tok1 + 1 - (int64_t)a.window : INT64_MIN;
 
         constexpr uint64_t ALL = KEYS == 64 ? ~0ull : (1ull << (KEYS & 63)) - 1;
-        // where a tile's rows are: lane l has position l's; bit l of the result: it has a page
-        auto locate = [&](int32_t tile, uint32_t *units) {
+        // where a tile's rows are: lane l has position l's page entry, then its place; bit l of the result: it has a page
+        auto entry = [&](int32_t tile) {
             const int32_t p = tile * KEYS + lane;
-            const bool ok = p < kend && lane < KEYS && paged_slot(a.kv, table, a.b.max_pages, (uint32_t)p, units);
-            if (!ok) *units = 0xFFFFFFFFu;
-            return (uint64_t)__ballot(ok);
+            return p < kend && lane < KEYS ? paged_entry(a.kv, table, a.b.max_pages, (uint32_t)p) : 0xFFFFFFFFu;
+        };
+        auto locate = [&](int32_t tile, uint32_t e, uint32_t *units) {
+            return (uint64_t)__ballot(paged_units(a.kv, e, (uint32_t)(tile * KEYS + lane), units));
         };
         const char *const kpool = a.kv.k + head_off, *const vpool = a.kv.v + head_off;
-        auto load_tile = [&](uint32_t units, uint64_t ok, int buf) {
-            constexpr uint32_t RPI = 64 / S::CPR; // rows of one wave's load
-            const uint32_t ln = (uint32_t)here(lane), rl = ln / S::CPR, place = ln % S::CPR;
-            const uint32_t last = (uint32_t)hd / 8 - 1, row0 = wave * S::LOADS * RPI + rl;
+        auto load_rows = [&](uint32_t units, uint64_t ok, int buf, auto whole) __attribute__((always_inline)) {
+            constexpr bool WHOLE = decltype(whole)::value; // every row has a page, every chunk is the head's
+            constexpr uint32_t RPI = 64 / S::CPR;          // rows of one wave's load
+            const uint32_t ln = (uint32_t)here(lane) & 63, row0 = wave * S::LOADS * RPI + ln / S::CPR;
+            const uint32_t c0 = (ln % S::CPR) ^ S::swizzle(row0);
             char *kd = kbuf + buf * S::TILE_BYTES + wave * S::LOADS * 1024, *vd = vbuf + (kd - kbuf);
+            uint32_t un[S::LOADS];
+#pragma unroll
+            for (uint32_t i = 0; i < S::LOADS; i++)
+                un[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(row0 * 4 + i * RPI * 4), (int)units);
 #pragma unroll
             for (uint32_t i = 0; i < S::LOADS; i++) {
-                // the row's low three bits: rl and, above them, i's
-                uint32_t c = place ^ S::swizzle((i * RPI & 7) + rl);
-                if (D != hd) c = min(c, last); // past the head: the queries are 0 there, the outputs not stored
-                const uint32_t un = (uint32_t)__builtin_amdgcn_ds_bpermute((int)((row0 + i * RPI) * 4), (int)units);
-                const uint64_t off = ((uint64_t)un << a.kv.unit_shift) + c * 16;
+                uint32_t c = c0 ^ S::swizzle(i * RPI); // row0 has none of its bits
+                // past the head: the queries are 0 there, the outputs not stored
+                if (!WHOLE) c = min(c, (uint32_t)hd / 8 - 1);
+                const uint64_t off = ((uint64_t)un[i] << a.kv.unit_shift) + c * 16;
                 const char *kp = kpool + off, *vp = vpool + off;
-                if (ok != ALL) { // uniform
+                if (!WHOLE) {
                     const bool has = (ok >> (row0 + i * RPI)) & 1;
                     kp = has ? kp : (const char *)&zeros;
                     vp = has ? vp : (const char *)&zeros;
@@ -144,6 +152,10 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                 __builtin_amdgcn_global_load_lds((const AQ_GLB void *)kp, (AQ_LDS void *)(kd + i * 1024), 16, 0, 0);
                 __builtin_amdgcn_global_load_lds((const AQ_GLB void *)vp, (AQ_LDS void *)(vd + i * 1024), 16, 0, 0);
             }
+        };
+        auto load_tile = [&](uint32_t units, uint64_t ok, int buf) __attribute__((always_inline)) {
+            if (ok == ALL && hd == D) load_rows(units, ok, buf, std::true_type{});
+            else load_rows(units, ok, buf, std::false_type{});
         };
 
         // ---- queries
@@ -179,11 +191,11 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
 
         int32_t t = (int32_t)(range.lo + sg.t0);
         const int32_t t_end = (int32_t)(range.lo + sg.t1);
-        uint32_t units, units_next = 0xFFFFFFFFu;
-        uint64_t ok = locate(t, &units), ok_next = 0;
+        uint32_t units;
+        uint64_t ok = locate(t, entry(t), &units);
         __syncthreads(); // the segment before has read its tiles
         load_tile(units, ok, 0);
-        if (t + 1 < t_end) ok_next = locate(t + 1, &units_next);
+        uint32_t next = t + 1 < t_end ? entry(t + 1) : 0; // the next tile's page entries, on their way for a tile's time
         int buf = 0;
         for (; t < t_end; t++) {
             const int32_t kb = t * KEYS;
@@ -193,9 +205,9 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
             asm volatile("" ::: "memory");
             const uint64_t ok_now = ok;
             if (t + 1 < t_end) {
-                load_tile(units_next, ok_next, buf ^ 1);
-                ok = ok_next;
-                if (t + 2 < t_end) ok_next = locate(t + 2, &units_next);
+                ok = locate(t + 1, next, &units);
+                load_tile(units, ok, buf ^ 1);
+                if (t + 2 < t_end) next = entry(t + 2);
             }
             const bool work = kb < max_hi && (int64_t)kb + KEYS > min_lo; // uniform in the wave
             const bool edge = kb + KEYS > min_hi || (int64_t)kb < max_lo || ok_now != ALL;
@@ -215,7 +227,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                     for (int k = 0; k < HALVES; k++) {
                         const u4 x = *reinterpret_cast<const u4 *>(kt + (ka ^ (st % 8 * 32)) + 32 * k * S::RB + (st / 8) * 256);
                         s[k] = mfma32<CT>(x, q[st], s[k]);
-                        if (st % (8 / HALVES) == 8 / HALVES - 1 && k == HALVES - 1) __builtin_amdgcn_sched_barrier(0);
+                        if (D == 256 && st % 8 == 7) __builtin_amdgcn_sched_barrier(0);
                     }
                 if (CAREFUL && edge) {
                     const int hr = hi - kb - 4 * h, lr = lo - kb - 4 * h; // of position 0 of this lane's
@@ -279,7 +291,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                     u4 x;
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const char *at = vt + (va ^ (db % 4 * 64)) + (16 * kk + 8 * e) * S::RB + (db / 4) * 256;
+                        const char *at = vt + (va ^ (db % 4 * 64 + e * 32)) + (16 * kk + 8 * e) * S::RB + (db / 4) * 256;
                         const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AQ_LDS s4 *)at);
                         const u2 z = __builtin_bit_cast(u2, y);
                         x[2 * e] = z[0];
@@ -297,7 +309,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                             for (int y = 0; y < 4; y++) x[y] &= ~odd_mask<CT>(x[y]);
                         }
                         o[db] = mfma32<CT>(x, p[kk], o[db]);
-                        if (CAREFUL || db % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                        if (CAREFUL || (D == 256 && db % 4 == 3)) __builtin_amdgcn_sched_barrier(0);
                     }
                 if (CAREFUL) {
                     // A position that only some rows see must not reach the others as a 0 times an infinity or a NaN: such
