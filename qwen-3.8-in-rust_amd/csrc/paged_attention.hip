@@ -33,7 +33,7 @@ typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 
 // Positions that a wave of the few-row kernel takes at once: 32, and 16 of a wide head, whose rows fill the registers.
-constexpr int few_tile(int CT, int D) { return CT != AQ_TYPE_F32 && D == 256 ? 16 : 32; }
+constexpr int few_tile(int D) { return D == 256 ? 16 : 32; }
 
 template <int CT>
 __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
@@ -86,13 +86,13 @@ constexpr int WAVES = 4;
 // on a wave's NR accumulator tiles; 32 rows of a wide head would not fit its registers, so there two waves take 16 rows
 // each over the same positions (RG = 2: the second reads them from the cache the first filled).
 constexpr int few_groups(int CT, int D, int R) { return R == 32 && (D == 256 || (CT == AQ_TYPE_F32 && D == 128)) ? 2 : 1; }
-constexpr int few_unit(int CT, int D, int R) { return WAVES / few_groups(CT, D, R) * few_tile(CT, D); }
+constexpr int few_unit(int CT, int D, int R) { return WAVES / few_groups(CT, D, R) * few_tile(D); }
 template <int CT, bool FQ, int D, int ROWS>
 struct FewShape {
     static constexpr int R = ROWS, RG = few_groups(CT, D, R), KW = WAVES / RG, NT = R / 16, NR = NT / RG;
     static constexpr bool F = CT == AQ_TYPE_F32;
     static constexpr int NP = !FQ || F ? 1 : (CT == AQ_TYPE_F16 ? 2 : 3); // pieces of q and of the probabilities
-    static constexpr int TILE = few_tile(CT, D);  // positions of a wave's step
+    static constexpr int TILE = few_tile(D);  // positions of a wave's step
     static constexpr int E = TILE / 4;                // of them a lane's: 16 (e / 4) + 4 g + e % 4
     static constexpr int STEPS = F ? D / 16 : D / 32; // 16-byte K operands of a row per lane
     static constexpr int VB = F || D == 64 ? 4 : 8;   // dimensions of a V row per lane and chunk
@@ -157,13 +157,12 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
         auto row_off = [&](uint32_t units, int pos) {
             return (uint64_t)(uint32_t)__shfl((int)units, pos) << a.kv.unit_shift;
         };
-        // operands s0 .. s0 + N - 1 of 16 rows of K; dimensions past the head repeat its last ones: q is 0 there
-        auto load_k = [&](uint32_t units, int t, int s0, auto &k) {
+        // 16 rows of K as operands; dimensions past the head repeat its last ones: q is 0 there
+        auto load_k = [&](uint32_t units, int t, u4 *k) {
             const char *p = kpool + (row_off(units, 16 * t + r) + (EXACT ? 16 * g : 0));
-            constexpr int N = sizeof(k) / 16;
 #pragma unroll
-            for (int s = 0; s < N; s++) {
-                const int at = EXACT ? 64 * (s0 + s) : min(64 * (s0 + s) + 16 * g, hd * ES - 16);
+            for (int s = 0; s < STEPS; s++) {
+                const int at = EXACT ? 64 * s : min(64 * s + 16 * g, hd * ES - 16);
                 k[s] = *reinterpret_cast<const u4 *>(p + at);
             }
         };
@@ -180,9 +179,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             }
         };
 
-        constexpr int KD = F && D == 256 ? STEPS / 2 : STEPS; // operands of a row in registers at once
-        constexpr int KH = F && D == 256 ? 1 : HT;
-        u4 k[KH][KD];
+        u4 k[HT][STEPS];
         uint32_t units = 0, okm = 0;
         uint32_t next = entry(tile); // page entries of the tile after this one, on their way for a tile's time
         if (tile < last_tile) {
@@ -255,11 +252,9 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             for (int nr = 0; nr < NR; nr++)
                 rscale[nr] = NP == 2 ? a.scale_log2 * __uint_as_float(exponent(16 * (rg * NR + nr) + r) << 23) : a.scale_log2;
         }
-        if constexpr (KH == HT) {
-            if (tile < last_tile) {
+        if (tile < last_tile) {
 #pragma unroll
-                for (int t = 0; t < HT; t++) load_k(units, t, 0, k[t]);
-            }
+            for (int t = 0; t < HT; t++) load_k(units, t, k[t]);
         }
         __syncthreads();
 
@@ -361,7 +356,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                 }
                 if (tile + KW < last_tile) { // the next tile's K rows, while this one is summed
 #pragma unroll
-                    for (int t = 0; t < HT; t++) load_k(units, t, 0, k[t]);
+                    for (int t = 0; t < HT; t++) load_k(units, t, k[t]);
                 }
                 VP pf[NR][NP];
 #pragma unroll
@@ -453,36 +448,21 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                 next = entry(tile + 2 * KW);
                 VV v[CHUNKS][VI];
                 const u4 *ql = qf + rg * NR * STEPS * NP * 64 + here(lane);
-                if constexpr (KH == HT) {
 #pragma unroll
-                    for (int i = 0; i < VI; i++) load_v(now, i, &v[0][i], VI);
-                }
+                for (int i = 0; i < VI; i++) load_v(now, i, &v[0][i], VI);
 #pragma unroll
-                for (int t = 0; t < HT; t++) {
+                for (int st = 0; st < STEPS; st++)
 #pragma unroll
-                    for (int s0 = 0; s0 < STEPS; s0 += KD) {
-                        if constexpr (KH < HT) {
-                            load_k(now, t, s0, k[0]);
-                            if (t == HT - 1 && s0 + KD == STEPS) {
+                    for (int nr = 0; nr < NR; nr++) {
+                        const u4 q = ql[(nr * STEPS + st) * 64];
 #pragma unroll
-                                for (int i = 0; i < VI; i++) load_v(now, i, &v[0][i], VI);
-                            }
-                        }
+                        for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int st = 0; st < KD; st++)
-#pragma unroll
-                            for (int nr = 0; nr < NR; nr++) {
-                                const u4 q = ql[(nr * STEPS + s0 + st) * 64];
-#pragma unroll
-                                for (int i = 0; i < 4; i++) s[nr][t] = mul(k[t % KH][st][i], q[i], s[nr][t]);
-                            }
+                            for (int t = 0; t < HT; t++) s[nr][t] = mul(k[t][st][i], q[i], s[nr][t]);
                     }
-                }
-                if constexpr (KH == HT) { // the next tile's K rows, while this one is summed
-                    if (tile + KW < last_tile) {
+                if (tile + KW < last_tile) { // the next tile's K rows, while this one is summed
 #pragma unroll
-                        for (int t = 0; t < HT; t++) load_k(units, t, 0, k[t]);
-                    }
+                    for (int t = 0; t < HT; t++) load_k(units, t, k[t]);
                 }
                 float x[NR][E];
 #pragma unroll
@@ -662,7 +642,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnPagedArgs a, int R) {
     const int tid = threadIdx.x;
     const uint32_t nkv = (uint32_t)a.kv.nkv, total = a.plan[0], chunk = a.plan[1], n_seg = a.plan[2];
     const uint32_t *line = a.plan + PLAN_HEAD;
-    uint32_t j, kvh, s0, cnt;
+    uint32_t j, kvh, s0, cnt, seq, rt;
     if constexpr (BY_SHARE) {
         const uint64_t end64 = (uint64_t)(blockIdx.x + 1) * chunk;
         if (end64 >= total) return; // the last share, or none
@@ -679,19 +659,23 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnPagedArgs a, int R) {
         s0 = p0 * nkv + kvh * places + a.lead; // the first unit's place
         cnt = places - a.lead;
         if (s0 >= end || s0 / chunk != blockIdx.x) return; // begins there, or before this share
+        seq = a.seg_seq[j];
+        rt = a.seg_rt[j];
     } else {
         j = blockIdx.x / nkv;
         kvh = blockIdx.x % nkv;
+        const uint32_t p0 = line[j], places = line[j + 1] - p0; // one latency for all of the plan
+        seq = a.seg_seq[j];
+        rt = a.seg_rt[j];
         if (j >= n_seg) return;
-        const uint32_t p0 = line[j], places = line[j + 1] - p0;
         s0 = p0 * nkv + kvh * places + a.lead;
         cnt = places - a.lead;
     }
     const uint32_t w0 = s0 / chunk, w1 = (s0 + cnt - 1) / chunk;
     if (w0 == w1) return; // one share had it all
-    const SeqRows sr = paged_seq(a.b, a.seg_seq[j]);
+    const SeqRows sr = paged_seq(a.b, seq);
     const int row = (int)blockIdx.y * ROWS + tid / (QUADS * GROUPS), grp = tid / QUADS % GROUPS, dim = tid % QUADS * 4;
-    const int32_t rr = (int32_t)a.seg_rt[j] * R + row;
+    const int32_t rr = (int32_t)rt * R + row;
     const bool have = row < R && rr < sr.n * a.G && dim < a.kv.hd;
     float m = -INFINITY, l = 0.0f;
     f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -887,7 +871,11 @@ int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uin
     c->R = c->many ? CHUNK_ROWS : rows <= 16 ? 16 : 32;
     c->unit = c->many ? chunk_keys(c->D) : few_unit(kv->type, c->D, c->R);
     c->min_chunk = c->many ? 256 / c->unit : 1;
-    c->lead = c->many ? 192 / c->unit : 0;
+    // What a segment costs besides its positions (queries, first loads, the waves' meeting, its output), in units. Prompts
+    // of three requests (10,500 rows of 32 heads of 128), of 64 positions: 0: 794 us, 2: 532, 4: 459, 6: 459, 8: 467. Eight
+    // verify batches of 32 rows (f32 over f16, heads of 256), of 32: 0: 46.4, 2: 42.5, 4: 42.6. Single tokens: none to gain;
+    // nor where a unit takes as long as that (f32 products).
+    c->lead = c->many ? 320 / c->unit : c->R == 32 && kv->type != AQ_TYPE_F32 ? 2 : 0;
     // row tiles: a whole one per R rows of all sequences together, and one begun per sequence
     const uint64_t n_seg = std::min<uint64_t>((uint64_t)b->n_rows * G / c->R + b->n_seq, (uint64_t)b->n_rows * G);
     c->planned = n_seg > INLINE_TILES || b->n_seq > INLINE_TILES;
@@ -896,8 +884,11 @@ int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uin
     if ((double)n_seg * (double)per * kv->n_head_kv >= 2147483648.0 || n_seg * kv->n_head_kv >= (1u << 31))
         return fail(AQ_EUNSUP, std::string(call) + ": batch of more than 2^31 units of work");
     c->n_seg = (uint32_t)n_seg;
-    // two work-groups per CU, and no more than there can be units
-    const uint64_t units = n_seg * kv->n_head_kv * per, shares = std::min<uint64_t>((uint64_t)compute_units(device) * 2, units);
+    // Two work-groups per CU; one of up to 16 rows over 16-bit pages, bound by the memory alone (48 sequences at 6000, 32
+    // heads on 8 of 128: one 215 us, two 228, three 223; one sequence at 8000, 24 heads on 4 of 256: 17.7 and 19.0; but f32
+    // pages, 64 rows at 4001: 131 and 101). No more than there can be units.
+    const uint64_t per_cu = !c->many && c->R == 16 && kv->type != AQ_TYPE_F32 ? 1 : 2;
+    const uint64_t units = n_seg * kv->n_head_kv * per, shares = std::min<uint64_t>((uint64_t)compute_units(device) * per_cu, units);
     c->shares = (uint32_t)(shares > 8 ? (shares + 7) / 8 * 8 : std::max<uint64_t>(shares, 1));
     c->join = c->cap > c->unit; // else no segment has a second unit
     c->space = paged_space(c->shares, c->n_seg, (size_t)c->R, (size_t)c->D);
