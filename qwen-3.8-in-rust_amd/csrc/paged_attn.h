@@ -1,4 +1,4 @@
-// paged_attn.h — what the two paged attention kernels (paged_attention.hip: few rows, pages streamed through registers;
+// paged_attn.h — what the two paged attention kernels (paged_few.h: few rows, pages streamed through registers;
 // paged_chunk.hip: many rows, tiles in the LDS) share: the division of the work, the partial results, the outputs.
 //
 // Rows. The G = n_head / n_head_kv query heads that share a K/V head, times a sequence's new tokens, are its rows over
@@ -323,8 +323,21 @@ inline PagedSpace paged_space(size_t shares, size_t n_seg, size_t R, size_t D) {
 }
 
 int launch_paged_plan(const AttnPagedArgs &a, int R, uint32_t tk, hipStream_t stream);
+// The few-row kernel (paged_few.h): a cache of this type, rows of its type or f32; D the padded head size, R 16 or 32 rows.
+int launch_paged_few_f32(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
+int launch_paged_few_f16(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
+int launch_paged_few_bf16(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
 int launch_paged_chunk(const AttnPagedArgs &a, int D, hipStream_t stream); // 16-bit rows and cache
 int launch_paged_combine(const AttnPagedArgs &a, int R, int D, int rows, hipStream_t stream);
+
+constexpr int WAVES = 4;
+
+// Positions that a wave of the few-row kernel takes at once: 32, and 16 of a wide head, whose rows fill the registers.
+constexpr int few_tile(int D) { return D == 256 ? 16 : 32; }
+// The rows (16 or 32) lie on a wave's NR accumulator tiles; 32 rows of a wide head would not fit its registers, so there two waves take 16 rows
+// each over the same positions (RG = 2: the second reads them from the cache the first filled).
+constexpr int few_groups(int CT, int D, int R) { return R == 32 && (D == 256 || (CT == AQ_TYPE_F32 && D == 128)) ? 2 : 1; }
+constexpr int few_unit(int CT, int D, int R) { return WAVES / few_groups(CT, D, R) * few_tile(D); }
 
 constexpr int CHUNK_ROWS = 128;                                   // paged_chunk.hip's row tile
 constexpr int chunk_keys(int D) { return D == 256 ? 32 : 64; } // and its unit

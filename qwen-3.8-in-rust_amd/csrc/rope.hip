@@ -198,19 +198,17 @@ struct RopeArgs {
     HeadsView x, y;
     const double *freq;
     const int32_t *pos;
-    uint32_t n_rows, n_heads, dim, rot_units, units, heads_per, items, row_shift;
-    FastDiv unit_div;
+    uint32_t n_rows, n_heads, dim, rot_units, units, heads_per, items;
+    FastDiv unit_div, item_div;
     float gain, sign;
 };
 
-// Rows over blockIdx.x (256 >> row_shift of them a work-group), a row's (head group, unit) items over the threads. 8191
-// rows x 40 heads x 128 in bf16: see the table of the design document's timed cases for what it reaches.
+// One (row, head group, unit) item per thread, in that order, 64 bytes or more in flight each.
 template <int T, bool INTER, int VEC, bool W>
 __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
     using E = typename RowType<T>::type;
-    const uint32_t row = blockIdx.x * (256u >> a.row_shift) + (threadIdx.x >> a.row_shift);
-    const uint32_t item = (blockIdx.y << a.row_shift) + (threadIdx.x & ((1u << a.row_shift) - 1));
-    if (row >= a.n_rows || item >= a.items) return;
+    const uint32_t at = blockIdx.x * 256u + threadIdx.x, row = a.item_div.quot(at), item = at - row * a.items;
+    if (row >= a.n_rows) return;
     const uint32_t grp = a.unit_div.quot(item), unit = item - grp * a.units;
     const bool rot = unit < a.rot_units;
     Unit<INTER, VEC> u;
@@ -410,17 +408,14 @@ int aq_rope_apply(const aq_rope *r, const aq_heads *x, const aq_heads *y, size_t
     unit_shape(r->layout, r->dim, (uint32_t)head_dim, wide ? vec : (inter ? 2 : 1), &a.rot_units, &a.units);
     if (x->data == y->data) a.units = a.rot_units; // the rest of the head stays where it is
     a.heads_per = heads_per_thread((uint64_t)n_rows * n_heads * a.units);
-    const uint64_t items = (uint64_t)a.units * ((n_heads + a.heads_per - 1) / a.heads_per);
-    AQ_REQUIRE(items <= 65535u * 256u, "aq_rope_apply: size");
+    const uint64_t items = (uint64_t)a.units * ((n_heads + a.heads_per - 1) / a.heads_per), all = items * n_rows;
+    if (all > (1ull << 31) - 256) return fail(AQ_EUNSUP, "aq_rope_apply: more than 2^31 pieces of rows");
     a.items = (uint32_t)items;
     a.unit_div = FastDiv(a.units);
+    a.item_div = FastDiv(a.items);
     a.gain = r->gain;
     a.sign = inverse ? -1.0f : 1.0f;
-    uint32_t sh = 4;
-    while (sh < 8 && (1u << sh) < a.items) sh++;
-    a.row_shift = sh;
-    const uint32_t rpb = 256u >> sh;
-    const dim3 grid((uint32_t)((n_rows + rpb - 1) / rpb), (a.items + (1u << sh) - 1) >> sh);
+    const dim3 grid((uint32_t)((all + 255) / 256));
     AQ_HIP(hipSetDevice(r->ctx->device));
     const hipStream_t st = stream ? (hipStream_t)stream : r->ctx->stream;
     switch (x->type) {
