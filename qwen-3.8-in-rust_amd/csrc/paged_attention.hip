@@ -26,40 +26,35 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnPagedArgs a, int R) {
     const int tid = threadIdx.x;
     const uint32_t nkv = (uint32_t)a.kv.nkv, total = a.plan[0], chunk = a.plan[1], n_seg = a.plan[2];
     const uint32_t *line = a.plan + PLAN_HEAD;
-    uint32_t j, kvh, s0, cnt, seq, rt;
+    uint32_t j, kvh, s0, cnt;
+    RowTile t;
     if constexpr (BY_SHARE) {
         const uint64_t end64 = (uint64_t)(blockIdx.x + 1) * chunk;
         if (end64 >= total) return; // the last share, or none
         const uint32_t end = (uint32_t)end64;
-        if (tid == 0) found = 0xFFFFFFFFu;
-        __syncthreads();
         for (uint32_t i = tid; i < n_seg; i += THREADS)
-            if (line[i] * nkv < end && end < line[i + 1] * nkv) found = i;
+            if (tile_holds(a.tiles[i], line[i], line[i + 1], nkv, end, &kvh)) found = i;
         __syncthreads();
         j = found;
-        if (j == 0xFFFFFFFFu) return; // a row tile's first K/V head begins there
-        const uint32_t p0 = line[j], places = line[j + 1] - p0;
-        kvh = (end - p0 * nkv) / places;
-        s0 = p0 * nkv + kvh * places + a.lead; // the first unit's place
-        cnt = places - a.lead;
+        t = a.tiles[j];
+        kvh = (end - t.p0 * nkv) / (t.p1 - t.p0);
+        s0 = tile_place(t, line[j], nkv, kvh) + a.lead; // the first unit's place
+        cnt = line[j + 1] - line[j] - a.lead;
         if (s0 >= end || s0 / chunk != blockIdx.x) return; // begins there, or before this share
-        seq = a.seg_seq[j];
-        rt = a.seg_rt[j];
     } else {
         j = blockIdx.x / nkv;
         kvh = blockIdx.x % nkv;
-        const uint32_t p0 = line[j], places = line[j + 1] - p0; // one latency for all of the plan
-        seq = a.seg_seq[j];
-        rt = a.seg_rt[j];
+        const uint32_t p0 = line[j], p1 = line[j + 1]; // one latency for all of the plan
+        t = a.tiles[j];
         if (j >= n_seg) return;
-        s0 = p0 * nkv + kvh * places + a.lead;
-        cnt = places - a.lead;
+        s0 = tile_place(t, p0, nkv, kvh) + a.lead;
+        cnt = p1 - p0 - a.lead;
     }
     const uint32_t w0 = s0 / chunk, w1 = (s0 + cnt - 1) / chunk;
     if (w0 == w1) return; // one share had it all
-    const SeqRows sr = paged_seq(a.b, seq);
+    const SeqRows sr = paged_seq(a.b, t.seq);
     const int row = (int)blockIdx.y * ROWS + tid / (QUADS * GROUPS), grp = tid / QUADS % GROUPS, dim = tid % QUADS * 4;
-    const int32_t rr = (int32_t)rt * R + row;
+    const int32_t rr = (int32_t)t.rt * R + row;
     const bool have = row < R && rr < sr.n * a.G && dim < a.kv.hd;
     float m = -INFINITY, l = 0.0f;
     f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -166,8 +161,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint
                 if (first[mid] <= j) lo = mid;
                 else hi = mid;
             }
-            a.seg_seq[j] = s0 + lo;
-            a.seg_rt[j] = j - first[lo];
+            a.tiles[j].seq = s0 + lo;
+            a.tiles[j].rt = j - first[lo];
         }
         __syncthreads();
         if (carry > a.n_seg) break; // sequences that overlap: not a batch
@@ -179,7 +174,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint
     for (uint32_t j0 = 0; j0 < n_seg; j0 += 1024) {
         const uint32_t j = j0 + tid;
         uint32_t n = 0;
-        if (j < n_seg) n = tile_count(a, a.seg_seq[j], a.seg_rt[j], R, tk); // its own, or ordered by the barriers above
+        if (j < n_seg) n = tile_count(a, a.tiles[j].seq, a.tiles[j].rt, R, tk); // its own, or ordered by the barriers above
         const uint32_t end = scan(n);
         if (j < n_seg) a.plan[PLAN_HEAD + j + 1] = end;
     }
@@ -189,6 +184,12 @@ __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint
         a.plan[1] = share_chunk(total, a.shares, a.min_chunk);
         a.plan[2] = n_seg;
         a.plan[PLAN_HEAD] = 0;
+    }
+    __syncthreads(); // the prefix sums are written
+    for (uint32_t j = tid; j < n_seg; j += 1024) {
+        const uint32_t j0 = j - a.tiles[j].rt, j1 = min(j0 + seq_tiles(a, a.tiles[j].seq, R), n_seg);
+        a.tiles[j].p0 = a.plan[PLAN_HEAD + j0];
+        a.tiles[j].p1 = a.plan[PLAN_HEAD + j1];
     }
 }
 
@@ -343,8 +344,7 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
     a.planned = c.planned;
     char *ws = (char *)workspace;
     a.plan = (uint32_t *)(ws + c.space.plan);
-    a.seg_seq = (uint32_t *)(ws + c.space.seg);
-    a.seg_rt = a.seg_seq + c.n_seg;
+    a.tiles = (RowTile *)(ws + c.space.seg);
     a.part_o = (float *)(ws + c.space.o);
     a.part_ml = (float *)(ws + c.space.ml);
     AQ_HIP(hipSetDevice(ctx->device));

@@ -6,7 +6,8 @@
 // head; its keys are counted in units of TK positions from position 0, and only the units that some row of the tile
 // sees are work.
 //
-// Split. All segments' units in order (sequence, row tile, K/V head, key unit), each segment's with `lead` places before
+// Split. All segments' units in order (sequence, K/V head, row tile, key unit: row tiles that read the same keys side by
+// side, on one XCD at one time), each segment's with `lead` places before
 // them for what a segment costs besides its units, form one line of `total` places, cut into work-group shares of `chunk`
 // places each, however long or short the sequences are. A share that holds a whole segment
 // writes its output; where a segment is cut, each share writes its part (row maxima, sums and unnormalised outputs, in
@@ -18,6 +19,11 @@
 #include "paged.h"
 
 namespace aq {
+
+// A row tile: its sequence, its index there, and the prefix sums where the sequence's row tiles begin and end.
+struct RowTile {
+    uint32_t seq, rt, p0, p1;
+};
 
 struct AttnPagedArgs {
     PagedKv kv;
@@ -31,11 +37,10 @@ struct AttnPagedArgs {
     uint32_t q_wide, out_wide; // 16-byte loads of q; 4-value stores of out and loads of gate
     uint32_t shares, min_chunk, lead; // work-groups; least places of a share; places before a segment's units
     uint32_t n_seg;   // row tiles of all sequences at most
-    uint32_t planned; // 1: a plan launch has filled plan, seg_seq, seg_rt; 0: the work-groups divide by themselves
+    uint32_t planned; // 1: a plan launch has filled plan and tiles; 0: the work-groups divide by themselves
     // workspace
     uint32_t *plan;    // [0] total places (of all K/V heads), [1] chunk, [2] row tiles; then prefix sums of their places
-    uint32_t *seg_seq; // of each row tile: its sequence and its index there
-    uint32_t *seg_rt;
+    RowTile *tiles;    // of each row tile
     float *part_o;  // [2 * shares][R][D]
     float *part_ml; // [2 * shares][R][2]
 };
@@ -83,11 +88,35 @@ struct PlanLds {
     uint32_t pre[INLINE_TILES + 1], first[INLINE_TILES + 1], seq[INLINE_TILES], wsum[4], found;
 };
 
-// A work-group's share of the line: its number, its places begin .. end - 1 (none: begin == end), the row tile that
-// begin lies in.
+// A work-group's share of the line: its number, its places begin .. end - 1 (none: begin == end); the row tile and K/V head
+// that begin lies in.
 struct Share {
-    uint32_t w, begin, end, j;
+    uint32_t w, begin, end, j, kvh, n_seg;
 };
+
+// Row tile j of the plan, wherever that is.
+__device__ __forceinline__ RowTile row_tile(const AttnPagedArgs &a, const PlanLds &lds, uint32_t n_seg, uint32_t j) {
+    if (a.planned) return a.tiles[j];
+    RowTile t;
+    t.seq = lds.seq[j];
+    const uint32_t j0 = lds.first[t.seq], j1 = t.seq + 1 < a.b.n_seq ? min(lds.first[t.seq + 1], n_seg) : n_seg;
+    t.rt = j - j0;
+    t.p0 = lds.pre[j0];
+    t.p1 = lds.pre[j1];
+    return t;
+}
+// The first place of row tile j on a K/V head (pre: its prefix sum).
+__device__ __forceinline__ uint32_t tile_place(const RowTile &t, uint32_t pre, uint32_t nkv, uint32_t kvh) {
+    return t.p0 * nkv + kvh * (t.p1 - t.p0) + (pre - t.p0);
+}
+// Whether place x lies in row tile j (its prefix sums pre .. end), and on which K/V head.
+__device__ __forceinline__ bool tile_holds(const RowTile &t, uint32_t pre, uint32_t end, uint32_t nkv, uint32_t x, uint32_t *kvh) {
+    if (x < t.p0 * nkv || x >= t.p1 * nkv) return false;
+    const uint32_t rel = x - t.p0 * nkv, size = t.p1 - t.p0;
+    *kvh = rel / size;
+    const uint32_t at = rel - *kvh * size + t.p0;
+    return pre <= at && at < end;
+}
 
 // Inclusive prefix sums over a wave, and over a work-group of 256 (wsum: 4 words; two barriers).
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lanes = 64) { // the first `lanes` lanes'
@@ -122,7 +151,7 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
     Share sh;
     // neighbouring shares on one XCD: work-groups go round the 8 XCDs, and neighbours read the same pages' lines
     sh.w = a.shares % 8 ? blockIdx.x : (blockIdx.x % 8) * (a.shares / 8) + blockIdx.x / 8;
-    sh.begin = sh.end = sh.j = 0;
+    sh.begin = sh.end = sh.j = sh.kvh = 0;
     uint32_t total, chunk, n_seg;
     bool one_wave = false;
     if (a.planned) {
@@ -196,8 +225,7 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
             }
             for (uint32_t j = tid; j < n_seg; j += 256) {
                 a.plan[PLAN_HEAD + j + 1] = lds.pre[j + 1];
-                a.seg_seq[j] = lds.seq[j];
-                a.seg_rt[j] = j - lds.first[lds.seq[j]];
+                a.tiles[j] = row_tile(a, lds, n_seg, j);
             }
         }
     }
@@ -205,46 +233,68 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
     if (first >= total) return sh;
     sh.begin = (uint32_t)first;
     sh.end = min(total, sh.begin + chunk);
-    // the row tile that the share begins in: the only one that begins at or before it and ends after it
+    // the row tile that the share begins in
+    uint32_t kvh = 0;
     if (one_wave) {
-        const bool in = (uint32_t)lane < n_seg && lds.pre[lane] * nkv <= sh.begin && sh.begin < lds.pre[lane + 1] * nkv;
+        const bool in = (uint32_t)lane < n_seg && tile_holds(row_tile(a, lds, n_seg, lane), lds.pre[lane], lds.pre[lane + 1],
+                                                             nkv, sh.begin, &kvh);
         sh.j = (uint32_t)__builtin_ctzll(__ballot(in));
     } else {
         const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : lds.pre;
         for (uint32_t j = tid; j < n_seg; j += 256)
-            if (line[j] * nkv <= sh.begin && sh.begin < line[j + 1] * nkv) lds.found = j;
+            if (tile_holds(row_tile(a, lds, n_seg, j), line[j], line[j + 1], nkv, sh.begin, &kvh)) lds.found = j;
         __syncthreads();
         sh.j = same(lds.found);
     }
+    const RowTile t = row_tile(a, lds, n_seg, sh.j);
+    sh.kvh = (sh.begin - same(t.p0) * nkv) / (same(t.p1) - same(t.p0));
+    sh.n_seg = n_seg;
     return sh;
 }
 
-// The next segment of a share, from place u on: K/V head, the sequence, its first row, the units t0 .. t1 - 1 of the
-// segment's cnt that are the share's (none: t1 <= t0). Advances u and j. All uniform.
+// The next segment of a share, from place u on (row tile j on K/V head kvh, or the one after it): the sequence, its first
+// row, the units t0 .. t1 - 1 of the segment's cnt that are the share's (none: t1 <= t0). Advances u, j and kvh. All uniform.
 struct Segment {
     uint32_t kvh, seq, cnt;
     int32_t t0, t1, r0;
 };
 __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, const PlanLds &lds, const Share &sh,
-                                                uint32_t &u, uint32_t &j) {
+                                                uint32_t &u, uint32_t &j, uint32_t &kvh) {
     const uint32_t nkv = (uint32_t)a.kv.nkv;
     const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : lds.pre;
-    uint32_t p0 = same(line[j]), p1 = same(line[j + 1]);
-    if (p1 * nkv <= u) { // every row tile has units
-        j++;
-        p0 = p1;
-        p1 = same(line[j + 1]);
+    RowTile t = row_tile(a, lds, sh.n_seg, j);
+    t.p0 = same(t.p0);
+    t.p1 = same(t.p1);
+    t.rt = same(t.rt);
+    uint32_t p = same(line[j]), e = same(line[j + 1]);
+    if (u >= tile_place(t, p, nkv, kvh) + (e - p)) { // past it: the sequence's next row tile, next head, or the next sequence
+        if (e < t.p1) {
+            j++;
+            t.rt++;
+        } else if (kvh + 1 < nkv) {
+            kvh++;
+            j -= t.rt;
+            t.rt = 0;
+        } else {
+            kvh = 0;
+            j++;
+            t = row_tile(a, lds, sh.n_seg, j);
+            t.p0 = same(t.p0);
+            t.p1 = same(t.p1);
+            t.rt = 0;
+        }
+        p = same(line[j]);
+        e = same(line[j + 1]);
     }
     Segment s;
-    const uint32_t places = p1 - p0, rel = u - p0 * nkv;
-    s.kvh = rel / places;
-    const uint32_t from = rel - s.kvh * places, to = min(places, from + (sh.end - u));
+    s.kvh = kvh;
+    const uint32_t places = e - p, from = u - tile_place(t, p, nkv, kvh), to = min(places, from + (sh.end - u));
     s.cnt = places - a.lead;
     s.t0 = max((int32_t)(from - a.lead), 0);
     s.t1 = (int32_t)(to - a.lead);
     u += to - from;
-    s.seq = same(a.planned ? a.seg_seq[j] : lds.seq[j]);
-    s.r0 = (int32_t)same(a.planned ? a.seg_rt[j] : j - lds.first[s.seq]) * R;
+    s.seq = same(t.seq);
+    s.r0 = (int32_t)t.rt * R;
     return s;
 }
 // Whether other shares have units of it too, and then the slot of this share's part.
@@ -316,7 +366,7 @@ inline PagedSpace paged_space(size_t shares, size_t n_seg, size_t R, size_t D) {
     PagedSpace s;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     s.seg = up((PLAN_HEAD + n_seg + 1) * 4);
-    s.o = s.seg + up(n_seg * 8);
+    s.o = s.seg + up(n_seg * sizeof(RowTile));
     s.ml = s.o + up(2 * shares * R * D * 4);
     s.bytes = s.ml + up(2 * shares * R * 2 * 4);
     return s;

@@ -48,6 +48,18 @@ __device__ __forceinline__ unsigned pack2(float x, float y) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, e2));
 }
 
+// l plus the two values of a packed word, in 32 bits.
+template <int CT>
+__device__ __forceinline__ float add2(unsigned w, float l) {
+    if constexpr (CT == AQ_TYPE_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{1, 1}, l, false);
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.0f, (__bf16)1.0f}, l, false);
+    }
+}
+
 // The larger of x's two halves (lanes l and l + 32).
 __device__ __forceinline__ float both_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -91,9 +103,9 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
     const int vaddr0 = vkey * S::RB + (int)(((2 * ((lane >> 4) & 1) + (vi % 4) / 2) ^ S::swizzle(vkey)) << 4) + (vi % 2) * 8;
 
     const Share sh = take_share(a, R, KEYS, plan);
-    uint32_t u = sh.begin, j = sh.j;
+    uint32_t u = sh.begin, j = sh.j, kv_at = sh.kvh;
     while (u < sh.end) { // uniform
-        const Segment sg = next_segment(a, R, plan, sh, u, j);
+        const Segment sg = next_segment(a, R, plan, sh, u, j, kv_at);
         if (sg.t1 <= sg.t0) continue;
         const int n = here(n0), h = here(h0);
         const SeqRows sr = paged_seq(a.b, sg.seq);
@@ -126,36 +138,41 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
         auto locate = [&](int32_t tile, uint32_t e, uint32_t *units) {
             return (uint64_t)__ballot(paged_units(a.kv, e, (uint32_t)(tile * KEYS + lane), units));
         };
+        // a load's rows lie in one page, and near enough for 32 bits
+        const bool runs = a.kv.page_size.d % (64 / S::CPR) == 0 && ((uint64_t)a.kv.slot_units << a.kv.unit_shift) < (1u << 27);
         const char *const kpool = a.kv.k + head_off, *const vpool = a.kv.v + head_off;
-        auto load_rows = [&](uint32_t units, uint64_t ok, int buf, auto whole) __attribute__((always_inline)) {
-            constexpr bool WHOLE = decltype(whole)::value; // every row has a page, every chunk is the head's
-            constexpr uint32_t RPI = 64 / S::CPR;          // rows of one wave's load
-            const uint32_t ln = (uint32_t)here(lane) & 63, row0 = wave * S::LOADS * RPI + ln / S::CPR;
+        // One wave's loads of its rows of a tile, RPI rows each.
+        auto load_tile = [&](uint32_t units, uint64_t ok, int buf) __attribute__((always_inline)) {
+            constexpr uint32_t RPI = 64 / S::CPR;
+            const uint32_t ln = (uint32_t)here(lane) & 63, first = wave * S::LOADS * RPI, row0 = first + ln / S::CPR;
             const uint32_t c0 = (ln % S::CPR) ^ S::swizzle(row0);
             char *kd = kbuf + buf * S::TILE_BYTES + wave * S::LOADS * 1024, *vd = vbuf + (kd - kbuf);
-            uint32_t un[S::LOADS];
+            // the lane's 16 bytes of row row0 + i RPI (whose low bits row0 has none of); past the head: the queries are 0
+            // there, the outputs not stored
+            auto chunk = [&](uint32_t i) {
+                const uint32_t c = c0 ^ S::swizzle(i * RPI);
+                return (hd == D ? c : min(c, (uint32_t)hd / 8 - 1)) * 16;
+            };
+            if (ok == ALL && runs) { // a load's rows are one run of a page: one address for the wave
+                const uint32_t lead = (ln / S::CPR) * (a.kv.slot_units << a.kv.unit_shift);
 #pragma unroll
-            for (uint32_t i = 0; i < S::LOADS; i++)
-                un[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(row0 * 4 + i * RPI * 4), (int)units);
-#pragma unroll
-            for (uint32_t i = 0; i < S::LOADS; i++) {
-                uint32_t c = c0 ^ S::swizzle(i * RPI); // row0 has none of its bits
-                // past the head: the queries are 0 there, the outputs not stored
-                if (!WHOLE) c = min(c, (uint32_t)hd / 8 - 1);
-                const uint64_t off = ((uint64_t)un[i] << a.kv.unit_shift) + c * 16;
-                const char *kp = kpool + off, *vp = vpool + off;
-                if (!WHOLE) {
-                    const bool has = (ok >> (row0 + i * RPI)) & 1;
-                    kp = has ? kp : (const char *)&zeros;
-                    vp = has ? vp : (const char *)&zeros;
+                for (uint32_t i = 0; i < S::LOADS; i++) {
+                    const uint64_t off = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)units, first + i * RPI) << a.kv.unit_shift;
+                    const uint32_t at = lead + chunk(i);
+                    __builtin_amdgcn_global_load_lds((const AQ_GLB void *)(kpool + off + at), (AQ_LDS void *)(kd + i * 1024), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((const AQ_GLB void *)(vpool + off + at), (AQ_LDS void *)(vd + i * 1024), 16, 0, 0);
                 }
-                __builtin_amdgcn_global_load_lds((const AQ_GLB void *)kp, (AQ_LDS void *)(kd + i * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const AQ_GLB void *)vp, (AQ_LDS void *)(vd + i * 1024), 16, 0, 0);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < S::LOADS; i++) {
+                    const uint32_t un = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(row0 * 4 + i * RPI * 4), (int)units);
+                    const uint64_t off = ((uint64_t)un << a.kv.unit_shift) + chunk(i);
+                    const bool has = (ok >> (row0 + i * RPI)) & 1;
+                    const char *kp = has ? kpool + off : (const char *)&zeros, *vp = has ? vpool + off : (const char *)&zeros;
+                    __builtin_amdgcn_global_load_lds((const AQ_GLB void *)kp, (AQ_LDS void *)(kd + i * 1024), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((const AQ_GLB void *)vp, (AQ_LDS void *)(vd + i * 1024), 16, 0, 0);
+                }
             }
-        };
-        auto load_tile = [&](uint32_t units, uint64_t ok, int buf) __attribute__((always_inline)) {
-            if (ok == ALL && hd == D) load_rows(units, ok, buf, std::true_type{});
-            else load_rows(units, ok, buf, std::false_type{});
         };
 
         // ---- queries
@@ -252,7 +269,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                 for (int i = 1; i < 16 * HALVES; i++) mt = fmaxf(mt, s[i / 16][i % 16]);
                 mt = both_max(mt) * a.scale_log2;
                 if (!CAREFUL && __any(!(fabsf(mt) < 1048576.0f))) return false;
-                if (__any(mt > mc + GROW || (mc == -INFINITY && mt > mc))) {
+                if (__any(mt > mc + GROW)) {
                     const float mn = fmaxf(mc, mt), mu = mn == -INFINITY ? 0.0f : mn;
                     const float alpha = fast_exp2(mc - mu);
                     l *= alpha;
@@ -276,16 +293,15 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
 #pragma unroll
                         for (int i = 0; i < 16; i++) s[k][i] = fast_exp2(fmaf(s[k][i], a.scale_log2, off));
                 }
-#pragma unroll
-                for (int k = 0; k < HALVES; k++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) l += s[k][i];
                 u4 p[2 * HALVES]; // of 16 positions each
 #pragma unroll
                 for (int kk = 0; kk < 2 * HALVES; kk++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
+                    {
                         p[kk][e] = pack2<CT>(s[kk / 2][8 * (kk % 2) + 2 * e], s[kk / 2][8 * (kk % 2) + 2 * e + 1]);
+                        l = add2<CT>(p[kk][e], l);
+                    }
 
                 auto v_operand = [&](int kk, int db) {
                     u4 x;
