@@ -236,13 +236,17 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
     // the row tile that the share begins in
     uint32_t kvh = 0;
     if (one_wave) {
-        const bool in = (uint32_t)lane < n_seg && tile_holds(row_tile(a, lds, n_seg, lane), lds.pre[lane], lds.pre[lane + 1],
-                                                             nkv, sh.begin, &kvh);
-        sh.j = (uint32_t)__builtin_ctzll(__ballot(in));
+        if (n_seg > 1) {
+            const bool in = (uint32_t)lane < n_seg && tile_holds(row_tile(a, lds, n_seg, lane), lds.pre[lane],
+                                                                 lds.pre[lane + 1], nkv, sh.begin, &kvh);
+            sh.j = (uint32_t)__builtin_ctzll(__ballot(in));
+        }
     } else {
-        const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : lds.pre;
-        for (uint32_t j = tid; j < n_seg; j += 256)
-            if (tile_holds(row_tile(a, lds, n_seg, j), line[j], line[j + 1], nkv, sh.begin, &kvh)) lds.found = j;
+        for (uint32_t j = tid; j < n_seg; j += 256) {
+            const uint32_t p = a.planned ? a.plan[PLAN_HEAD + j] : lds.pre[j];
+            const uint32_t e = a.planned ? a.plan[PLAN_HEAD + j + 1] : lds.pre[j + 1];
+            if (tile_holds(row_tile(a, lds, n_seg, j), p, e, nkv, sh.begin, &kvh)) lds.found = j;
+        }
         __syncthreads();
         sh.j = same(lds.found);
     }
@@ -261,12 +265,12 @@ struct Segment {
 __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, const PlanLds &lds, const Share &sh,
                                                 uint32_t &u, uint32_t &j, uint32_t &kvh) {
     const uint32_t nkv = (uint32_t)a.kv.nkv;
-    const uint32_t *line = a.planned ? a.plan + PLAN_HEAD : lds.pre;
+    auto line = [&](uint32_t i) { return same(a.planned ? a.plan[PLAN_HEAD + i] : lds.pre[i]); };
     RowTile t = row_tile(a, lds, sh.n_seg, j);
     t.p0 = same(t.p0);
     t.p1 = same(t.p1);
     t.rt = same(t.rt);
-    uint32_t p = same(line[j]), e = same(line[j + 1]);
+    uint32_t p = line(j), e = line(j + 1);
     if (u >= tile_place(t, p, nkv, kvh) + (e - p)) { // past it: the sequence's next row tile, next head, or the next sequence
         if (e < t.p1) {
             j++;
@@ -283,8 +287,8 @@ __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, c
             t.p1 = same(t.p1);
             t.rt = 0;
         }
-        p = same(line[j]);
-        e = same(line[j + 1]);
+        p = line(j);
+        e = line(j + 1);
     }
     Segment s;
     s.kvh = kvh;

@@ -72,7 +72,8 @@ struct ChunkShape {
     static constexpr int KEYS = chunk_keys(D), HALVES = KEYS / 32; // positions of a tile; 32 x 32 score tiles
     static constexpr int TILE_BYTES = KEYS * RB;
     static constexpr int LOADS = TILE_BYTES / (256 * 16);     // 16-byte loads per thread and tile, of K and of V
-    static constexpr int LDS = 4 * TILE_BYTES;                // two buffers of each
+    static constexpr int OROW = 68;                           // floats of a row of 64 outputs there
+    static constexpr int OUT = CHUNK_ROWS * OROW * 4, LDS = 4 * TILE_BYTES > OUT ? 4 * TILE_BYTES : OUT; // two buffers of each
     // Which chunk of row r lies at place p: p ^ swizzle(r). A clock serves 256 bytes: of K 16 bytes of 16 rows, which all
     // have another value; of V 64 bytes of four rows, whose values differ above those four chunks. Linear: swizzle(x ^ y) =
     // swizzle(x) ^ swizzle(y).
@@ -83,6 +84,54 @@ struct ChunkShape {
 
 #define AQ_LDS __attribute__((address_space(3)))
 #define AQ_GLB __attribute__((address_space(1)))
+
+// Rows row0 + 8 i (i < 4) of a wave's 32, from w0 on: eight outputs each, at x + row * stride; times the gate, rounded,
+// stored. All four gates are on their way before the first is used.
+template <int CT>
+__device__ __forceinline__ void store_rows(const AttnPagedArgs &a, const SeqRows &sr, int kvh, int32_t w0, int32_t n_rows,
+                                           int dim, int row0, const float *x, int stride) {
+    using E = typename RowType<CT>::type;
+    typedef E vec __attribute__((ext_vector_type(8)));
+    int64_t row[4], head[4];
+    bool have[4];
+    vec gate[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int32_t rr = w0 + row0 + 8 * i, tok = (int32_t)a.by_g.quot(rr);
+        have[i] = rr < n_rows && dim < a.kv.hd;
+        row[i] = sr.first + tok;
+        head[i] = kvh * a.G + (rr - tok * a.G);
+        if (a.gate.p && have[i]) {
+            const E *g = (const E *)a.gate.p + row[i] * a.gate.row + head[i] * a.gate.head + dim;
+            if (a.out_wide) {
+                gate[i] = *reinterpret_cast<const vec *>(g);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) gate[i][e] = g[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const f4 u = *reinterpret_cast<const f4 *>(x + (row0 + 8 * i) * stride),
+                 v = *reinterpret_cast<const f4 *>(x + (row0 + 8 * i) * stride + 4);
+        vec y;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float z = e < 4 ? u[e & 3] : v[e & 3];
+            if (a.gate.p) z *= 1.0f / (1.0f + expf(-(float)gate[i][e]));
+            y[e] = (E)z;
+        }
+        if (!have[i]) continue;
+        E *o = (E *)a.out.p + row[i] * a.out.row + head[i] * a.out.head + dim;
+        if (a.out_wide) {
+            *reinterpret_cast<vec *>(o) = y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = y[e];
+        }
+    }
+}
 
 template <int CT, int D>
 __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
@@ -370,35 +419,49 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
             buf ^= 1;
         }
 
-        // ---- out: the whole segment's rows, or this share's part
+        // ---- out: the whole segment's rows, or this share's part, through the LDS so that neighbouring lanes have
+        // neighbouring values; each wave its own 32 rows, 64 dimensions a pass
         {
             const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
             l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
         }
-        if (!have) continue; // no barrier below in this pass
-        const int hs = here(h);
         const bool cut = is_cut(sg);
         const uint32_t slot = part_slot(sg, sh);
-        float *part = a.part_o + ((size_t)slot * R + 32 * wave + n) * D;
-        if (cut && hs == 0) {
+        const int ln = here(lane);
+        if (cut && have && h == 0) {
             float *ml = a.part_ml + ((size_t)slot * R + 32 * wave + n) * 2;
             ml[0] = mc;
             ml[1] = l;
         }
         const float inv = cut ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        constexpr int OROW = S::OROW;
+        float *mine = reinterpret_cast<float *>(smem) + wave * 32 * OROW;
+        __syncthreads(); // every wave is past its tiles
 #pragma unroll
-        for (int db = 0; db < DB; db++) {
-            const int d0 = here(4 * hs) + 32 * db;
+        for (int pass = 0; pass < D / 64; pass++) {
+            asm volatile("" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (d0 + 8 * i >= hd) break;
-                float out[4];
+            for (int i = 0; i < 8; i++) { // dimensions 8 i + 4 h .. of the pass
+                f4 x;
 #pragma unroll
-                for (int e = 0; e < 4; e++) out[e] = inv == 0.0f ? 0.0f : o[db][4 * i + e] * inv;
-                if (cut) *reinterpret_cast<f4 *>(part + d0 + 8 * i) = f4{out[0], out[1], out[2], out[3]};
-                else store_out<CT>(a, sr.first + tok, (int)sg.kvh * G + (rr - tok * G), d0 + 8 * i, out);
+                for (int e = 0; e < 4; e++) {
+                    const float y = o[2 * pass + i / 4][4 * (i % 4) + e];
+                    x[e] = inv == 0.0f ? 0.0f : y * inv;
+                }
+                *reinterpret_cast<f4 *>(mine + (ln & 31) * OROW + 8 * i + 4 * (ln >> 5)) = x;
             }
             asm volatile("" ::: "memory");
+            if (cut) { // 16 lanes a row
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int row = 4 * i + (ln >> 4), dim = 64 * pass + 4 * (ln & 15);
+                    const f4 x = *reinterpret_cast<const f4 *>(mine + row * OROW + 4 * (ln & 15));
+                    if (w0 + row < n_rows && dim < hd)
+                        *reinterpret_cast<f4 *>(a.part_o + ((size_t)slot * R + 32 * wave + row) * D + dim) = x;
+                }
+            } else { // 8 lanes a row
+                store_rows<CT>(a, sr, (int)sg.kvh, w0, n_rows, 64 * pass + 8 * (ln & 7), ln >> 3, mine + 8 * (ln & 7), OROW);
+            }
         }
     }
 }
