@@ -222,8 +222,12 @@ int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uin
     const uint64_t rows = (uint64_t)b->max_rows * G;
     c->D = kv->head_dim <= 64 ? 64 : kv->head_dim <= 128 ? 128 : 256;
     c->cap = (uint32_t)std::min<uint64_t>((uint64_t)b->max_pages * kv->page_size, b->max_len);
-    // 16-bit rows past what one pass of the few-row kernel holds
-    c->many = !f32_rows && rows > 32;
+    // Paged chunks for 16-bit rows past one row tile of the few-row kernel, once there is enough to do: its start (code,
+    // 128-row blocks) takes 12 to 30 us whatever the work, each further row tile of the other reads K and V again. Few-row
+    // and chunk kernel, by rows x heads x positions (bf16, us): heads of 256: 0.04M 13.6 and 29.2, 3.1M 37.7 and 43.3, 4.6M
+    // 40.7 and 43.9, 7.4M 54.6 and 48.7; of 128: 0.05M 9.8 and 18.2, 4.1M 27.4 and 30.0, 4.4M 30.9 and 30.0, 7.7M 41.9 and
+    // 38.5, 46M 211 and 136; of 64: 5.0M 22.2 and 24.2, 10M 30.0 and 26.1, 31M 81 and 59.
+    c->many = !f32_rows && rows > 32 && (double)b->n_rows * n_head * c->cap > 5.0 * (1 << 20);
     c->R = c->many ? CHUNK_ROWS : rows <= 16 ? 16 : 32;
     c->unit = c->many ? chunk_keys(c->D) : few_unit(kv->type, c->D, c->R);
     c->min_chunk = c->many ? 256 / c->unit : 1;
