@@ -23,7 +23,8 @@ struct FastDiv {
 // pool a device can hold.
 struct PagedKv {
     const char *k = nullptr, *v = nullptr;
-    uint32_t n_pages = 0, page_units = 0, slot_units = 0, unit_shift = 0, head_bytes = 0;
+    uint32_t n_pages = 0, page_units = 0, slot_units = 0, unit_shift = 0;
+    uint64_t head_bytes = 0;
     FastDiv page_size;
     int nkv = 0, hd = 0, type = 0;
 };

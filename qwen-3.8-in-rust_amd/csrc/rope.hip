@@ -64,7 +64,7 @@ int check_paged(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b
     while (sh < 40 && (pb | sb) && !(((pb | sb) >> sh) & 1)) sh++;
     const uint64_t pu = pb >> sh, su = sb >> sh;
     const double reach = (double)(kv->n_pages - 1) * (double)pu + (double)(kv->page_size - 1) * (double)su;
-    if (reach >= 4294967295.0 || (uint64_t)kv->head_stride * tb * kv->n_head_kv >= (1ull << 32))
+    if (reach >= 4294967295.0)
         return fail(AQ_EUNSUP, who + ": the pool reaches past 2^32 units of " + std::to_string(1ull << sh) + " bytes");
     AQ_REQUIRE(b->n_rows < (1u << 24) && b->n_seq < (1u << 24), who + ": batch size (fewer than 2^24 rows)");
     AQ_REQUIRE(b->n_seq == 0 || (b->row_start && b->kv_len && b->pages), who + ": null batch array");
@@ -77,7 +77,7 @@ int check_paged(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b
         out->page_units = (uint32_t)pu;
         out->slot_units = (uint32_t)su;
         out->unit_shift = sh;
-        out->head_bytes = (uint32_t)((uint64_t)kv->head_stride * tb);
+        out->head_bytes = (uint64_t)kv->head_stride * tb;
         out->page_size = FastDiv(kv->page_size);
         out->nkv = (int)kv->n_head_kv;
         out->hd = (int)kv->head_dim;
