@@ -81,19 +81,18 @@ __device__ __forceinline__ bool paged_slot(const PagedKv &c, const int32_t *tabl
     return paged_units(c, paged_entry(c, table, max_pages, pos), pos, units);
 }
 
-// The sequence that row `row` belongs to (n_seq: none): the number of sequences that end at or before it, counted by
-// the whole wave.
+// The sequence that row `row` belongs to (n_seq: none): the number of sequences that end at or before it. row_start never
+// falls, so the whole wave looks at the ends of 64 blocks of sequences, then inside the first that ends after the row.
 __device__ __forceinline__ uint32_t paged_seq_of(const PagedBatch &b, uint32_t row) {
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t seq = 0;
-    for (uint32_t s0 = 0; s0 < b.n_seq; s0 += 64) {
-        const uint32_t s = s0 + lane;
-        const bool before = s < b.n_seq && b.row_start[s + 1] <= (int32_t)row;
-        const uint32_t n = (uint32_t)__popcll(__ballot(before));
-        seq += n;
-        if (n < 64) break;
+    uint32_t lo = 0, hi = b.n_seq; // the answer is one of lo .. hi
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + 63) / 64, s = lo + lane * step;
+        const bool before = s < hi && b.row_start[min(s + step, hi)] <= (int32_t)row;
+        lo = min(lo + (uint32_t)__popcll(__ballot(before)) * step, hi);
+        hi = min(lo + step - 1, hi);
     }
-    return seq;
+    return lo;
 }
 
 // A sequence's rows within the batch's n_rows, whatever row_start holds, and its length.

@@ -113,7 +113,7 @@ void join_launch(const AttnPagedArgs &a, int R, int rows, hipStream_t stream) {
         const uint32_t y = (uint32_t)((rows + ROWS - 1) / ROWS);
         if (segs <= a.shares) join_kernel<QT, 256, D, 1, false><<<dim3(segs, y), 256, 0, stream>>>(a, R);
         else join_kernel<QT, 256, D, 1, true><<<dim3(a.shares, y), 256, 0, stream>>>(a, R);
-    } else if (segs * 16 <= a.shares) {
+    } else if (segs <= a.shares / 16) {
         join_kernel<QT, 1024, D, 1024 / (D / 4), false><<<dim3(segs, (uint32_t)rows), 1024, 0, stream>>>(a, R);
     } else if (segs <= a.shares) {
         join_kernel<QT, 256, D, 256 / (D / 4), false><<<dim3(segs, (uint32_t)rows), 256, 0, stream>>>(a, R);

@@ -126,6 +126,8 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
         const UnitRange range = tile_units(a, sr, r0, R, UNIT);
         const int32_t tok0 = (int32_t)a.by_g.quot(r0), tok1 = (int32_t)a.by_g.quot(min(r0 + R, n_rows) - 1);
         const int32_t kend = min(max(base + tok1 + 1, 0), (int32_t)a.cap);
+        // before this position nobody of the tile looks: there is no page there, whatever it holds
+        const int32_t kbegin = a.window ? (int32_t)max((int64_t)base + tok0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
         const int32_t min_hi = base + tok0 + 1;
         const int64_t max_lo = a.window ? (int64_t)base + tok1 + 1 - (int64_t)a.window : INT64_MIN;
         const int32_t *table = a.b.pages + (size_t)sg.seq * a.b.max_pages;
@@ -137,7 +139,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
         // where a tile's rows are: lane l has position l % TILE's page entry, then its place; bit l: it has a page
         auto entry = [&](int32_t t) {
             const int32_t p = t * TILE + lane % TILE;
-            return t < last_tile && p < kend ? paged_entry(a.kv, table, a.b.max_pages, (uint32_t)p) : 0xFFFFFFFFu;
+            return t < last_tile && p >= kbegin && p < kend ? paged_entry(a.kv, table, a.b.max_pages, (uint32_t)p) : 0xFFFFFFFFu;
         };
         auto locate = [&](int32_t t, uint32_t e, uint32_t *units) {
             const bool ok = paged_units(a.kv, e, (uint32_t)(t * TILE + lane % TILE), units);
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                             t[h] = __builtin_amdgcn_perm(v[c][2 * h + 1][jj / 2], v[c][2 * h][jj / 2], sel);
                         return t;
                     };
-                    if ((edge && tok0 < tok1) || NP > 1) {
+                    if ((edge && tok0 < tok1) || NP > 1) { // one token's rows all see what has a page
                         // Nor are infinities and NaN of positions that only some of the rows see, and an infinity times
                         // the pieces of one number is a NaN: such values are added position by position, to the rows
                         // that see them, by the probability's first piece, and taken out of the product of the others.

@@ -7,8 +7,8 @@
 // applies them to several heads of the row, so the 64-bit work (a product, a floor, a difference per pair) stays
 // below the memory time from four heads on.
 #include <cmath>
+#include <memory>
 #include <new>
-#include <vector>
 
 #include "paged.h"
 
@@ -22,15 +22,15 @@ struct aq_rope {
 namespace aq {
 
 int check_heads(const char *call, const char *what, const aq_heads *h, size_t n_rows, size_t n_heads, size_t head_dim) {
-    const std::string who = std::string(call) + ": " + what;
-    AQ_REQUIRE(h && h->data, who + ": null");
-    AQ_REQUIRE(row_type(h->type), who + ": type " + std::to_string(h->type) + " is not F32, F16 or BF16");
-    AQ_REQUIRE((uintptr_t)h->data % type_bytes(h->type) == 0, who + ": data is not aligned to its type");
+    auto who = [&] { return std::string(call) + ": " + what; };
+    AQ_REQUIRE(h && (h->data || n_rows == 0), who() + ": null");
+    AQ_REQUIRE(row_type(h->type), who() + ": type " + std::to_string(h->type) + " is not F32, F16 or BF16");
+    AQ_REQUIRE((uintptr_t)h->data % type_bytes(h->type) == 0, who() + ": data is not aligned to its type");
     AQ_REQUIRE(h->row_stride >= 0 && h->head_stride >= 0 && h->row_stride < ((int64_t)1 << 40) &&
                    h->head_stride < ((int64_t)1 << 40),
-               who + ": strides");
-    AQ_REQUIRE(n_heads <= 1 || h->head_stride >= (int64_t)head_dim, who + ": heads overlap");
-    AQ_REQUIRE(n_rows <= 1 || h->row_stride >= (int64_t)head_dim, who + ": rows overlap");
+               who() + ": strides");
+    AQ_REQUIRE(n_heads <= 1 || h->head_stride >= (int64_t)head_dim, who() + ": heads overlap");
+    AQ_REQUIRE(n_rows <= 1 || h->row_stride >= (int64_t)head_dim, who() + ": rows overlap");
     return 0;
 }
 
@@ -41,23 +41,23 @@ bool heads_aligned(const aq_heads *h, size_t n_rows, size_t n_heads) {
 }
 
 int check_paged(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, PagedKv *out, PagedBatch *bout) {
-    const std::string who(call);
-    AQ_REQUIRE(kv && b, who + ": null argument");
-    AQ_REQUIRE(kv->k && kv->v, who + ": null k or v pages");
-    AQ_REQUIRE(row_type(kv->type), who + ": cache type " + std::to_string(kv->type) + " is not F32, F16 or BF16");
+    auto who = [&] { return std::string(call); };
+    AQ_REQUIRE(kv && b, who() + ": null argument");
+    AQ_REQUIRE(kv->k && kv->v, who() + ": null k or v pages");
+    AQ_REQUIRE(row_type(kv->type), who() + ": cache type " + std::to_string(kv->type) + " is not F32, F16 or BF16");
     AQ_REQUIRE(kv->n_pages > 0 && kv->n_pages < (1u << 31) && kv->page_size > 0 && kv->page_size < (1u << 31),
-               who + ": pages");
-    AQ_REQUIRE(kv->n_head_kv > 0 && kv->n_head_kv <= 65535, who + ": n_head_kv");
+               who() + ": pages");
+    AQ_REQUIRE(kv->n_head_kv > 0 && kv->n_head_kv <= 65535, who() + ": n_head_kv");
     if (kv->head_dim == 0 || kv->head_dim > 256 || kv->head_dim % 8)
-        return fail(AQ_EUNSUP, who + ": head_dim " + std::to_string(kv->head_dim) + " (a multiple of 8, at most 256)");
+        return fail(AQ_EUNSUP, who() + ": head_dim " + std::to_string(kv->head_dim) + " (a multiple of 8, at most 256)");
     const int64_t tb = (int64_t)type_bytes(kv->type), lim = (int64_t)1 << 40;
-    AQ_REQUIRE((uintptr_t)kv->k % 16 == 0 && (uintptr_t)kv->v % 16 == 0, who + ": pages are not 16-byte aligned");
+    AQ_REQUIRE((uintptr_t)kv->k % 16 == 0 && (uintptr_t)kv->v % 16 == 0, who() + ": pages are not 16-byte aligned");
     const int64_t st[3] = {kv->page_stride, kv->slot_stride, kv->head_stride};
     for (int i = 0; i < 3; i++)
-        AQ_REQUIRE(st[i] >= 0 && st[i] < lim && st[i] * tb % 16 == 0, who + ": page strides (multiples of 16 bytes)");
-    AQ_REQUIRE(kv->n_head_kv == 1 || kv->head_stride >= (int64_t)kv->head_dim, who + ": heads of a page overlap");
-    AQ_REQUIRE(kv->page_size == 1 || kv->slot_stride >= (int64_t)kv->head_dim, who + ": slots of a page overlap");
-    AQ_REQUIRE(kv->n_pages == 1 || kv->page_stride >= (int64_t)kv->head_dim, who + ": pages overlap");
+        AQ_REQUIRE(st[i] >= 0 && st[i] < lim && st[i] * tb % 16 == 0, who() + ": page strides (multiples of 16 bytes)");
+    AQ_REQUIRE(kv->n_head_kv == 1 || kv->head_stride >= (int64_t)kv->head_dim, who() + ": heads of a page overlap");
+    AQ_REQUIRE(kv->page_size == 1 || kv->slot_stride >= (int64_t)kv->head_dim, who() + ": slots of a page overlap");
+    AQ_REQUIRE(kv->n_pages == 1 || kv->page_stride >= (int64_t)kv->head_dim, who() + ": pages overlap");
     const uint64_t pb = kv->n_pages > 1 ? (uint64_t)kv->page_stride * tb : 0,
                    sb = kv->page_size > 1 ? (uint64_t)kv->slot_stride * tb : 0;
     uint32_t sh = 4;
@@ -65,11 +65,12 @@ int check_paged(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b
     const uint64_t pu = pb >> sh, su = sb >> sh;
     const double reach = (double)(kv->n_pages - 1) * (double)pu + (double)(kv->page_size - 1) * (double)su;
     if (reach >= 4294967295.0)
-        return fail(AQ_EUNSUP, who + ": the pool reaches past 2^32 units of " + std::to_string(1ull << sh) + " bytes");
-    AQ_REQUIRE(b->n_rows < (1u << 24) && b->n_seq < (1u << 24), who + ": batch size (fewer than 2^24 rows)");
-    AQ_REQUIRE(b->n_seq == 0 || (b->row_start && b->kv_len && b->pages), who + ": null batch array");
-    AQ_REQUIRE(b->n_seq == 0 || b->max_pages > 0, who + ": max_pages");
-    AQ_REQUIRE((uint64_t)b->max_pages * kv->page_size < (1ull << 31), who + ": the page table reaches past 2^31 positions");
+        return fail(AQ_EUNSUP, who() + ": the pool reaches past 2^32 units of " + std::to_string(1ull << sh) + " bytes");
+    AQ_REQUIRE(b->n_rows < (1u << 24) && b->n_seq < (1u << 24), who() + ": batch size (fewer than 2^24 rows)");
+    AQ_REQUIRE(b->n_seq == 0 || (b->row_start && b->kv_len && b->pages), who() + ": null batch array");
+    AQ_REQUIRE(b->n_seq == 0 || b->max_pages > 0, who() + ": max_pages");
+    AQ_REQUIRE((uint64_t)b->max_pages * kv->page_size <= (1ull << 31) - 1024,
+               who() + ": the page table reaches past 2^31 positions");
     if (out) {
         out->k = (const char *)kv->k;
         out->v = (const char *)kv->v;
@@ -339,7 +340,8 @@ int aq_rope_new(aq_ctx *ctx, const aq_rope_config *c, aq_rope **out) {
         gain = c->attn_factor > 0 ? c->attn_factor
                                   : (c->factor <= 1.0f ? 1.0f : (float)(0.1 * std::log((double)c->factor) + 1.0));
     }
-    std::vector<double> f(half);
+    std::unique_ptr<double[]> f(new (std::nothrow) double[half]);
+    if (!f) return fail(AQ_ENOMEM, "aq_rope_new: host memory");
     for (uint32_t i = 0; i < half; i++) {
         f[i] = std::pow((double)c->theta, -2.0 * i / c->dim);
         if (c->scaling == AQ_ROPE_LINEAR) f[i] /= (double)c->factor;
@@ -360,7 +362,7 @@ int aq_rope_new(aq_ctx *ctx, const aq_rope_config *c, aq_rope **out) {
         delete r;
         return fail(AQ_ENOMEM, "aq_rope_new: hipMalloc");
     }
-    hipError_t e = hipMemcpyAsync(r->freq, f.data(), half * sizeof(double), hipMemcpyHostToDevice, ctx->stream);
+    hipError_t e = hipMemcpyAsync(r->freq, f.get(), half * sizeof(double), hipMemcpyHostToDevice, ctx->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) {
         (void)hipFree(r->freq);

@@ -149,7 +149,7 @@ def test_holes(ctx, row_t, cache_t, new):
 
 
 @pytest.mark.parametrize("row_t,cache_t", PAIRS)
-@pytest.mark.parametrize("new,window", [(4, 0), (4, 6), (60, 0), (60, 40)])
+@pytest.mark.parametrize("new,window", [(1, 0), (1, 6), (4, 0), (4, 6), (60, 0), (60, 40)])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
 def test_what_a_row_does_not_see_never_reaches_it(ctx, row_t, cache_t, new, window, bad):
     """Values and keys that are not finite, at positions that only some rows of a tile see: the others are as without
@@ -158,8 +158,12 @@ def test_what_a_row_does_not_see_never_reaches_it(ctx, row_t, cache_t, new, wind
     rng = np.random.default_rng(11)
     pg = P.Paged(ctx, rng, [new], [150], 2, 128, 16, cache_t)
     at = [150 - 1, 150 - new // 2, 150 - new - 3]  # the last row's alone; half the rows'; all (or the window's)
+    if new == 1:
+        at = [150 - 1, 150, 150 - 8]  # its own; past it; all positions but the window's
     for i, p in enumerate(at):
         pg.v[pg.row_of(0, p)][i % 2, 5 + 40 * i] = bad
+    if window:
+        pg.k[pg.row_of(0, 150 - new - window)] = bad  # before all windows
     pg.upload()
     q = P.Rows(ctx, rng.standard_normal((new, 4, 128)), row_t)
     want, parts = P.attention(pg, q.values(), 0.08, window)

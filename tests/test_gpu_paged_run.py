@@ -344,3 +344,38 @@ def test_rows_past_the_bounds_stay(ctx, row_t, cache_t, new):
     ctx.sync()
     got = out.get()
     assert np.all(got[n:] == 9.0) and np.all(np.abs(got - want)[: 2 * new] <= limit[: 2 * new])
+
+
+@pytest.mark.parametrize("n_seq", [1, 64, 65, 4096, 5000])
+def test_append_of_many_sequences(ctx, n_seq):
+    """Each row finds its sequence among thousands, empty ones between them; rows behind the last store nothing."""
+    print(f"append of {n_seq} sequences", flush=True)
+    rng = np.random.default_rng(n_seq)
+    new = [int(n) for n in rng.integers(0, 3, n_seq)]
+    new[-1] = 2
+    lens = [int(n + x) for n, x in zip(new, rng.integers(0, 9, n_seq))]
+    pg = P.Paged(ctx, rng, new, lens, 1, 8, 4, "f32", n_rows=sum(new) + 5)
+    k, v = (P.Rows(ctx, rng.standard_normal((pg.rows, 1, 8)), "f32") for _ in range(2))
+    want = [pg.k.copy(), pg.v.copy()]
+    for s in range(n_seq):
+        for i in range(new[s]):
+            at = pg.row_of(s, lens[s] - new[s] + i)
+            want[0][at], want[1][at] = k.values()[pg.starts[s] + i], v.values()[pg.starts[s] + i]
+    cache, batch = pg.structs()
+    aq.paged_append(ctx, cache, batch, k.heads_struct(), v.heads_struct())
+    ctx.sync()
+    for a, b in zip(pg.pools(), want):
+        assert np.array_equal(a, b, equal_nan=True)
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("new", [1, 40])
+def test_no_positions_at_all(ctx, row_t, cache_t, new):
+    """max_len 0: every row is 0."""
+    pg = P.Paged(ctx, np.random.default_rng(1), [new, new], [0, 0], 2, 64, 16, cache_t, max_len=0)
+    q, out = (P.Rows(ctx, np.full((pg.rows, 4, 64), x), row_t) for x in (1.0, 9.0))
+    cache, batch = pg.structs()
+    ws = aq.DeviceBuffer(ctx, aq.paged_attention_workspace(ctx, cache, batch, 4))
+    aq.paged_attention(ctx, cache, batch, 4, q.heads_struct(), out.heads_struct(), 0.125, 0, None, ws)
+    ctx.sync()
+    assert np.all(out.get() == 0.0)

@@ -180,3 +180,20 @@ def test_attention(ctx):
     aq.paged_attention(ctx, good_kv(), good_batch(n_rows=0), 4, rows(heads=4), rows(heads=4), 0.1)  # nothing to do
     assert aq.lib().aq_paged_attention(None, *[None] * 2, 4, None, None, 0.1, 0, None, None, 0, None) == aq.AQ_EINVAL
     assert aq.lib().aq_paged_attention_workspace(ctx.h, C.byref(good_kv()), C.byref(good_batch()), 4, None) == aq.AQ_EINVAL
+
+
+def test_empty_batches_need_no_rows(ctx):
+    """Row tensors without rows may have no address."""
+    none, batch = rows(data=None), good_batch(n_rows=0)
+    aq.paged_append(ctx, good_kv(), batch, none, none)
+    aq.paged_append(ctx, good_kv(), batch, none, none, FakeRope(ctx, 64), none, none, 2)
+    aq.paged_attention(ctx, good_kv(), batch, 2, none, none, 0.1, 0, none)
+    aq.rope_apply(FakeRope(ctx, 64), none, none, 0, 2, 64, None)
+
+
+def test_reach_of_a_table(ctx):
+    """Up to 2^31 - 1024 positions; heads any distance apart."""
+    most = ((1 << 31) - 1024) // 16
+    assert aq.paged_attention_workspace(ctx, good_kv(), good_batch(max_pages=most), 4) > 0
+    refused(aq.AQ_EINVAL, "2^31 positions", aq.paged_attention_workspace, ctx, good_kv(), good_batch(max_pages=most + 1), 4)
+    assert aq.paged_attention_workspace(ctx, good_kv(head_stride=1 << 39), good_batch(), 4) > 0
