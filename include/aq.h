@@ -257,12 +257,12 @@ typedef struct aq_rope_config {
     float attn_factor;   /* YARN: multiplies cos and sin (0: 1 + 0.1 ln factor, or 1 for a factor below 1) */
 } aq_rope_config;
 
-/* The rotation's frequencies on the device (`RopeTable`-like state of rope.rs:10-28, without its position limit:
- * angles are computed in 64 bits for any 32-bit position). Usable from any stream of the context's device. */
+/* The rotation's frequencies on the device (`inv_freq`, rope.rs:10-16; angles are computed in 64 bits for
+ * any 32-bit position). Usable from any stream of the context's device. */
 typedef struct aq_rope aq_rope;
 int aq_rope_new(aq_ctx *ctx, const aq_rope_config *cfg, aq_rope **out);
 int aq_rope_free(aq_rope *r);
-/* y[r][h] = x[r][h] rotated by pos_dev[r] (`rope_apply`, rope.rs:31-45); inverse != 0 rotates back (times the same
+/* y[r][h] = x[r][h] rotated by pos_dev[r] (`apply_rope`, rope.rs:31-45); inverse != 0 rotates back (times the same
  * attn_factor): the gradient of the rotation, and cached keys moved to other positions. y may be x (same strides), and
  * else must not overlap it. Same type on both sides. */
 int aq_rope_apply(const aq_rope *r, const aq_heads *x, const aq_heads *y, size_t n_rows, size_t n_heads, size_t head_dim,

@@ -763,7 +763,7 @@ def paged_batch(n_seq, row_start, kv_len, pages, max_pages, n_rows, max_rows, ma
 
 
 class Rope:
-    """aq_rope: a rotation's frequencies on the device (rope.rs:10-28); layout "half" or "interleaved", scaling "none",
+    """aq_rope: a rotation's frequencies on the device (rope.rs:10-16); layout "half" or "interleaved", scaling "none",
     "linear" or "yarn"."""
     LAYOUTS = {"half": 0, "interleaved": 1}
     SCALINGS = {"none": 0, "linear": 1, "yarn": 2}

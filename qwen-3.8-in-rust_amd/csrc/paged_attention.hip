@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnPagedArgs a, int R) {
 }
 
 // Few rows: a work-group per row, of 1024 threads where a row has many parts (a long context of one sequence has hundreds:
-// 24 rows of 63 parts of 256 dimensions take 5.1 us, with 256 threads 10.4). Many rows: 256 threads, a row per D / 4 of
+// 24 rows of 63 parts of 256 dimensions take 5.9 us, with 256 threads 9.9). Many rows: 256 threads, a row per D / 4 of
 // them, its two to a few parts one after the other.
 template <int QT, int D>
 void join_launch(const AttnPagedArgs &a, int R, int rows, hipStream_t stream) {

@@ -7,10 +7,9 @@
 // sees are work.
 //
 // Split. All segments' units in order (sequence, K/V head, row tile, key unit: row tiles that read the same keys side by
-// side, on one XCD at one time), each segment's with `lead` places before
-// them for what a segment costs besides its units, form one line of `total` places, cut into work-group shares of `chunk`
-// places each, however long or short the sequences are. A share that holds a whole segment
-// writes its output; where a segment is cut, each share writes its part (row maxima, sums and unnormalised outputs, in
+// side, on one XCD at one time), each segment's with `lead` places before them for what a segment costs besides its units,
+// form one line of `total` places, cut into work-group shares of `chunk` places each, however long or short the sequences
+// are. A share that holds a whole segment writes its output; where a segment is cut, each share writes its part (row maxima, sums and unnormalised outputs, in
 // f32) to the workspace, slot 2w for the segment that began before share w, slot 2w + 1 for the one that goes on after
 // it, and a second launch joins the parts in order. Which share has which part follows from the lengths alone, so the
 // same call gives the same bits.
@@ -388,8 +387,8 @@ constexpr int WAVES = 4;
 
 // Positions that a wave of the few-row kernel takes at once: 32, and 16 of a wide head, whose rows fill the registers.
 constexpr int few_tile(int D) { return D == 256 ? 16 : 32; }
-// The rows (16 or 32) lie on a wave's NR accumulator tiles; 32 rows of a wide head would not fit its registers, so there two waves take 16 rows
-// each over the same positions (RG = 2: the second reads them from the cache the first filled).
+// The rows (16 or 32) lie on a wave's NR accumulator tiles; 32 rows of a wide head would not fit its registers, so there two
+// waves take 16 rows each over the same positions (RG = 2: the second reads them from the cache the first filled).
 constexpr int few_groups(int CT, int D, int R) { return R == 32 && (D == 256 || (CT == AQ_TYPE_F32 && D == 128)) ? 2 : 1; }
 constexpr int few_unit(int CT, int D, int R) { return WAVES / few_groups(CT, D, R) * few_tile(D); }
 
