@@ -305,8 +305,9 @@ int aq_paged_append(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *ba
  * never reaches it, infinities and NaN included. q, gate and out have one type: F32, or the cache's; F32 rows over a
  * 16-bit cache keep 32-bit accuracy (queries and probabilities go through the matrix cores in pieces). out may be q or
  * gate (same strides), and else must not overlap what the call reads. scale > 0.
- * workspace: aq_paged_attention_workspace bytes of device memory for these arguments, 16-byte aligned, contents
- * irrelevant before and after; calls (and captured graphs) that can run at the same time need one each. */
+ * workspace: aq_paged_attention_workspace bytes of device memory for these arguments (those for a batch's largest bounds
+ * serve every batch within them), 16-byte aligned, contents irrelevant before and after; calls (and captured graphs)
+ * that can run at the same time need one each. */
 int aq_paged_attention_workspace(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, uint32_t n_head,
                                  size_t *bytes);
 int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, uint32_t n_head,

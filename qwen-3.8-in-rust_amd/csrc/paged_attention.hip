@@ -211,7 +211,7 @@ int compute_units(int device) {
 struct Choice {
     bool many = false; // paged_chunk.hip
     int R = 16, D = 64;
-    uint32_t unit = 0, shares = 0, min_chunk = 1, lead = 0, n_seg = 0, cap = 0;
+    uint32_t unit = 0, shares = 0, min_chunk = 1, lead = 0, whole = 0, n_seg = 0, cap = 0;
     bool planned = false, join = false;
     PagedSpace space;
 };
@@ -250,8 +250,19 @@ int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uin
     const uint64_t per_cu = !c->many && c->R == 16 && kv->type != AQ_TYPE_F32 ? 1 : 2;
     const uint64_t units = n_seg * kv->n_head_kv * per, shares = std::min<uint64_t>((uint64_t)compute_units(device) * per_cu, units);
     c->shares = (uint32_t)(shares > 8 ? (shares + 7) / 8 * 8 : std::max<uint64_t>(shares, 1));
-    c->join = c->cap > c->unit; // else no segment has a second unit
     c->space = paged_space(c->shares, c->n_seg, (size_t)c->R, (size_t)c->D);
+    // Short contexts: a share to each segment, and no join, whose launch costs as much as three or four units. Line and whole
+    // segments (us): one sequence of 32 heads on 8 of 128 (bf16) at 150: 11.2 and 8.4, at 300: 11.2 and 10.1, at 500: 11.3
+    // and 11.5; 64 of them at 150: 27.5 and 16.6, at 300: 37.2 and 26.2, at 500: 44.6 and 43.9, at 800: 59.0 and 65.0; 24
+    // heads on 4 of 256 (f16), one at 150: 12.1 and 11.0, at 300: 13.2 and 13.5. Not where two waves share a unit (32 rows
+    // of 256 at 150: 14.3 and 18.2), nor with more segments than measured (1536).
+    const uint64_t segs = n_seg * kv->n_head_kv, cus = (uint64_t)compute_units(device);
+    if (!c->many && !c->planned && few_groups(kv->type, c->D, c->R) == 1 && segs <= 8 * cus &&
+        c->cap <= (c->D == 256 ? 256u : segs >= cus ? 512u : 384u)) {
+        c->whole = (uint32_t)per;
+        c->shares = (uint32_t)(segs > 8 ? (segs + 7) / 8 * 8 : segs);
+    }
+    c->join = !c->whole && c->cap > c->unit; // else no segment has a second unit
     return 0;
 }
 
@@ -344,6 +355,7 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
     a.shares = c.shares;
     a.min_chunk = c.min_chunk;
     a.lead = c.lead;
+    a.whole = c.whole;
     a.n_seg = c.n_seg;
     a.planned = c.planned;
     char *ws = (char *)workspace;

@@ -9,7 +9,7 @@
 // Split. All segments' units in order (sequence, K/V head, row tile, key unit: row tiles that read the same keys side by
 // side, on one XCD at one time), each segment's with `lead` places before them for what a segment costs besides its units,
 // form one line of `total` places, cut into work-group shares of `chunk` places each, however long or short the sequences
-// are. A share that holds a whole segment writes its output; where a segment is cut, each share writes its part (row maxima, sums and unnormalised outputs, in
+// are (short contexts: every segment has `whole` places and is a share). A share that holds a whole segment writes its output; where a segment is cut, each share writes its part (row maxima, sums and unnormalised outputs, in
 // f32) to the workspace, slot 2w for the segment that began before share w, slot 2w + 1 for the one that goes on after
 // it, and a second launch joins the parts in order. Which share has which part follows from the lengths alone, so the
 // same call gives the same bits.
@@ -35,6 +35,7 @@ struct AttnPagedArgs {
     float scale_log2;          // scale * log2(e)
     uint32_t q_wide, out_wide; // 16-byte loads of q; 4-value stores of out and loads of gate
     uint32_t shares, min_chunk, lead; // work-groups; least places of a share; places before a segment's units
+    uint32_t whole;   // places of every segment, where each share is one whole segment; 0: as many as it has units, and cut
     uint32_t n_seg;   // row tiles of all sequences at most
     uint32_t planned; // 1: a plan launch has filled plan and tiles; 0: the work-groups divide by themselves
     // workspace
@@ -140,6 +141,7 @@ __device__ __forceinline__ uint32_t seq_tiles(const AttnPagedArgs &a, uint32_t s
     return s < a.b.n_seq ? (uint32_t)((paged_seq(a.b, s).n * a.G + R - 1) / R) : 0u;
 }
 __device__ __forceinline__ uint32_t tile_count(const AttnPagedArgs &a, uint32_t s, uint32_t rt, int R, uint32_t tk) {
+    if (a.whole) return a.whole;
     const UnitRange u = tile_units(a, paged_seq(a.b, s), (int32_t)rt * R, R, tk);
     return u.hi - u.lo + a.lead;
 }
@@ -214,7 +216,7 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
             n_seg = same(n_seg);
             total = same(lds.pre[n_seg]) * nkv;
         }
-        chunk = share_chunk(total, a.shares, a.min_chunk);
+        chunk = a.whole ? a.whole : share_chunk(total, a.shares, a.min_chunk);
         if (blockIdx.x == 0) { // for the join
             if (tid == 0) {
                 a.plan[0] = total;
@@ -261,7 +263,7 @@ struct Segment {
     uint32_t kvh, seq, cnt;
     int32_t t0, t1, r0;
 };
-__device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, const PlanLds &lds, const Share &sh,
+__device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, uint32_t tk, const PlanLds &lds, const Share &sh,
                                                 uint32_t &u, uint32_t &j, uint32_t &kvh) {
     const uint32_t nkv = (uint32_t)a.kv.nkv;
     auto line = [&](uint32_t i) { return same(a.planned ? a.plan[PLAN_HEAD + i] : lds.pre[i]); };
@@ -298,6 +300,11 @@ __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, c
     u += to - from;
     s.seq = same(t.seq);
     s.r0 = (int32_t)t.rt * R;
+    if (a.whole) {
+        const UnitRange range = tile_units(a, paged_seq(a.b, s.seq), s.r0, R, tk);
+        s.t0 = 0;
+        s.t1 = (int32_t)(s.cnt = range.hi - range.lo);
+    }
     return s;
 }
 // Whether other shares have units of it too, and then the slot of this share's part.

@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
     const Share sh = take_share(a, R, UNIT, plan);
     uint32_t u = sh.begin, j = sh.j, kv_at = sh.kvh;
     while (u < sh.end) { // uniform
-        const Segment sg = next_segment(a, R, plan, sh, u, j, kv_at);
+        const Segment sg = next_segment(a, R, UNIT, plan, sh, u, j, kv_at);
         if (sg.t1 <= sg.t0) continue;
         const uint32_t kvh = sg.kvh;
         const int32_t r0 = sg.r0;

@@ -21,18 +21,21 @@ def ctx():
 
 
 ENOUGH = 5 << 20  # rows x heads x positions past which many 16-bit rows go to a kernel of their own
+SHORT = 512       # positions up to which a work-group may have whole sequences
 
 
 def bounds(pg, q):
-    """The batch's bounds as they are and, where that changes the kernel, with wide tables and a large max_len."""
-    many = q.t != "f32" and pg.max_rows * (q.heads // pg.kv) > 32
-    return (False, True) if many and pg.rows * q.heads * min(pg.max_len, pg.cols * pg.page) <= ENOUGH else (False,)
+    """The batch's bounds as they are and, where that changes the kernel or the division of the work, with wide tables and
+    a large max_len."""
+    reach = min(pg.max_len, pg.cols * pg.page)
+    many = q.t != "f32" and pg.max_rows * (q.heads // pg.kv) > 32 and pg.rows * q.heads * reach <= ENOUGH
+    return (False, True) if many or reach <= SHORT else (False,)
 
 
 def run(ctx, pg, q, out, scale, window=0, gate=None, stream=None, sync=True, loose=False):
     cache, batch = pg.structs()
     if loose:
-        positions = ENOUGH // (pg.rows * q.heads) + 1
+        positions = max(ENOUGH // (pg.rows * q.heads) + 1, 4 * SHORT)
         wide = P.Dev(ctx, np.full((len(pg.lens), max(pg.cols, -(-positions // pg.page))), 10 ** 9, np.int32))
         wide.buf.upload(np.concatenate([pg.table, wide.get()[:, pg.cols:]], 1))
         batch = aq.paged_batch(len(pg.lens), pg.dstarts.buf, pg.dlens.buf, wide.buf, wide.shape[1], pg.rows, pg.max_rows,

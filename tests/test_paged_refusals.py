@@ -197,3 +197,25 @@ def test_reach_of_a_table(ctx):
     assert aq.paged_attention_workspace(ctx, good_kv(), good_batch(max_pages=most), 4) > 0
     refused(aq.AQ_EINVAL, "2^31 positions", aq.paged_attention_workspace, ctx, good_kv(), good_batch(max_pages=most + 1), 4)
     assert aq.paged_attention_workspace(ctx, good_kv(head_stride=1 << 39), good_batch(), 4) > 0
+
+
+def test_workspace_of_larger_bounds_serves_smaller_batches(ctx):
+    """A workspace made for a batch's largest bounds is enough for every batch within them."""
+    import random
+    rng = random.Random(1)
+
+    def need(n_seq, per_seq, max_len, kv, heads):
+        batch = good_batch(n_seq=n_seq, n_rows=n_seq * per_seq, max_rows=per_seq, max_pages=1 << 12, max_len=max_len)
+        return aq.paged_attention_workspace(ctx, kv, batch, heads)
+
+    def log(lo, hi):
+        return int(round(lo * (hi / lo) ** rng.random()))
+
+    for _ in range(4000):
+        n_kv = rng.choice([1, 2, 4, 8])
+        kv = good_kv(n_head_kv=n_kv, head_dim=rng.choice([64, 80, 128, 192, 256]), type=rng.choice([aq.F32, aq.F16, aq.BF16]))
+        heads = n_kv * rng.choice([1, 2, 4, 6, 12])
+        n_seq = log(1, 3000)
+        big = [n_seq, log(1, max(30000 // n_seq, 1)), log(1, 60000)]
+        small = [log(1, b) for b in big]
+        assert need(*small, kv, heads) <= need(*big, kv, heads), (small, big, kv.type, kv.head_dim, n_kv, heads)
