@@ -103,8 +103,10 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnPagedArgs a, int R) {
 }
 
 // Few rows: a work-group per row, of 1024 threads where a row has many parts (a long context of one sequence has hundreds:
-// 24 rows of 63 parts of 256 dimensions take 5.9 us, with 256 threads 9.9). Many rows: 256 threads, a row per D / 4 of
-// them, its two to a few parts one after the other.
+// 24 rows of 63 parts of 256 dimensions take 5.9 us, with 256 threads 9.9); with more segments than shares 512 threads on
+// 512 / D rows, most of which have two parts or are whole (work-groups of 256 on a row each: f32 prompts of four requests of
+// 500, 16 heads on 2 of 64, 71.4 us in all for 55.1). Many rows: 256 threads, a row per D / 4 of them, its two to a few
+// parts one after the other.
 template <int QT, int D>
 void join_launch(const AttnPagedArgs &a, int R, int rows, hipStream_t stream) {
     const uint32_t segs = a.n_seg * (uint32_t)a.kv.nkv;
@@ -118,7 +120,8 @@ void join_launch(const AttnPagedArgs &a, int R, int rows, hipStream_t stream) {
     } else if (segs <= a.shares) {
         join_kernel<QT, 256, D, 256 / (D / 4), false><<<dim3(segs, (uint32_t)rows), 256, 0, stream>>>(a, R);
     } else {
-        join_kernel<QT, 256, D, 256 / (D / 4), true><<<dim3(a.shares, (uint32_t)rows), 256, 0, stream>>>(a, R);
+        constexpr int ROWS = 512 / D;
+        join_kernel<QT, 512, D, 4, true><<<dim3(a.shares, (uint32_t)((rows + ROWS - 1) / ROWS)), 512, 0, stream>>>(a, R);
     }
 }
 template <int QT>

@@ -259,6 +259,7 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
 
 // The next segment of a share, from place u on (row tile j on K/V head kvh, or the one after it): the sequence, its first
 // row, the units t0 .. t1 - 1 of the segment's cnt that are the share's (none: t1 <= t0). Advances u, j and kvh. All uniform.
+// tk: the unit, 0 where a share is never a whole segment by itself.
 struct Segment {
     uint32_t kvh, seq, cnt;
     int32_t t0, t1, r0;
@@ -300,7 +301,7 @@ __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, u
     u += to - from;
     s.seq = same(t.seq);
     s.r0 = (int32_t)t.rt * R;
-    if (a.whole) {
+    if (tk && a.whole) {
         const UnitRange range = tile_units(a, paged_seq(a.b, s.seq), s.r0, R, tk);
         s.t0 = 0;
         s.t1 = (int32_t)(s.cnt = range.hi - range.lo);

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
     const Share sh = take_share(a, R, KEYS, plan);
     uint32_t u = sh.begin, j = sh.j, kv_at = sh.kvh;
     while (u < sh.end) { // uniform
-        const Segment sg = next_segment(a, R, KEYS, plan, sh, u, j, kv_at);
+        const Segment sg = next_segment(a, R, 0, plan, sh, u, j, kv_at);
         if (sg.t1 <= sg.t0) continue;
         const int n = here(n0), h = here(h0);
         const SeqRows sr = paged_seq(a.b, sg.seq);
