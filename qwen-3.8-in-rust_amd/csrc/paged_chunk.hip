@@ -15,8 +15,8 @@
 // which 16 bytes of its row it fetches: the row's chunks are swapped by an exclusive or with the row's low bits, so that
 // neither kind of read meets a bank twice. Rows without a page come from a row of zeros.
 //
-// Measured: 512 rows of 24 heads on 4 of 256 at 32,000 (bf16) 487 us, 833 TFLOP/s, where a library product of 8192^3 reaches
-// 1121; prompts of three requests of 3500, 32 heads on 8 of 128 (f16), 423 us, 716. Products and softmax (per score a
+// Measured: 512 rows of 24 heads on 4 of 256 at 32,000 (bf16) 479 us, 847 TFLOP/s, where a library product of 8192^3 reaches
+// 1121; prompts of three requests of 3500, 32 heads on 8 of 128 (f16), 412 us, 734. Products and softmax (per score a
 // product, an exponential, a rounding, half a sum) take turns on two waves a SIMD; the next tile's products put beside
 // this one's softmax need the registers that hold the rows (770 for 792).
 #include <atomic>

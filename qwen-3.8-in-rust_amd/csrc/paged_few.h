@@ -12,8 +12,8 @@
 // One running maximum and sum per row; a wave's four lane groups share the maximum, the sum is joined at the end.
 //
 // Measured: single tokens of 48 sequences at 6000 (bf16, 32 heads on 8 of 128) 215 us, 5.5 TB/s, where a plain read reaches
-// 6.3; of one sequence at 8000 (f16, 24 heads on 4 of 256) 17.5 us, two launches of latencies; four new tokens of eight
-// sequences at 3000 (f32 over f16, the same heads) 42.5 us, 2.5 TB/s: its 16 rows of 256 outputs leave registers for two
+// 6.3; of one sequence at 8000 (f16, 24 heads on 4 of 256) 17.8 us, two launches of latencies; four new tokens of eight
+// sequences at 3000 (f32 over f16, the same heads) 42.7 us, 2.5 TB/s: its 16 rows of 256 outputs leave registers for two
 // waves a SIMD, which wait for loads 56% of their time. Eight waves to a work-group there: 40.4 us, but contexts below 1000
 // 1 to 2 us slower and single tokens 5 to 8%.
 //

@@ -7,8 +7,8 @@
 // applies them to several heads of the row, so the 64-bit work (a product, a floor, a difference per pair) stays
 // below the memory time from four heads on.
 //
-// Bound by their bytes: 8191 rows of 40 heads of 128 (bf16) 34.2 us, 4.9 TB/s where a copy reaches 5.3; 6000 new rows of 24
-// query and 4 K/V heads of 256 (f32 into f16) appended in 65.4 us, 5.0 TB/s; 48 single tokens 5.0 us, an empty launch 2.4.
+// Bound by their bytes: 8191 rows of 40 heads of 128 (bf16) 34.1 us, 4.9 TB/s where a copy reaches 5.3; 6000 new rows of 24
+// query and 4 K/V heads of 256 (f32 into f16) appended in 65.5 us, 5.0 TB/s; 48 single tokens 5.2 us, an empty launch 2.4.
 #include <cmath>
 #include <memory>
 #include <new>
@@ -208,7 +208,7 @@ struct RopeArgs {
 };
 
 // One (row, head group, unit) item per thread, in that order, 64 bytes or more in flight each. Items run on from row to row:
-// with a row's items to a work-group, 80 items left most of its lanes idle (8191 rows of 40 heads of 128: 40.8 us for 34.2).
+// with a row's items to a work-group, 80 items left most of its lanes idle (8191 rows of 40 heads of 128: 40.8 us for 34.1).
 template <int T, bool INTER, int VEC, bool W>
 __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
     using E = typename RowType<T>::type;
