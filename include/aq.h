@@ -294,7 +294,8 @@ typedef struct aq_paged_batch {
 /* The new rows' k and v into their pages, rounded to the cache's type: the append of gqa_attention.rs:327-418 over
  * pages. With a rope, k is rotated by its position on the way, and q (nullable; n_head heads) into q_out (q itself, or
  * not overlapping it); without one q must be NULL. k, v and q have one type: F32, or the cache's. A row whose position
- * is negative or has no page stores nothing; its q is rotated all the same. */
+ * is negative or has no page stores nothing; its q is rotated all the same. Of rows of one call whose positions lie in
+ * the same slot (sequences that share a page there) any one may be kept: shared pages are for what is only read. */
 int aq_paged_append(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, const aq_heads *k,
                     const aq_heads *v, const aq_rope *rope, const aq_heads *q, const aq_heads *q_out, uint32_t n_head,
                     void *stream);

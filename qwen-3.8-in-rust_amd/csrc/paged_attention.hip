@@ -277,7 +277,8 @@ int check_attention(const char *call, aq_ctx *ctx, const aq_paged_kv *kv, const 
     AQ_REQUIRE(n_head > 0 && n_head <= 65535 && n_head % kv->n_head_kv == 0,
                std::string(call) + ": n_head " + std::to_string(n_head) + " is not a multiple of n_head_kv " +
                    std::to_string(kv->n_head_kv));
-    AQ_REQUIRE((uint64_t)batch->n_rows * (n_head / kv->n_head_kv) < (1ull << 31), std::string(call) + ": batch size");
+    AQ_REQUIRE((uint64_t)batch->n_rows * (n_head / kv->n_head_kv) <= (1ull << 31) - 1024,
+               std::string(call) + ": batch size (rows of a K/V head)");
     return 0;
 }
 

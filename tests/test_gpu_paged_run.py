@@ -159,7 +159,7 @@ def test_steps_of_a_batch(ctx, row_t, cache_t, window):
 
 
 @pytest.mark.parametrize("row_t,cache_t", PAIRS)
-@pytest.mark.parametrize("most,max_len", [(1, 1500), (4, 1500), (40, 1500), (40, 6000)])
+@pytest.mark.parametrize("most,max_len", [(1, 300), (4, 300), (1, 1500), (4, 1500), (40, 1500), (40, 6000)])
 def test_captured_steps(ctx, row_t, cache_t, most, max_len):
     """One graph of append and attention, replayed as the batch changes, with the workspace overwritten and eager calls
     between: each replay gives the bits of the eager call."""
@@ -168,7 +168,7 @@ def test_captured_steps(ctx, row_t, cache_t, most, max_len):
     graph = st.capture(s.call)
     other = aq.DeviceBuffer(ctx, s.ws.nbytes)
     junk = np.full(s.ws.nbytes, 0xFF, np.uint8)
-    s.lens[:] = [0, 700, 20]
+    s.lens[:] = [0, min(700, max_len // 2), 20]
     filled = P.store(s.rng.standard_normal((s.pages, s.page, s.kv, s.hd)), cache_t)
     s.k.buf.upload(filled)
     s.v.buf.upload(filled)

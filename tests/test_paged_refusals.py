@@ -199,6 +199,13 @@ def test_reach_of_a_table(ctx):
     assert aq.paged_attention_workspace(ctx, good_kv(head_stride=1 << 39), good_batch(), 4) > 0
 
 
+def test_rows_of_a_kv_head(ctx):
+    """Rows times the query heads of a K/V head stay 1024 under 2^31."""
+    kv, most = good_kv(n_head_kv=1), ((1 << 31) - 1024) // 256
+    assert aq.paged_attention_workspace(ctx, kv, good_batch(n_rows=most, max_len=16), 256) > 0
+    refused(aq.AQ_EINVAL, "batch size", aq.paged_attention_workspace, ctx, kv, good_batch(n_rows=most + 1, max_len=16), 256)
+
+
 def test_workspace_of_larger_bounds_serves_smaller_batches(ctx):
     """A workspace made for a batch's largest bounds is enough for every batch within them."""
     import random
