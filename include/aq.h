@@ -281,10 +281,10 @@ typedef struct aq_paged_kv {
 /* New rows of n_seq sequences: sequence s has rows row_start[s] .. row_start[s+1]-1 (row_start: n_seq + 1 values, never
  * falling; a sequence may have none) and kv_len[s] positions with them, so its row i stands at position
  * kv_len[s] - (its rows) + i; its position p lies in page pages[s * max_pages + p / page_size]. All three arrays on the
- * device. n_rows: rows of the row tensors (those past row_start[n_seq] are left as they are); max_rows: the most rows a
- * sequence has (an attention may leave rows past it unwritten); max_len: no kv_len is larger (an attention takes
- * positions from max_len on as holes). Bounds, not exact: a captured call keeps them as the arrays' contents change.
- * Fewer than 2^24 rows and sequences; a table reaches at most 2^31 - 1024 positions. */
+ * device. n_rows: rows of the row tensors (those before row_start[0], which need not be 0, and from row_start[n_seq] on
+ * are left as they are); max_rows: the most rows a sequence has (an attention may leave rows past it unwritten); max_len:
+ * no kv_len is larger (an attention takes positions from max_len on as holes). Bounds, not exact: a captured call keeps
+ * them as the arrays' contents change. Fewer than 2^24 rows and sequences; a table reaches at most 2^31 - 1024 positions. */
 typedef struct aq_paged_batch {
     uint32_t n_seq, max_pages;
     const int32_t *row_start, *kv_len, *pages;

@@ -1,0 +1,87 @@
+"""Which rows of the row tensors and which positions of the cache the paged calls touch: sequences that begin past the
+tensor's first row or before it, or end past its last; lengths below 0; queries of rows without a page. Append and attention
+place a row alike. Tolerances: paged_plain.bound and rotate_bound; what is not a row's stays bit for bit."""
+import numpy as np
+import pytest
+
+import aqueduct as aq
+import paged_plain as P
+from test_gpu_paged_attention import PAIRS, bounds, run
+
+pytestmark = pytest.mark.gpu
+THETA = 1e6
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return aq.Context(0)
+
+
+class Shifted:
+    """A batch whose row_start begins at `first`, over row tensors of n rows: sequence s's row i is row
+    first + (rows before it) + i of the tensors, or none of them."""
+
+    def __init__(self, ctx, rng, new, lens, first, n, kv, hd, cache_t, page=16):
+        self.pg = P.Paged(ctx, rng, new, lens, kv, hd, page, cache_t, n_rows=n)
+        self.first, self.n = first, n
+        self.pg.dstarts = P.Dev(ctx, (self.pg.starts + first).astype(np.int32))
+        self.rows = [(int(self.pg.starts[s]) + first + i, s, max(lens[s], 0) - a + i)
+                     for s, a in enumerate(new) for i in range(a)]
+        self.rows = [(r, s, p) for r, s, p in self.rows if 0 <= r < n]
+        self.mine = np.zeros(n, bool)
+        self.mine[[r for r, _, _ in self.rows]] = True
+
+    def attention(self, q, scale, window=0):
+        """The definition's outputs and its bound's parts, of the tensors' rows."""
+        lead = max(0, -self.first)
+        wide = np.concatenate([np.zeros((lead, *q.shape[1:])), q])
+        plain = P.Paged.__new__(P.Paged)
+        plain.__dict__.update(self.pg.__dict__, starts=self.pg.starts + self.first + lead)
+        want, parts = P.attention(plain, wide, scale, window)
+        return want[lead:], tuple(x[lead:] for x in parts)
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("first,cut", [(0, 0), (5, 0), (0, 1), (7, 2), (-1, 0), (-2, 1)])
+@pytest.mark.parametrize("new", [[2, 4, 4], [40, 0, 45, 40], [1] * 70])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_of_rows_around_the_tensor(ctx, row_t, cache_t, first, cut, new, in_place):
+    """Only the sequences' rows are stored, at the positions that attention gives them, and only their queries turned: the
+    rows before the first start are somebody else's, and what the cache held stays."""
+    print(f"places, append {row_t}/{cache_t} first {first} cut {cut} new {new[:4]} x {len(new)} in place {in_place}", flush=True)
+    rng = np.random.default_rng(62)
+    lens = [n + int(x) for n, x in zip(new, rng.integers(0, 300, len(new)))]
+    lens[0] = 103 + new[0]
+    n = first + sum(new) - cut
+    b = Shifted(ctx, rng, new, lens, first, n, 2, 64, cache_t)
+    check_append(ctx, rng, b, row_t, cache_t, in_place)
+
+
+def check_append(ctx, rng, b, row_t, cache_t, in_place):
+    pg, n = b.pg, b.n
+    k, v = (P.Rows(ctx, rng.standard_normal((n, 2, 64)), row_t) for _ in range(2))
+    q = P.Rows(ctx, rng.standard_normal((n, 4, 64)), row_t)
+    qo = q if in_place else P.Rows(ctx, np.full((n, 4, 64), 9.0), row_t)
+    cache, batch = pg.structs()
+    rope = aq.Rope(ctx, 48, THETA)
+    aq.paged_append(ctx, cache, batch, k.heads_struct(), v.heads_struct(), rope, q.heads_struct(), qo.heads_struct(), 4)
+    ctx.sync()
+    pos = np.zeros(n, np.int64)
+    for r, _, p in b.rows:
+        pos[r] = p
+    freq, _ = P.frequencies(48, THETA)
+    turned_k, turned_q = (P.rotate(x.values(), pos, 48, "half", freq) for x in (k, q))
+    limit = P.rotate_bound(k.values(), turned_k, cache_t)
+    got_k, got_v = pg.pools()
+    want_k, want_v = pg.k.copy(), pg.v.copy()
+    for r, s, p in b.rows:
+        at = pg.row_of(s, p)
+        if at is None:
+            continue
+        assert np.all(np.abs(got_k[at] - turned_k[r]) <= limit[r]), (r, s, p)
+        want_k[at], want_v[at] = got_k[at], P.values(P.store(v.values()[r], cache_t), cache_t)
+    assert np.array_equal(want_k, got_k, equal_nan=True), "keys that are not the rows'"
+    assert np.array_equal(want_v, got_v, equal_nan=True), "values that are not the rows'"
+    got, before = qo.get(), q.values() if in_place else np.full((n, 4, 64), 9.0)
+    assert np.array_equal(got[~b.mine], before[~b.mine]), "queries of rows that are no sequence's"
+    assert np.all((np.abs(got - turned_q) <= P.rotate_bound(q.values(), turned_q, row_t))[b.mine])
