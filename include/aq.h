@@ -230,7 +230,7 @@ int aq_sampler_accept_or_resample(aq_sampler *sp, const float *target_dev, const
  * the order of a row's sums follows the batch it is computed in.
  *
  * Offsets are 64-bit; data, strides and device arrays are checked as far as the host can see them. What only the device
- * sees is bounded there: rows at or past n_rows are never touched, a page outside 0..n_pages-1 or a position past the
+ * sees is bounded there: rows outside 0..n_rows-1 are never touched, a page outside 0..n_pages-1 or a position past the
  * table is a hole (nothing is stored there, nothing attended), a length below 0 counts as 0. */
 
 /* [rows][heads][head_dim] values on the device, type F32, F16 or BF16; strides in elements, head_dim contiguous. */

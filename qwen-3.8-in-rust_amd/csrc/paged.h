@@ -96,9 +96,10 @@ __device__ __forceinline__ uint32_t paged_seq_of(const PagedBatch &b, uint32_t r
     return lo;
 }
 
-// A sequence's rows within the batch's n_rows, whatever row_start holds, and its length.
+// A sequence's rows within the tensors' n_rows, whatever row_start holds, and the position of the first of them: a sequence
+// that begins before the tensors or ends past them keeps its other rows' positions.
 struct SeqRows {
-    int32_t first, n, len;
+    int32_t first, n, base;
 };
 __device__ __forceinline__ SeqRows paged_seq(const PagedBatch &b, uint32_t s) {
     const int32_t lo = b.row_start[s], hi = b.row_start[s + 1], len = b.kv_len[s];
@@ -106,7 +107,7 @@ __device__ __forceinline__ SeqRows paged_seq(const PagedBatch &b, uint32_t s) {
     r.first = lo < 0 ? 0 : lo;
     const int32_t end = hi < (int32_t)b.n_rows ? hi : (int32_t)b.n_rows;
     r.n = end > r.first ? end - r.first : 0;
-    r.len = len > 0 ? len : 0;
+    r.base = (len > 0 ? len : 0) - (hi > r.first ? hi - r.first : 0);
     return r;
 }
 

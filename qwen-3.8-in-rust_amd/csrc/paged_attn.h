@@ -53,7 +53,7 @@ struct UnitRange {
 };
 __device__ __forceinline__ UnitRange tile_units(const AttnPagedArgs &a, const SeqRows &sr, int32_t r0, int32_t R, uint32_t tk) {
     const int32_t last = min(r0 + R, sr.n * a.G) - 1;
-    const int32_t t0 = (int32_t)a.by_g.quot(r0), t1 = (int32_t)a.by_g.quot(last), base = sr.len - sr.n; // row tokens' positions are base + token
+    const int32_t t0 = (int32_t)a.by_g.quot(r0), t1 = (int32_t)a.by_g.quot(last), base = sr.base; // row tokens' positions are base + token
     const int32_t end = min(max(base + t1 + 1, 0), (int32_t)a.cap);
     const int64_t begin = a.window ? max((int64_t)base + t0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
     UnitRange u;

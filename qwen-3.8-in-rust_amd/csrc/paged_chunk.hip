@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
         if (sg.t1 <= sg.t0) continue;
         const int n = here(n0), h = here(h0);
         const SeqRows sr = paged_seq(a.b, sg.seq);
-        const int32_t n_rows = sr.n * G, base = sr.len - sr.n;
+        const int32_t n_rows = sr.n * G, base = sr.base;
         const UnitRange range = tile_units(a, sr, sg.r0, R, KEYS);
         const int32_t *table = a.b.pages + (size_t)sg.seq * a.b.max_pages;
         const uint64_t head_off = (uint64_t)sg.kvh * a.kv.head_bytes;

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
         const uint32_t kvh = sg.kvh;
         const int32_t r0 = sg.r0;
         const SeqRows sr = paged_seq(a.b, sg.seq);
-        const int32_t n_rows = sr.n * G, base = sr.len - sr.n;
+        const int32_t n_rows = sr.n * G, base = sr.base;
         const UnitRange range = tile_units(a, sr, r0, R, UNIT);
         const int32_t tok0 = (int32_t)a.by_g.quot(r0), tok1 = (int32_t)a.by_g.quot(min(r0 + R, n_rows) - 1);
         const int32_t kend = min(max(base + tok1 + 1, 0), (int32_t)a.cap);

@@ -42,6 +42,29 @@ class Shifted:
 
 
 @pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("first,cut", [(5, 0), (0, 1), (7, 2), (-1, 0), (-2, 1)])
+@pytest.mark.parametrize("new", [[2, 4, 4], [40, 0, 45, 40], [1] * 70])
+@pytest.mark.parametrize("window", [0, 30])
+def test_attention_of_rows_around_the_tensor(ctx, row_t, cache_t, first, cut, new, window):
+    """Rows before the first sequence and rows that the tensors do not have; a sequence that is cut keeps its other rows'
+    positions."""
+    print(f"places {row_t}/{cache_t} first {first} cut {cut} new {new[:4]} x {len(new)} window {window}", flush=True)
+    rng = np.random.default_rng(61)
+    lens = [n + int(x) for n, x in zip(new, rng.integers(0, 300, len(new)))]
+    n = first + sum(new) - cut
+    b = Shifted(ctx, rng, new, lens, first, n, 2, 64, cache_t)
+    q = P.Rows(ctx, rng.standard_normal((n, 4, 64)), row_t)
+    want, parts = b.attention(q.values(), 0.125, window)
+    limit = P.bound(parts, want, row_t, cache_t, 64)
+    for loose in bounds(b.pg, q):
+        out = P.Rows(ctx, np.full((n, 4, 64), 9.0), row_t)
+        run(ctx, b.pg, q, out, 0.125, window, loose=loose)
+        got = out.get()
+        assert np.all(got[~b.mine] == 9.0)
+        assert np.all(np.abs(got - want)[b.mine] <= limit[b.mine])
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
 @pytest.mark.parametrize("first,cut", [(0, 0), (5, 0), (0, 1), (7, 2), (-1, 0), (-2, 1)])
 @pytest.mark.parametrize("new", [[2, 4, 4], [40, 0, 45, 40], [1] * 70])
 @pytest.mark.parametrize("in_place", [False, True])
