@@ -243,8 +243,9 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
     const uint32_t row = blockIdx.x, item = blockIdx.y * blockDim.x + threadIdx.x;
     const uint32_t seq = paged_seq_of(a.b, row);
     if (seq >= a.b.n_seq || row >= a.b.n_rows || item >= a.items) return;
-    if ((int32_t)row < a.b.row_start[seq]) return; // before the first sequence's rows
-    const int32_t pos = a.b.kv_len[seq] - (a.b.row_start[seq + 1] - (int32_t)row);
+    const SeqRows sr = paged_seq(a.b, seq);
+    if ((int32_t)row < sr.first) return; // before the first sequence's rows
+    const int32_t pos = sr.base + ((int32_t)row - sr.first);
     const bool isv = item >= a.qk_items;
     const uint32_t it = isv ? item - a.qk_items : item;
     const uint32_t grp = isv ? a.vunit_div.quot(it) : a.unit_div.quot(it);

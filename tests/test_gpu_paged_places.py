@@ -80,6 +80,16 @@ def test_append_of_rows_around_the_tensor(ctx, row_t, cache_t, first, cut, new, 
     check_append(ctx, rng, b, row_t, cache_t, in_place)
 
 
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("below", [-1, -5, -2 ** 31 + 1])
+def test_append_at_lengths_below_zero(ctx, row_t, cache_t, below):
+    """A length below 0 counts as 0: the rows stand before position 0, store nothing, and are turned by where they stand."""
+    print(f"places, length {below} {row_t}/{cache_t}", flush=True)
+    rng = np.random.default_rng(63)
+    b = Shifted(ctx, rng, [3, 2, 1], [below, 40, 0], 0, 6, 2, 64, cache_t)
+    check_append(ctx, rng, b, row_t, cache_t, False)
+
+
 def check_append(ctx, rng, b, row_t, cache_t, in_place):
     pg, n = b.pg, b.n
     k, v = (P.Rows(ctx, rng.standard_normal((n, 2, 64)), row_t) for _ in range(2))
