@@ -118,3 +118,28 @@ def check_append(ctx, rng, b, row_t, cache_t, in_place):
     got, before = qo.get(), q.values() if in_place else np.full((n, 4, 64), 9.0)
     assert np.array_equal(got[~b.mine], before[~b.mine]), "queries of rows that are no sequence's"
     assert np.all((np.abs(got - turned_q) <= P.rotate_bound(q.values(), turned_q, row_t))[b.mine])
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_queries_of_rows_without_a_page_are_turned(ctx, row_t, cache_t, layout, in_place):
+    """At negative positions, in holes and past the table a row stores nothing; its q is rotated all the same."""
+    rng = np.random.default_rng(64)
+    pg = P.Paged(ctx, rng, [4, 3, 2], [2, 60, 40], 2, 64, 16, cache_t, cols=3)
+    pg.table[2, 2] = pg.k.shape[0]  # positions 32 .. 47; those of sequence 1 lie past the table
+    pg.upload()
+    k = P.Rows(ctx, rng.standard_normal((9, 2, 64)), row_t)
+    q = P.Rows(ctx, rng.standard_normal((9, 4, 64)), row_t)
+    qo = q if in_place else P.Rows(ctx, np.full((9, 4, 64), 9.0), row_t)
+    cache, batch = pg.structs()
+    aq.paged_append(ctx, cache, batch, k.heads_struct(), k.heads_struct(), aq.Rope(ctx, 64, THETA, layout=layout),
+                    q.heads_struct(), qo.heads_struct(), 4)
+    ctx.sync()
+    pos = np.array([-2, -1, 0, 1, 57, 58, 59, 38, 39])
+    want = P.rotate(q.values(), pos, 64, layout, P.frequencies(64, THETA)[0])
+    assert np.all(np.abs(qo.get() - want) <= P.rotate_bound(q.values(), want, row_t))
+    want_v = pg.v.copy()
+    for r in (2, 3):
+        want_v[pg.row_of(0, int(pos[r]))] = P.values(P.store(k.values()[r], cache_t), cache_t)
+    assert np.array_equal(want_v, pg.pools()[1], equal_nan=True)
