@@ -201,13 +201,9 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
             const uint32_t ln = (uint32_t)here(lane) & 63, first = wave * S::LOADS * RPI, row0 = first + ln / S::CPR;
             const uint32_t c0 = (ln % S::CPR) ^ S::swizzle(row0);
             char *kd = kbuf + buf * S::TILE_BYTES + wave * S::LOADS * 1024, *vd = vbuf + (kd - kbuf);
-            // the lane's 16 bytes of row row0 + i RPI (whose low bits row0 has none of); past the head: the queries are 0
-            // there, the outputs not stored
-            auto chunk = [&](uint32_t i) {
-                const uint32_t c = c0 ^ S::swizzle(i * RPI);
-                return (hd == D ? c : min(c, (uint32_t)hd / 8 - 1)) * 16;
-            };
-            if (ok == ALL && runs) { // a load's rows are one run of a page: one address for the wave
+            // the lane's 16 bytes of row row0 + i RPI (whose low bits row0 has none of)
+            auto chunk = [&](uint32_t i) { return (c0 ^ S::swizzle(i * RPI)) * 16; };
+            if (ok == ALL && runs && hd == D) { // a load's rows are one run of a page: one address for the wave
                 const uint32_t lead = (ln / S::CPR) * (a.kv.slot_units << a.kv.unit_shift);
 #pragma unroll
                 for (uint32_t i = 0; i < S::LOADS; i++) {
@@ -216,12 +212,13 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                     __builtin_amdgcn_global_load_lds((const AQ_GLB void *)(kpool + off + at), (AQ_LDS void *)(kd + i * 1024), 16, 0, 0);
                     __builtin_amdgcn_global_load_lds((const AQ_GLB void *)(vpool + off + at), (AQ_LDS void *)(vd + i * 1024), 16, 0, 0);
                 }
-            } else {
+            } else { // rows without a page are zeros, and dimensions past the head like the queries' there: 0 times an infinity
+                     // would be a NaN
 #pragma unroll
                 for (uint32_t i = 0; i < S::LOADS; i++) {
                     const uint32_t un = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(row0 * 4 + i * RPI * 4), (int)units);
                     const uint64_t off = ((uint64_t)un << a.kv.unit_shift) + chunk(i);
-                    const bool has = (ok >> (row0 + i * RPI)) & 1;
+                    const bool has = ((ok >> (row0 + i * RPI)) & 1) && chunk(i) < (uint32_t)hd * 2;
                     const char *kp = has ? kpool + off : (const char *)&zeros, *vp = has ? vpool + off : (const char *)&zeros;
                     __builtin_amdgcn_global_load_lds((const AQ_GLB void *)kp, (AQ_LDS void *)(kd + i * 1024), 16, 0, 0);
                     __builtin_amdgcn_global_load_lds((const AQ_GLB void *)vp, (AQ_LDS void *)(vd + i * 1024), 16, 0, 0);

@@ -37,6 +37,8 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 
+__device__ const u4 zeros = {0, 0, 0, 0};
+
 template <int CT>
 __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
     if constexpr (CT == AQ_TYPE_F16)
@@ -155,14 +157,13 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
         auto row_off = [&](uint32_t units, int pos) {
             return (uint64_t)(uint32_t)__shfl((int)units, pos) << a.kv.unit_shift;
         };
-        // 16 rows of K as operands; dimensions past the head repeat its last ones: q is 0 there
+        // 16 rows of K as operands; dimensions past the head are zeros like q's there (0 times an infinity would be a NaN),
+        // chosen by the address, so that nothing waits for the load
         auto load_k = [&](uint32_t units, int t, u4 *k) {
-            const char *p = kpool + (row_off(units, 16 * t + r) + (EXACT ? 16 * g : 0));
+            const char *p = kpool + (row_off(units, 16 * t + r) + 16 * g);
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                const int at = EXACT ? 64 * s : min(64 * s + 16 * g, hd * ES - 16);
-                k[s] = *reinterpret_cast<const u4 *>(p + at);
-            }
+            for (int s = 0; s < STEPS; s++)
+                k[s] = *reinterpret_cast<const u4 *>(EXACT || 64 * s + 16 * g < hd * ES ? p + 64 * s : (const char *)&zeros);
         };
         using VV = typename std::conditional<VB * ES == 8, u2, u4>::type;
         using VP = typename std::conditional<HT == 1, u2, u4>::type; // probabilities, V^T: E 16-bit values

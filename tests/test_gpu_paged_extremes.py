@@ -1,0 +1,43 @@
+"""Attention over pages at the ends of the types' ranges: infinite keys at every head size.
+Tolerances: paged_plain.bound."""
+import numpy as np
+import pytest
+
+import aqueduct as aq
+import paged_plain as P
+from test_gpu_paged_attention import PAIRS, bounds, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return aq.Context(0)
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("hd", [8, 24, 64, 72, 80, 96, 128, 160, 192, 200, 256])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+def test_infinite_keys_at_the_end_of_a_head(ctx, row_t, cache_t, hd, new, value):
+    """An infinity in a key's last value: a row whose score is plus infinity is NaN, one whose score is minus infinity is as
+    if the position were not there, whatever the head's size."""
+    print(f"infinite keys {row_t}/{cache_t} head {hd} new {new} {value}", flush=True)
+    rng = np.random.default_rng(71)
+    pg = P.Paged(ctx, rng, [new], [150], 2, hd, 1, cache_t)
+    pg.k[pg.row_of(0, 70)][:, hd - 1] = value
+    pg.upload()
+    q = P.Rows(ctx, rng.standard_normal((new, 4, hd)), row_t)
+    up = q.values()[..., hd - 1] * np.sign(value) > 0
+    scale = float(np.float32(hd ** -0.5))
+    without = P.Paged.__new__(P.Paged)
+    without.__dict__.update(pg.__dict__, table=pg.table.copy())
+    without.table[0, 70] = -1  # its page is its own
+    want, parts = P.attention(without, q.values(), scale)
+    limit = P.bound(parts, want, row_t, cache_t, hd)
+    for loose in bounds(pg, q):
+        out = P.Rows(ctx, np.full((new, 4, hd), 9.0), row_t)
+        run(ctx, pg, q, out, scale, loose=loose)
+        got = out.get()
+        assert np.array_equal(np.isnan(got).all(-1), up) and np.array_equal(np.isnan(got).any(-1), up)
+        assert np.all((np.abs(got - want) <= limit)[~up])
