@@ -214,55 +214,74 @@ int compute_units(int device) {
 struct Choice {
     bool many = false; // paged_chunk.hip
     int R = 16, D = 64;
-    uint32_t unit = 0, shares = 0, min_chunk = 1, lead = 0, whole = 0, n_seg = 0, cap = 0;
+    uint32_t unit = 0, per = 0, shares = 0, min_chunk = 1, lead = 0, whole = 0, n_seg = 0, cap = 0;
     bool planned = false, join = false;
     PagedSpace space;
 };
 
-int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uint32_t n_head, bool f32_rows, int device,
-           Choice *c) {
+// Rows of a K/V head of the longest sequence, and the positions a batch can reach.
+uint64_t longest_rows(const aq_paged_kv *kv, const aq_paged_batch *b, uint32_t n_head) {
+    return (uint64_t)b->max_rows * (n_head / kv->n_head_kv);
+}
+uint32_t reach_of(const aq_paged_kv *kv, const aq_paged_batch *b) {
+    return (uint32_t)std::min<uint64_t>((uint64_t)b->max_pages * kv->page_size, b->max_len);
+}
+// Paged chunks for 16-bit rows past one row tile of the few-row kernel, once there is enough to do: its start (code,
+// 128-row blocks) takes 12 to 30 us whatever the work, each further row tile of the other reads K and V again. Few-row
+// and chunk kernel, by rows x heads x positions (bf16, us): heads of 256: 0.04M 13.6 and 29.2, 3.1M 37.7 and 43.3, 4.6M
+// 40.7 and 43.9, 7.4M 54.6 and 48.7; of 128: 0.05M 9.8 and 18.2, 4.1M 27.4 and 30.0, 4.4M 30.9 and 30.0, 7.7M 41.9 and
+// 38.5, 46M 211 and 136; of 64: 5.0M 22.2 and 24.2, 10M 30.0 and 26.1, 31M 81 and 59.
+bool takes_chunks(const aq_paged_kv *kv, const aq_paged_batch *b, uint32_t n_head) {
+    return longest_rows(kv, b, n_head) > 32 && (double)b->n_rows * n_head * reach_of(kv, b) > 5.0 * (1 << 20);
+}
+
+// The work on row tiles of R rows, and the workspace it takes: that grows with each of the batch's bounds.
+Choice on_tiles(const aq_paged_kv *kv, const aq_paged_batch *b, uint32_t n_head, bool many, int R, int device) {
+    Choice c;
     const uint32_t G = n_head / kv->n_head_kv;
-    const uint64_t rows = (uint64_t)b->max_rows * G;
-    c->D = kv->head_dim <= 64 ? 64 : kv->head_dim <= 128 ? 128 : 256;
-    c->cap = (uint32_t)std::min<uint64_t>((uint64_t)b->max_pages * kv->page_size, b->max_len);
-    // Paged chunks for 16-bit rows past one row tile of the few-row kernel, once there is enough to do: its start (code,
-    // 128-row blocks) takes 12 to 30 us whatever the work, each further row tile of the other reads K and V again. Few-row
-    // and chunk kernel, by rows x heads x positions (bf16, us): heads of 256: 0.04M 13.6 and 29.2, 3.1M 37.7 and 43.3, 4.6M
-    // 40.7 and 43.9, 7.4M 54.6 and 48.7; of 128: 0.05M 9.8 and 18.2, 4.1M 27.4 and 30.0, 4.4M 30.9 and 30.0, 7.7M 41.9 and
-    // 38.5, 46M 211 and 136; of 64: 5.0M 22.2 and 24.2, 10M 30.0 and 26.1, 31M 81 and 59.
-    c->many = !f32_rows && rows > 32 && (double)b->n_rows * n_head * c->cap > 5.0 * (1 << 20);
-    c->R = c->many ? CHUNK_ROWS : rows <= 16 ? 16 : 32;
-    c->unit = c->many ? chunk_keys(c->D) : few_unit(kv->type, c->D, c->R);
-    c->min_chunk = c->many ? 256 / c->unit : 1;
+    c.many = many;
+    c.R = R;
+    c.D = kv->head_dim <= 64 ? 64 : kv->head_dim <= 128 ? 128 : 256;
+    c.cap = reach_of(kv, b);
+    c.unit = c.many ? chunk_keys(c.D) : few_unit(kv->type, c.D, c.R);
+    c.min_chunk = c.many ? 256 / c.unit : 1;
     // What a segment costs besides its positions (queries, first loads, the waves' meeting, its output), in units. Prompts
     // of three requests (10,500 rows of 32 heads of 128), of 64 positions: 0: 794 us, 2: 532, 4: 459, 6: 459, 8: 467. Eight
     // verify batches of 32 rows (f32 over f16, heads of 256), of 32: 0: 46.4, 2: 42.5, 4: 42.6. Single tokens: none to gain;
     // nor where a unit takes as long as that (f32 products).
-    c->lead = c->many ? 320 / c->unit : c->R == 32 && kv->type != AQ_TYPE_F32 ? 2 : 0;
+    c.lead = c.many ? 320 / c.unit : c.R == 32 && kv->type != AQ_TYPE_F32 ? 2 : 0;
     // row tiles: a whole one per R rows of all sequences together, and one begun per sequence
-    const uint64_t n_seg = std::min<uint64_t>((uint64_t)b->n_rows * G / c->R + b->n_seq, (uint64_t)b->n_rows * G);
-    c->planned = n_seg > INLINE_TILES || b->n_seq > INLINE_TILES;
+    const uint64_t n_seg = std::min<uint64_t>((uint64_t)b->n_rows * G / c.R + b->n_seq, (uint64_t)b->n_rows * G);
+    c.planned = n_seg > INLINE_TILES || b->n_seq > INLINE_TILES;
     // places of a segment at most (a window may begin inside a unit)
-    const uint64_t per = (c->cap + c->unit - 1) / c->unit + 1 + c->lead;
-    if ((double)n_seg * (double)per * kv->n_head_kv >= 2147483648.0 || n_seg * kv->n_head_kv >= (1u << 31))
-        return fail(AQ_EUNSUP, std::string(call) + ": batch of more than 2^31 units of work");
-    c->n_seg = (uint32_t)n_seg;
+    c.per = (c.cap + c.unit - 1) / c.unit + 1 + c.lead;
+    c.n_seg = (uint32_t)n_seg;
     // Two work-groups per CU; one of up to 16 rows over 16-bit pages, bound by the memory alone (48 sequences at 6000, 32
     // heads on 8 of 128: one 215 us, two 228, three 223; one sequence at 8000, 24 heads on 4 of 256: 17.7 and 19.0; but f32
     // pages, 64 rows at 4001: 131 and 101). No more than there can be units.
-    const uint64_t per_cu = !c->many && c->R == 16 && kv->type != AQ_TYPE_F32 ? 1 : 2;
-    const uint64_t units = n_seg * kv->n_head_kv * per, shares = std::min<uint64_t>((uint64_t)compute_units(device) * per_cu, units);
-    c->shares = (uint32_t)(shares > 8 ? (shares + 7) / 8 * 8 : std::max<uint64_t>(shares, 1));
-    c->space = paged_space(c->shares, c->n_seg, (size_t)c->R, (size_t)c->D);
+    const uint32_t per_cu = !c.many && c.R == 16 && kv->type != AQ_TYPE_F32 ? 1 : 2, most = (uint32_t)compute_units(device) * per_cu;
+    const double units = (double)n_seg * kv->n_head_kv * c.per;
+    const uint32_t shares = units < most ? (uint32_t)units : most;
+    c.shares = shares > 8 ? (shares + 7) / 8 * 8 : std::max(shares, 1u);
+    c.space = paged_space(c.shares, c.n_seg, (size_t)c.R, (size_t)c.D);
+    return c;
+}
+
+int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uint32_t n_head, bool f32_rows, int device,
+           Choice *c) {
+    const bool many = !f32_rows && takes_chunks(kv, b, n_head);
+    *c = on_tiles(kv, b, n_head, many, many ? CHUNK_ROWS : longest_rows(kv, b, n_head) <= 16 ? 16 : 32, device);
+    const uint64_t segs = (uint64_t)c->n_seg * kv->n_head_kv, cus = (uint64_t)compute_units(device);
+    if ((double)segs * c->per >= 2147483648.0)
+        return fail(AQ_EUNSUP, std::string(call) + ": batch of more than 2^31 units of work");
     // Short contexts: a share to each segment, and no join, whose launch costs as much as three or four units. Line and whole
     // segments (us): one sequence of 32 heads on 8 of 128 (bf16) at 150: 11.2 and 8.4, at 300: 11.2 and 10.1, at 500: 11.3
     // and 11.5; 64 of them at 150: 27.5 and 16.6, at 300: 37.2 and 26.2, at 500: 44.6 and 43.9, at 800: 59.0 and 65.0; 24
     // heads on 4 of 256 (f16), one at 150: 12.1 and 11.0, at 300: 13.2 and 13.5. Not where two waves share a unit (32 rows
     // of 256 at 150: 14.3 and 18.2), nor with more segments than measured (1536).
-    const uint64_t segs = n_seg * kv->n_head_kv, cus = (uint64_t)compute_units(device);
     if (!c->many && !c->planned && few_groups(kv->type, c->D, c->R) == 1 && segs <= 8 * cus &&
         c->cap <= (c->D == 256 ? 256u : segs >= cus ? 512u : 384u)) {
-        c->whole = (uint32_t)per;
+        c->whole = c->per;
         c->shares = (uint32_t)(segs > 8 ? (segs + 7) / 8 * 8 : segs);
     }
     c->join = !c->whole && c->cap > c->unit; // else no segment has a second unit
@@ -311,13 +330,17 @@ int aq_paged_attention_workspace(aq_ctx *ctx, const aq_paged_kv *kv, const aq_pa
     AQ_REQUIRE(bytes, "aq_paged_attention_workspace: null bytes");
     int rc = check_attention("aq_paged_attention_workspace", ctx, kv, batch, n_head, nullptr, nullptr);
     if (rc) return rc;
-    size_t most = 0;
-    for (int f32_rows = 0; f32_rows < 2; f32_rows++) { // enough for either type of rows
-        Choice c;
-        rc = choose("aq_paged_attention_workspace", kv, batch, n_head, f32_rows != 0, ctx->device, &c);
-        if (rc) return rc;
-        most = std::max(most, c.space.bytes);
-    }
+    // Enough for either type of rows, and for every batch within these bounds: one with shorter sequences may take smaller
+    // row tiles, of which there are more.
+    Choice c;
+    rc = choose("aq_paged_attention_workspace", kv, batch, n_head, true, ctx->device, &c);
+    if (rc && kv->type != AQ_TYPE_F32) rc = choose("aq_paged_attention_workspace", kv, batch, n_head, false, ctx->device, &c);
+    if (rc) return rc;
+    size_t most = on_tiles(kv, batch, n_head, false, 16, ctx->device).space.bytes;
+    if (longest_rows(kv, batch, n_head) > 16)
+        most = std::max(most, on_tiles(kv, batch, n_head, false, 32, ctx->device).space.bytes);
+    if (kv->type != AQ_TYPE_F32 && takes_chunks(kv, batch, n_head))
+        most = std::max(most, on_tiles(kv, batch, n_head, true, CHUNK_ROWS, ctx->device).space.bytes);
     *bytes = most;
     return 0;
 }
