@@ -8,8 +8,8 @@
 //                 sum are in two lanes: one exchange (v_permlane32_swap) per tile.
 //   O^T = V^T P^T the exponentials, rounded, are B's layout as they stand if k-slot (h, e) stands for position 8 (e / 4) +
 //                 4 h + e % 4; A = V^T comes from the row-major V tile by transposing LDS reads (ds_read_b64_tr_b16).
-// The maximum a row's exponentials are taken against moves only when it grows by more than 2^7 (the sums hold that), so
-// that outputs are rarely rescaled.
+// The maximum a row's exponentials are taken against moves only when it grows by more than 2^7 (their scale leaves room
+// for that), so that outputs are rarely rescaled.
 //
 // Tiles are loaded straight into the LDS (16 bytes a lane, consecutive lanes consecutive addresses), each lane choosing
 // which 16 bytes of its row it fetches: the row's chunks are swapped by an exclusive or with the row's low bits, so that
@@ -142,7 +142,9 @@ template <int CT, int D>
 __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
     using S = ChunkShape<D>;
     constexpr int R = CHUNK_ROWS, KEYS = S::KEYS, HALVES = S::HALVES, STEPS = D / 16, DB = D / 32;
-    constexpr float P_SHIFT = CT == AQ_TYPE_F16 ? 7.0f : 0.0f, GROW = 7.0f;
+    // Exponentials lie up to 2^GROW over those of the maximum they are taken against. f16: between 2^7 and 2^14, so that small
+    // ones stay normal numbers; bf16, whose values may be as large as sums are: never above 1.
+    constexpr float GROW = 7.0f, P_SHIFT = CT == AQ_TYPE_F16 ? 7.0f : -GROW;
     extern __shared__ __align__(16) char smem[];
     __shared__ PlanLds plan;
     char *kbuf = smem, *vbuf = smem + 2 * S::TILE_BYTES;

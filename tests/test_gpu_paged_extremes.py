@@ -1,4 +1,4 @@
-"""Attention over pages at the ends of the types' ranges: infinite keys at every head size.
+"""Attention over pages at the ends of the types' ranges: infinite keys at every head size, values near the largest number.
 Tolerances: paged_plain.bound."""
 import numpy as np
 import pytest
@@ -41,3 +41,30 @@ def test_infinite_keys_at_the_end_of_a_head(ctx, row_t, cache_t, hd, new, value)
         got = out.get()
         assert np.array_equal(np.isnan(got).all(-1), up) and np.array_equal(np.isnan(got).any(-1), up)
         assert np.all((np.abs(got - want) <= limit)[~up])
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("hd", [64, 128, 200, 256])
+@pytest.mark.parametrize("new", [1, 40])
+def test_values_near_the_largest_number(ctx, row_t, cache_t, hd, new):
+    """Scores that rise by e^4 after the first tiles, over values whose sum is still finite: no weight is above 1 on the way.
+    At positions from 128 on (22 of them) the value is `big`: their sum, 22 big, is below the type's largest number."""
+    print(f"large values {row_t}/{cache_t} head {hd} new {new}", flush=True)
+    rng = np.random.default_rng(72)
+    pg = P.Paged(ctx, rng, [new], [150], 2, hd, 16, cache_t)
+    big = 2000.0 if cache_t == "f16" else 1e37
+    for p in range(150):
+        at = pg.row_of(0, p)
+        pg.k[at] = 4.0 if p >= 128 else 0.0
+        if p >= 128:
+            pg.v[at] = big * rng.choice([-1.0, 1.0], (2, hd))
+    pg.upload()
+    q = P.Rows(ctx, np.ones((new, 4, hd)), row_t)
+    scale = 1.0 / hd if hd != 200 else float(np.float32(1.0 / hd))
+    want, parts = P.attention(pg, q.values(), scale)
+    limit = P.bound(parts, want, row_t, cache_t, hd)
+    for loose in bounds(pg, q):
+        out = P.Rows(ctx, np.full((new, 4, hd), 9.0), row_t)
+        run(ctx, pg, q, out, scale, loose=loose)
+        got = out.get()
+        assert np.all(np.isfinite(got)) and np.all(np.abs(got - want) <= limit)
