@@ -360,6 +360,11 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
     AQ_REQUIRE(q->type == AQ_TYPE_F32 || q->type == kv->type, "aq_paged_attention: rows are F32 or of the cache's type");
     AQ_REQUIRE(out->type == q->type && (!gate || gate->type == q->type),
                "aq_paged_attention: q, gate and out of different types");
+    auto apart = [&](const aq_heads *x) { // each output where its own input is, or in memory of its own
+        return out->data != x->data || ((rows <= 1 || out->row_stride == x->row_stride) &&
+                                        (n_head <= 1 || out->head_stride == x->head_stride));
+    };
+    AQ_REQUIRE(apart(q) && (!gate || apart(gate)), "aq_paged_attention: in place needs the same strides");
     AQ_REQUIRE(std::isfinite(scale) && scale > 0.0f, "aq_paged_attention: scale");
     if (rows == 0 || batch->n_seq == 0 || batch->max_rows == 0) return 0;
     Choice c;

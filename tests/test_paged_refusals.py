@@ -226,3 +226,20 @@ def test_workspace_of_larger_bounds_serves_smaller_batches(ctx):
         big = [n_seq, log(1, max(30000 // n_seq, 1)), log(1, 60000)]
         small = [log(1, b) for b in big]
         assert need(*small, kv, heads) <= need(*big, kv, heads), (small, big, kv.type, kv.head_dim, n_kv, heads)
+
+
+def test_attention_in_place(ctx):
+    """The output over the queries or the gate has their strides, where those matter."""
+    def go(text, q, out, gate=None, heads=4, **kw):
+        refused(aq.AQ_EINVAL, text, aq.paged_attention, ctx, good_kv(), good_batch(**kw), heads, q, out, 0.1, 0, gate, FAKE, 0)
+
+    def at(place, **kw):
+        return rows(heads=4, data=place, **kw)
+
+    go("same strides", at(FAKE), at(FAKE, row=512))
+    go("same strides", at(FAKE, head=128, row=512), at(FAKE, row=512))
+    go("same strides", at(2 * FAKE), at(FAKE), at(FAKE, row=512))
+    go("needed", at(FAKE), at(FAKE))  # no workspace: everything before that is as it should be
+    go("needed", at(2 * FAKE), at(FAKE), at(FAKE))
+    go("needed", at(FAKE), at(FAKE, row=512), n_rows=1)
+    go("needed", at(FAKE), at(2 * FAKE, row=512))
