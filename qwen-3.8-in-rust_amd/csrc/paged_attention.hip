@@ -1,7 +1,6 @@
 // paged_attention.hip — attention over a paged K/V cache (aq_paged_attention): the choice of kernel (paged_few.h for
 // few rows and for f32 rows, paged_chunk.hip for many 16-bit rows), the plan and the join of split sequences.
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <mutex>
 

@@ -21,7 +21,6 @@
 // f16 or three bf16 pieces whose sum has 22 or 24 bits. f32 over f32 takes the f32 matrix cores (16x16x4).
 #pragma once
 
-#include <atomic>
 #include <type_traits>
 
 #include "paged_attn.h"
@@ -631,15 +630,7 @@ template <int CT, bool FQ, int D, int R, bool EXACT>
 int few_launch(const AttnPagedArgs &a, hipStream_t stream) {
     using S = FewShape<CT, FQ, D, R>;
     const auto kernel = few_rows_kernel<CT, FQ, D, R, EXACT>;
-    if constexpr (S::LDS > 56 * 1024) { // with the static arrays past the 64 KiB that need no asking
-        static std::atomic<uint64_t> raised{0}; // bit d: done on device d
-        int dev = 0;
-        AQ_HIP(hipGetDevice(&dev));
-        if (!(raised.load() & (1ull << (dev & 63)))) {
-            AQ_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
-            raised.fetch_or(1ull << (dev & 63));
-        }
-    }
+    static_assert(S::LDS + sizeof(PlanLds) + R * 4 <= 64 * 1024, "more LDS than a launch has without asking for it");
     kernel<<<a.shares, 256, S::LDS, stream>>>(a);
     AQ_HIP(hipGetLastError());
     return 0;
