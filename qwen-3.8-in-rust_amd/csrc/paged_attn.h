@@ -369,6 +369,18 @@ __device__ __forceinline__ unsigned odd_mask(unsigned w) {
     return ((odd_bits<CT>(w) & 0x80008000u) >> 15) * 0xFFFFu;
 }
 
+// l plus the two values of a packed word, in 32 bits.
+template <int CT>
+__device__ __forceinline__ float add2(unsigned w, float l) {
+    if constexpr (CT == AQ_TYPE_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{1, 1}, l, false);
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.0f, (__bf16)1.0f}, l, false);
+    }
+}
+
 // Workspace layout, the same in the size query and in the launch.
 struct PagedSpace {
     size_t plan = 0, seg = 0, o = 0, ml = 0, bytes = 0;

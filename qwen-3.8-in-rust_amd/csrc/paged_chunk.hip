@@ -53,18 +53,6 @@ __device__ __forceinline__ unsigned pack2(float x, float y) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, e2));
 }
 
-// l plus the two values of a packed word, in 32 bits.
-template <int CT>
-__device__ __forceinline__ float add2(unsigned w, float l) {
-    if constexpr (CT == AQ_TYPE_F16) {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{1, 1}, l, false);
-    } else {
-        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.0f, (__bf16)1.0f}, l, false);
-    }
-}
-
 // The larger of x's two halves (lanes l and l + 32).
 __device__ __forceinline__ float both_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

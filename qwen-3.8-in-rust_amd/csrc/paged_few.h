@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 x[e] = fast_exp2((x[e] - mu) + P_SHIFT);
-                l[nr] += x[e];
+                if (F || NP > 1) l[nr] += x[e];
             }
         };
 
@@ -364,6 +364,10 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                     for (int e = 0; e < E; e++) x[e] = s[nr][e / 4][e % 4];
                     soften(nr, x, kb, ok, edge);
                     pieces<CT, NP>(x, pf[nr]);
+                    if constexpr (NP == 1) { // the sum is of what the product takes, so that roundings weigh on both alike
+#pragma unroll
+                        for (int h = 0; h < E / 2; h++) l[nr] = add2<CT>(pf[nr][0][h], l[nr]);
+                    }
                 }
                 if (edge) { // rows of positions that no page holds are not numbers that may be multiplied by 0
                     const uint32_t mine = ok >> here(4 * g);
