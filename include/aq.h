@@ -303,9 +303,12 @@ int aq_paged_append(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *ba
 /* out[r][h] = sum_j softmax_j(scale * q[r][h] . K[j][h / (n_head / n_head_kv)]) V[j][...] over the positions j up to
  * the row's own (with window > 0: the last `window` of them), times sigmoid(gate[r][h]) when gate is given (nullable):
  * the attention core of gqa_attention.rs:327-418 over pages. A row that sees nothing is 0. What a row does not see
- * never reaches it, infinities and NaN included. q, gate and out have one type: F32, or the cache's; F32 rows over a
- * 16-bit cache keep 32-bit accuracy (queries and probabilities go through the matrix cores in pieces). out may be q or
- * gate (same strides), and else must not overlap what the call reads. scale > 0.
+ * never reaches it, infinities and NaN included. q, gate and out have one type: F32, or the cache's. F32 rows over a
+ * 16-bit cache keep 32-bit accuracy (queries and probabilities go through the matrix cores in pieces). Of 16-bit rows the
+ * probabilities are rounded to their type before they meet the values, half a step each (2^-8 of their size in BF16, 2^-11
+ * in F16), beside the output's own rounding; statistics and sums are in 32 bits, and divided by the sum of the rounded
+ * ones. out may be q or gate (same strides where there is more than one row or head), and else must not overlap what the
+ * call reads. scale > 0.
  * workspace: aq_paged_attention_workspace bytes of device memory for these arguments (those for a batch's largest bounds
  * serve every batch within them), 16-byte aligned, contents irrelevant before and after; calls (and captured graphs)
  * that can run at the same time need one each. */

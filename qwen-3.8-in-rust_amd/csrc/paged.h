@@ -81,9 +81,9 @@ __device__ __forceinline__ bool paged_slot(const PagedKv &c, const int32_t *tabl
     return paged_units(c, paged_entry(c, table, max_pages, pos), pos, units);
 }
 
-// The sequence that row `row` belongs to, if any: the number of sequences that end at or before it (n_seq: all). A row before
-// the first one's row_start is in none all the same, which the caller looks at. row_start never falls, so the whole wave
-// looks at the ends of 64 blocks of sequences, then inside the first that ends after the row.
+// The sequence that row `row` belongs to, if any: the number of sequences that end at or before it (n_seq: all do). A row
+// before the first one's row_start is in none all the same, which the caller looks at. row_start never falls, so the whole
+// wave looks at the ends of 64 blocks of sequences, then inside the first that ends after the row.
 __device__ __forceinline__ uint32_t paged_seq_of(const PagedBatch &b, uint32_t row) {
     const uint32_t lane = threadIdx.x & 63;
     uint32_t lo = 0, hi = b.n_seq; // the answer is one of lo .. hi

@@ -132,7 +132,8 @@ void join_pick(const AttnPagedArgs &a, int R, int D, int rows, hipStream_t strea
 
 // ---------------------------------------------------------------------------------------------------- the plan
 // Of batches of more sequences or row tiles than a work-group divides by itself: all row tiles in order, and the prefix
-// sums of their units; one work-group.
+// sums of their units; one work-group. Around the border (single tokens at 200, 32 heads on 8 of 128, bf16): 1020 sequences
+// 260 us, 1030 265.
 __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint32_t tk) {
     __shared__ uint32_t wsum[16], carry, first[1024];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -245,7 +246,7 @@ Choice on_tiles(const aq_paged_kv *kv, const aq_paged_batch *b, uint32_t n_head,
     c.unit = c.many ? chunk_keys(c.D) : few_unit(kv->type, c.D, c.R);
     c.min_chunk = c.many ? 256 / c.unit : 1;
     // What a segment costs besides its positions (queries, first loads, the waves' meeting, its output), in units. Prompts
-    // of three requests (10,500 rows of 32 heads of 128), of 64 positions: 0: 794 us, 2: 532, 4: 459, 6: 459, 8: 467. Eight
+    // of three requests (9733 rows of 32 heads of 128), of 64 positions: 0: 794 us, 2: 532, 4: 459, 6: 459, 8: 467. Eight
     // verify batches of 32 rows (f32 over f16, heads of 256), of 32: 0: 46.4, 2: 42.5, 4: 42.6. Single tokens: none to gain;
     // nor where a unit takes as long as that (f32 products).
     c.lead = c.many ? 320 / c.unit : c.R == 32 && kv->type != AQ_TYPE_F32 ? 2 : 0;
@@ -257,8 +258,11 @@ Choice on_tiles(const aq_paged_kv *kv, const aq_paged_batch *b, uint32_t n_head,
     c.n_seg = (uint32_t)n_seg;
     // Two work-groups per CU; one of up to 16 rows over 16-bit pages, bound by the memory alone (48 sequences at 6000, 32
     // heads on 8 of 128: one 215 us, two 228, three 223; one sequence at 8000, 24 heads on 4 of 256: 17.7 and 19.0; but f32
-    // pages, 64 rows at 4001: 131 and 101). No more than there can be units.
-    const uint32_t per_cu = !c.many && c.R == 16 && kv->type != AQ_TYPE_F32 ? 1 : 2, most = (uint32_t)compute_units(device) * per_cu;
+    // pages, 64 rows at 4001: 131 and 101). Chunks at heads of 64 fit three: prompts 3 x 3500 of 16 heads 152 us with two,
+    // 148 with three, 512 rows at 8000 of 16 heads 45 and 45, 128 rows at 4000 of 16 heads on 4 23.7 and 25.3. No more than
+    // there can be units.
+    const uint32_t per_cu = !c.many && c.R == 16 && kv->type != AQ_TYPE_F32 ? 1 : 2;
+    const uint32_t most = (uint32_t)compute_units(device) * per_cu;
     const double units = (double)n_seg * kv->n_head_kv * c.per;
     const uint32_t shares = units < most ? (uint32_t)units : most;
     c.shares = shares > 8 ? (shares + 7) / 8 * 8 : std::max(shares, 1u);
@@ -277,7 +281,8 @@ int choose(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b, uin
     // segments (us): one sequence of 32 heads on 8 of 128 (bf16) at 150: 11.2 and 8.4, at 300: 11.2 and 10.1, at 500: 11.3
     // and 11.5; 64 of them at 150: 27.5 and 16.6, at 300: 37.2 and 26.2, at 500: 44.6 and 43.9, at 800: 59.0 and 65.0; 24
     // heads on 4 of 256 (f16), one at 150: 12.1 and 11.0, at 300: 13.2 and 13.5. Not where two waves share a unit (32 rows
-    // of 256 at 150: 14.3 and 18.2), nor with more segments than measured (1536).
+    // of 256 at 150: 14.3 and 18.2), nor with more segments than measured, eight a CU (128 sequences of 16 heads of 80 at
+    // 130: 74.3 and 35.7, of 64 at 285: 94.0 and 43.8).
     if (!c->many && !c->planned && few_groups(kv->type, c->D, c->R) == 1 && segs <= 8 * cus &&
         c->cap <= (c->D == 256 ? 256u : segs >= cus ? 512u : 384u)) {
         c->whole = c->per;

@@ -9,10 +9,11 @@
 // Split. All segments' units in order (sequence, K/V head, row tile, key unit: row tiles that read the same keys side by
 // side, on one XCD at one time), each segment's with `lead` places before them for what a segment costs besides its units,
 // form one line of `total` places, cut into work-group shares of `chunk` places each, however long or short the sequences
-// are (short contexts: every segment has `whole` places and is a share). A share that holds a whole segment writes its output; where a segment is cut, each share writes its part (row maxima, sums and unnormalised outputs, in
-// f32) to the workspace, slot 2w for the segment that began before share w, slot 2w + 1 for the one that goes on after
-// it, and a second launch joins the parts in order. Which share has which part follows from the lengths alone, so the
-// same call gives the same bits.
+// are (short contexts: every segment has `whole` places and is a share). A share that holds a whole segment writes its
+// output; where a segment is cut, each share writes its part (row maxima, sums and unnormalised outputs, in f32) to the
+// workspace, slot 2w for the segment that began before share w, slot 2w + 1 for the one that goes on after it, and a second
+// launch joins the parts in order. Which share has which part follows from the lengths alone, so the same call gives the
+// same bits.
 #pragma once
 
 #include "paged.h"

@@ -8,6 +8,9 @@
 //                 sum are in two lanes: one exchange (v_permlane32_swap) per tile.
 //   O^T = V^T P^T the exponentials, rounded, are B's layout as they stand if k-slot (h, e) stands for position 8 (e / 4) +
 //                 4 h + e % 4; A = V^T comes from the row-major V tile by transposing LDS reads (ds_read_b64_tr_b16).
+//                 Rounded to the rows' type, once, and summed as rounded: a second piece would be half as many products
+//                 again in a kernel that they bound. Largest error against 64 bits, relative to the largest output: bf16
+//                 0.0023, f16 0.00026, where the output's rounding alone gives 0.0017 and 0.00020.
 // The maximum a row's exponentials are taken against moves only when it grows by more than 2^7 (their scale leaves room
 // for that), so that outputs are rarely rescaled.
 //
@@ -15,10 +18,12 @@
 // which 16 bytes of its row it fetches: the row's chunks are swapped by an exclusive or with the row's low bits, so that
 // neither kind of read meets a bank twice. Rows without a page come from a row of zeros.
 //
-// Measured: 512 rows of 24 heads on 4 of 256 at 32,000 (bf16) 479 us, 847 TFLOP/s, where a library product of 8192^3 reaches
-// 1121; prompts of three requests of 3500, 32 heads on 8 of 128 (f16), 412 us, 734. Products and softmax (per score a
-// product, an exponential, a rounding, half a sum) take turns on two waves a SIMD; the next tile's products put beside
-// this one's softmax need the registers that hold the rows (770 for 792).
+// Measured, by box: 512 rows of 24 heads on 4 of 256 at 32,000 (bf16) 472 to 492 us, 860 to 825 TFLOP/s, where a library
+// product of 8192^3 reaches 1121; prompts of three requests of 3500, 32 heads on 8 of 128 (f16), 411 to 433 us, 736 to 698.
+// Heads that do not fill their padded size load by an address each: 512 rows at 8000, heads of 192, 98 us for 95 without
+// the zeros past the head. Products and softmax (per score a product, an exponential, a rounding, half a sum) take turns on
+// two waves a SIMD; at heads of 256 the next tile's products beside this one's softmax need the registers that hold the
+// rows (770 for 792 TFLOP/s). Heads of 128 and 64 leave some (198 and 150 registers); it was not tried there.
 #include <atomic>
 #include <type_traits>
 

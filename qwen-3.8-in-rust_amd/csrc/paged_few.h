@@ -11,11 +11,17 @@
 //                positions and turns the 8 x 8 block in registers (one v_perm per dword).
 // One running maximum and sum per row; a wave's four lane groups share the maximum, the sum is joined at the end.
 //
-// Measured: single tokens of 48 sequences at 6000 (bf16, 32 heads on 8 of 128) 215 us, 5.5 TB/s, where a plain read reaches
-// 6.3; of one sequence at 8000 (f16, 24 heads on 4 of 256) 17.8 us, two launches of latencies; four new tokens of eight
-// sequences at 3000 (f32 over f16, the same heads) 42.7 us, 2.5 TB/s: its 16 rows of 256 outputs leave registers for two
-// waves a SIMD, which wait for loads 56% of their time. Eight waves to a work-group there: 40.4 us, but contexts below 1000
-// 1 to 2 us slower and single tokens 5 to 8%.
+// 16-bit rows: the exponentials are rounded to the rows' type for the second product, once, and summed as rounded. Largest
+// error against 64 bits, relative to the largest output, where the output's rounding alone gives 0.0017 (bf16) and 0.00020
+// (f16): 0.0020 and 0.00022. A second piece of them, as f32 rows have, would take that away: single tokens of 48 sequences
+// at 6000 1% slower, at 3000 with heads of 64 5%, of 64 at 130 5%, verify batches 1 to 2%. Callers to whom it matters have
+// f32 rows.
+//
+// Measured: single tokens of 48 sequences at 6000 (bf16, 32 heads on 8 of 128) 215 to 223 us by box, 5.5 to 5.3 TB/s, where
+// a plain read reaches 6.3; of one sequence at 8000 (f16, 24 heads on 4 of 256) 17.8 us, two launches of latencies; four
+// new tokens of eight sequences at 3000 (f32 over f16, the same heads) 42.5 to 44.1 us, 2.5 TB/s: its 16 rows of 256
+// outputs leave registers for two waves a SIMD, which wait for loads 55% of their time. Eight waves to a work-group there:
+// 40.4 us for 42.7, but contexts below 1000 1 to 2 us slower and single tokens 5 to 8%.
 //
 // f32 rows over a 16-bit cache keep 32-bit accuracy: q, scaled to its row's exponent, and the probabilities go in as two
 // f16 or three bf16 pieces whose sum has 22 or 24 bits. f32 over f32 takes the f32 matrix cores (16x16x4).

@@ -7,7 +7,7 @@
 // applies them to several heads of the row, so the 64-bit work (a product, a floor, a difference per pair) stays
 // below the memory time from four heads on.
 //
-// Bound by their bytes: 8191 rows of 40 heads of 128 (bf16) 34.1 us, 4.9 TB/s where a copy reaches 5.3; 6000 new rows of 24
+// Bound by their bytes: 8191 rows of 40 heads of 128 (bf16) 34.1 us, 4.9 TB/s where a copy reaches 5.3; 5342 new rows of 24
 // query and 4 K/V heads of 256 (f32 into f16) appended in 65.5 us, 5.0 TB/s; 48 single tokens 5.2 us, an empty launch 2.4.
 #include <cmath>
 #include <memory>
