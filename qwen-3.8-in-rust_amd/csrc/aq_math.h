@@ -4,7 +4,7 @@
  *
  * The reference's `f32::exp` / `f32::ln_1p` (act.rs:7-40, softmax.rs:22-49, deltanet.rs:43-86) lower to the
  * platform libm's `expf` / `log1pf`: on Linux x86-64, GNU libc. This header restates the two algorithms of GNU
- * libc 2.35 (the version of this image and of the GPU boxes), from their published sources:
+ * libc 2.35, from their published sources:
  *
  *  expf   — the table method of Szabolcs Nagy's optimized-routines expf (glibc sysdeps/ieee754/flt-32/e_expf.c,
  *           e_exp2f_data.c; MIT/LGPL): x·32/ln2 = k + r, 2^(k/32) from a 32-entry table of 2^(i/32) with the

@@ -18,7 +18,7 @@
 // which 16 bytes of its row it fetches: the row's chunks are swapped by an exclusive or with the row's low bits, so that
 // neither kind of read meets a bank twice. Rows without a page come from a row of zeros.
 //
-// Measured, by box: 512 rows of 24 heads on 4 of 256 at 32,000 (bf16) 472 to 492 us, 860 to 825 TFLOP/s, where a library
+// Measured, by card: 512 rows of 24 heads on 4 of 256 at 32,000 (bf16) 472 to 492 us, 860 to 825 TFLOP/s, where a library
 // product of 8192^3 reaches 1121; prompts of three requests of 3500, 32 heads on 8 of 128 (f16), 411 to 433 us, 736 to 698.
 // Heads that do not fill their padded size load by an address each: 512 rows at 8000, heads of 192, 98 us for 95 without
 // the zeros past the head. Products and softmax (per score a product, an exponential, a rounding, half a sum) take turns on

@@ -17,7 +17,7 @@
 // at 6000 1% slower, at 3000 with heads of 64 5%, of 64 at 130 5%, verify batches 1 to 2%. Callers to whom it matters have
 // f32 rows.
 //
-// Measured: single tokens of 48 sequences at 6000 (bf16, 32 heads on 8 of 128) 215 to 223 us by box, 5.5 to 5.3 TB/s, where
+// Measured: single tokens of 48 sequences at 6000 (bf16, 32 heads on 8 of 128) 215 to 223 us by card, 5.5 to 5.3 TB/s, where
 // a plain read reaches 6.3; of one sequence at 8000 (f16, 24 heads on 4 of 256) 17.8 us, two launches of latencies; four
 // new tokens of eight sequences at 3000 (f32 over f16, the same heads) 42.5 to 44.1 us, 2.5 TB/s: its 16 rows of 256
 // outputs leave registers for two waves a SIMD, which wait for loads 55% of their time. Eight waves to a work-group there:
