@@ -318,6 +318,70 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
                        const aq_heads *q, const aq_heads *out, float scale, uint32_t window, const aq_heads *gate,
                        void *workspace, size_t workspace_bytes, void *stream);
 
+/* A norm for each head of queries and keys with the rotation in the same pass: the projections' rows as the 27B shapes'
+ * full-attention layers take them (gqa_attention.rs:340-363). y[r][h] = x[r][h] / sqrt(mean(x[r][h]^2) + eps) * weight, in 32
+ * bits, then rotated by pos_dev[r] and rounded once; the weights are head_dim f32 on the device, eps > 0. q or k may be null
+ * (with its output and weight); rope and pos_dev are null together: the norm alone. Both tensors have one type; each
+ * output may be its input (same strides), and else must not overlap what the call reads or writes. head_dim 1 to 256.
+ * Queued on `stream`, capturable, nothing allocated, as all of these calls. */
+int aq_qk_norm_rope(aq_ctx *ctx, const aq_heads *q, const aq_heads *q_out, uint32_t n_head, const aq_heads *k,
+                    const aq_heads *k_out, uint32_t n_head_kv, uint32_t head_dim, size_t n_rows, const float *q_weight,
+                    const float *k_weight, float eps, const aq_rope *rope, const int32_t *pos_dev, void *stream);
+/* aq_paged_append with that norm: k normed, rotated and stored in its page, v stored, q (nullable, with q_out and q_weight)
+ * normed and rotated into q_out. rope nullable: the norm alone. pos_dev (nullable): the position each of the n_rows rows is
+ * rotated by, where that is not its place in the sequence (a tree's drafts, which lie in the pages one after the other and
+ * stand at their depths); the page is by the place in either case. */
+int aq_paged_append_norm(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, const aq_heads *k,
+                         const aq_heads *v, const aq_heads *q, const aq_heads *q_out, uint32_t n_head,
+                         const float *q_weight, const float *k_weight, float eps, const aq_rope *rope,
+                         const int32_t *pos_dev, void *stream);
+
+/* Attention of trees of drafted tokens: each sequence's new rows are a tree's nodes, in any order. aq_paged_attention, but a
+ * row sees all that stands before its sequence's new rows, and of the new rows those that its mask names: bit j of the
+ * mask_words 32-bit words at mask_dev + r * mask_words (n_rows rows; mask_words * 32 at least max_rows) is the j-th new row of
+ * row r's sequence, its own among them (a row does not see itself unless its bit says so). With window > 0 a row whose mask
+ * has n bits sees of what stands before the new rows the last window - n positions, as the n-th of a run would. The same
+ * workspace (aq_paged_attention_workspace). A row that sees nothing is 0. */
+int aq_paged_tree_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, const uint32_t *mask_dev,
+                            uint32_t mask_words, uint32_t n_head, const aq_heads *q, const aq_heads *out, float scale,
+                            uint32_t window, const aq_heads *gate, void *workspace, size_t workspace_bytes, void *stream);
+/* The accepted path of each sequence's tree kept: of sequence s the new rows path_dev[s * max_path + i], i <
+ * path_len_dev[s], which rise (a tree whose nodes stand behind their parents: root first), become its new rows 0, 1, .. :
+ * their K and V rows move there, in the pages of all n_kv caches (one a layer: the same shape, strides and type, their own k
+ * and v), and kv_len_out[s] (nullable; not batch's kv_len) is the length without the others. The path ends at an entry that
+ * is no new row or not past the one before it. A row with no page is neither moved nor written over. Pages that are written
+ * belong to one sequence. */
+int aq_paged_tree_commit(aq_ctx *ctx, const aq_paged_kv *kv, uint32_t n_kv, const aq_paged_batch *batch,
+                         const int32_t *path_dev, const int32_t *path_len_dev, uint32_t max_path, int32_t *kv_len_out,
+                         void *stream);
+
+/* The page tables of n_seq sequences over a pool, and its free pages, all on the device: sequence s holds the pages
+ * pages[s * max_pages + i], i < held[s]. free_pages is a ring of n_pages entries, of which free_state[1] from place
+ * free_state[0] on are free pages. held_out and free_state_out receive the new counts: the same arrays for a step in place,
+ * others to look at a step before it is taken (what the old counts say is not touched). free_state and free_state_out are
+ * 4 values each; the third is the call's own and begins as 0 (two calls with one free_state_out must not overlap). */
+typedef struct aq_page_tables {
+    uint32_t n_seq, max_pages, n_pages, page_size;
+    int32_t *pages;
+    const int32_t *held;
+    int32_t *held_out;
+    int32_t *free_pages;
+    const int32_t *free_state;
+    int32_t *free_state_out;
+} aq_page_tables;
+/* One step's tables and maps from the requests' lengths: sequence s has kv_before[s] positions (below 0: 0) and gets n_new[s]
+ * new rows; n_new[s] < 0: it has ended. kv_len[s] becomes their sum (0 for one that ended), row_start (n_seq + 1 values) the
+ * sums of the new rows before each, as aq_paged_batch takes them. A sequence holds then as many pages as kv_len[s] needs,
+ * max_pages at most: what it lacks comes from the ring's front, in order of the sequences; what it has too many goes to the
+ * ring's end, for later calls. From the first sequence on whose pages are more than there are, no sequence gets any: its
+ * table has -1 for them, and missing[s] (nullable) says how many of the pages it needs it lacks. Of row r < n_rows, pos[r]
+ * (nullable) is its position, kv_before[s] + row_depth[r] where row_depth is given (a tree's drafts), and slots[r]
+ * (nullable) its place in the pool, page * page_size + slot; without a page, and behind the last sequence's rows, -1 (and
+ * position 0 there). kv_len may be kv_before, the other outputs are memory of their own. A page is held once. */
+int aq_paged_tables(aq_ctx *ctx, const aq_page_tables *tables, const int32_t *kv_before, const int32_t *n_new,
+                    uint32_t n_rows, int32_t *row_start, int32_t *kv_len, int32_t *missing, int32_t *pos, int64_t *slots,
+                    const int32_t *row_depth, void *stream);
+
 /* ------------------------------------------------------------------------------------ synthetic tensors */
 
 /* A deterministic synthetic tensor: value i is drawn from splitmix64 of (seed, i) (normal: the inverse normal CDF of

@@ -168,6 +168,11 @@ def lib():
         "aq_paged_append": (i, [P, P, P, P, P, P, P, P, C.c_uint32, P]),
         "aq_paged_attention_workspace": (i, [P, P, P, C.c_uint32, C.POINTER(sz)]),
         "aq_paged_attention": (i, [P, P, P, C.c_uint32, P, P, C.c_float, C.c_uint32, P, P, sz, P]),
+        "aq_qk_norm_rope": (i, [P, P, P, C.c_uint32, P, P, C.c_uint32, C.c_uint32, sz, P, P, C.c_float, P, P, P]),
+        "aq_paged_append_norm": (i, [P, P, P, P, P, P, P, C.c_uint32, P, P, C.c_float, P, P, P]),
+        "aq_paged_tree_attention": (i, [P, P, P, P, C.c_uint32, C.c_uint32, P, P, C.c_float, C.c_uint32, P, P, sz, P]),
+        "aq_paged_tree_commit": (i, [P, P, C.c_uint32, P, P, P, C.c_uint32, P, P]),
+        "aq_paged_tables": (i, [P, P, P, P, C.c_uint32, P, P, P, P, P, P, P]),
     }
     for name, (res, args) in sigs.items():
         f = getattr(L, name)
@@ -762,6 +767,31 @@ def paged_batch(n_seq, row_start, kv_len, pages, max_pages, n_rows, max_rows, ma
     return b
 
 
+class AqPageTables(C.Structure):
+    _fields_ = [("n_seq", C.c_uint32), ("max_pages", C.c_uint32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("pages", C.c_void_p), ("held", C.c_void_p), ("held_out", C.c_void_p), ("free_pages", C.c_void_p),
+                ("free_state", C.c_void_p), ("free_state_out", C.c_void_p)]
+
+
+def page_tables(n_seq, max_pages, n_pages, page_size, pages, held, free_pages, free_state, held_out=None,
+                free_state_out=None):
+    """aq_page_tables: the sequences' page tables and the pool's free pages (device int32 arrays); without held_out and
+    free_state_out a step is taken in place."""
+    held_out = held if held_out is None else held_out
+    free_state_out = free_state if free_state_out is None else free_state_out
+    t = AqPageTables(n_seq, max_pages, n_pages, page_size, dev_ptr(pages), dev_ptr(held), dev_ptr(held_out),
+                     dev_ptr(free_pages), dev_ptr(free_state), dev_ptr(free_state_out))
+    t.keep = (pages, held, held_out, free_pages, free_state, free_state_out)
+    return t
+
+
+def paged_kv_array(kvs):
+    """The caches of several layers (paged_kv) as the array that paged_tree_commit takes."""
+    a = (AqPagedKv * len(kvs))(*kvs)
+    a.keep = [kv.keep for kv in kvs]
+    return a
+
+
 class Rope:
     """aq_rope: a rotation's frequencies on the device (rope.rs:10-16); layout "half" or "interleaved", scaling "none",
     "linear" or "yarn"."""
@@ -818,6 +848,50 @@ def paged_attention(ctx: Context, kv, batch, n_head, q, out, scale, window=0, ga
         workspace_bytes = workspace.nbytes if isinstance(workspace, DeviceBuffer) else 0
     check(lib().aq_paged_attention(ctx.h, _ref(kv), _ref(batch), n_head, _ref(q), _ref(out), scale, window, _ref(gate),
                                    dev_ptr(workspace), workspace_bytes, stream))
+
+
+def qk_norm_rope(ctx: Context, q, q_out, n_head, k, k_out, n_head_kv, head_dim, n_rows, q_weight, k_weight, eps,
+                 rope=None, pos=None, stream=None):
+    """Each head of q and k over its root mean square, times its weight, rotated by pos (aq_qk_norm_rope), queued."""
+    check(lib().aq_qk_norm_rope(ctx.h, _ref(q), _ref(q_out), n_head, _ref(k), _ref(k_out), n_head_kv, head_dim, n_rows,
+                                dev_ptr(q_weight), dev_ptr(k_weight), eps, None if rope is None else rope.h,
+                                dev_ptr(pos), stream))
+
+
+def paged_append_norm(ctx: Context, kv, batch, k, v, q, q_out, n_head, q_weight, k_weight, eps, rope=None, pos=None,
+                      stream=None):
+    """paged_append with the heads' norms; pos: positions other than the rows' places (aq_paged_append_norm), queued."""
+    check(lib().aq_paged_append_norm(ctx.h, _ref(kv), _ref(batch), _ref(k), _ref(v), _ref(q), _ref(q_out), n_head,
+                                     dev_ptr(q_weight), dev_ptr(k_weight), eps, None if rope is None else rope.h,
+                                     dev_ptr(pos), stream))
+
+
+def paged_tree_attention(ctx: Context, kv, batch, mask, mask_words, n_head, q, out, scale, window=0, gate=None,
+                         workspace=None, workspace_bytes=None, stream=None):
+    """Attention of each sequence's tree of new rows over its pages (aq_paged_tree_attention), queued; the workspace is
+    paged_attention's."""
+    if workspace_bytes is None:
+        workspace_bytes = workspace.nbytes if isinstance(workspace, DeviceBuffer) else 0
+    check(lib().aq_paged_tree_attention(ctx.h, _ref(kv), _ref(batch), dev_ptr(mask), mask_words, n_head, _ref(q),
+                                        _ref(out), scale, window, _ref(gate), dev_ptr(workspace), workspace_bytes,
+                                        stream))
+
+
+def paged_tree_commit(ctx: Context, kvs, batch, path, path_len, max_path, kv_len_out=None, stream=None):
+    """Each sequence's accepted path moved to the front of its new rows, in all caches (paged_kv_array, or one paged_kv;
+    aq_paged_tree_commit), queued."""
+    n = len(kvs) if isinstance(kvs, C.Array) else 1
+    check(lib().aq_paged_tree_commit(ctx.h, _ref(kvs), n, _ref(batch), dev_ptr(path), dev_ptr(path_len), max_path,
+                                     dev_ptr(kv_len_out), stream))
+
+
+def paged_tables(ctx: Context, tables, kv_before, n_new, n_rows, row_start, kv_len, missing=None, pos=None, slots=None,
+                 row_depth=None, stream=None):
+    """A step's page tables, row starts, lengths, positions and slots from the requests' lengths (aq_paged_tables),
+    queued."""
+    check(lib().aq_paged_tables(ctx.h, _ref(tables), dev_ptr(kv_before), dev_ptr(n_new), n_rows, dev_ptr(row_start),
+                                dev_ptr(kv_len), dev_ptr(missing), dev_ptr(pos), dev_ptr(slots), dev_ptr(row_depth),
+                                stream))
 
 
 # ------------------------------------------------------------------------------------------------ GGUF files

@@ -1,0 +1,382 @@
+// page_tables.hip — the page tables of a step of a batch of sequences, on the device (aq_paged_tables), and the accepted path
+// of a tree of drafts kept in the pages (aq_paged_tree_commit).
+//
+// Tables. A sequence that will have n positions wants ceil(n / page_size) pages. What it lacks it takes from the front of a
+// ring of free pages, what it has too many it puts at the ring's end, and each knows its place in the ring from the sums over
+// the sequences before it: the same call gives the same tables. Pages put back are for the next call, so that what is read
+// (the ring's free pages, the tables' held entries) and what is written (the ring behind them, the entries past them) are
+// apart, and every work-group can work all of it out by itself: each scans the sequences, 1024 at a time, then takes every
+// so many of the rows, of the pages taken and of those put back. Only the lengths, the counts and the ring's state may be
+// written over what the others still read: the last work-group to arrive at a counter writes those.
+//
+// Commit. A path's rows rise, so its e-th row lies at or past place e, and moved in order none overwrites one that is still
+// to move. A work-group has one sequence's K or V rows in one cache: its lanes find 64 entries' places at a time, then each
+// thread moves its 16 bytes of a row for entry after entry, eight on their way.
+#include <climits>
+
+#include "paged.h"
+
+namespace aq {
+namespace {
+
+constexpr uint32_t SCAN = 1024, TABLE_THREADS = 256, PER = SCAN / TABLE_THREADS;
+
+struct TablesArgs {
+    const int32_t *before, *fresh, *held, *state, *depth;
+    int32_t *pages, *ring, *held_out, *state_out, *row_start, *kv_len, *missing, *pos;
+    int64_t *slots;
+    uint32_t n_seq, max_pages, n_pages, n_rows;
+    FastDiv page_size;
+};
+
+// Of a chunk of sequences: the sums of rows, of pages taken and of pages put back before each, and what each has and wants.
+struct TablesLds {
+    uint64_t rows[SCAN + 1], take[SCAN + 1], back[SCAN + 1], wsum[3][4], taken;
+    int32_t before[SCAN];
+    uint32_t held[SCAN], want[SCAN];
+    uint32_t last;
+};
+
+// One sequence: its new rows, the pages it holds, those it needs and those of them that its table has room for.
+struct Request {
+    uint32_t rows, held, want, need;
+    int32_t before, len;
+};
+__device__ __forceinline__ Request request(const TablesArgs &a, uint32_t s) {
+    Request r = {0, 0, 0, 0, 0, 0};
+    if (s >= a.n_seq) return r;
+    const int32_t fresh = a.fresh[s], before = a.before[s], held = a.held[s];
+    r.held = (uint32_t)min(max(held, 0), (int32_t)a.max_pages);
+    if (fresh < 0) return r; // ended: it needs nothing
+    r.before = max(before, 0);
+    r.rows = (uint32_t)fresh;
+    r.len = (int32_t)min((uint64_t)r.before + r.rows, (uint64_t)INT_MAX);
+    r.need = (uint32_t)(((uint64_t)r.len + a.page_size.d - 1) / a.page_size.d);
+    r.want = min(r.need, a.max_pages);
+    return r;
+}
+__device__ __forceinline__ uint32_t over(uint32_t x, uint32_t y) { return x > y ? x - y : 0u; }
+
+// The last of sums[0 .. n - 1] that is at or below x, for sums[0] <= x < sums[n].
+__device__ __forceinline__ uint32_t find(const uint64_t *sums, uint64_t x, uint32_t n) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (sums[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(TablesArgs a) {
+    __shared__ TablesLds lds;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t first = (uint32_t)a.state[0] % a.n_pages, count = (uint32_t)min(max(a.state[1], 0), (int32_t)a.n_pages);
+    const uint32_t me = blockIdx.x * TABLE_THREADS + tid, all = gridDim.x * TABLE_THREADS;
+    auto ring = [&](uint64_t i) -> int32_t & { // its i-th place; past the second turn only where the counts are wrong
+        i += first;
+        return a.ring[i < a.n_pages ? i : i < 2ull * a.n_pages ? i - a.n_pages : i % a.n_pages];
+    };
+
+    // The chunk of sequences from s0 on, onto the sums of those before it.
+    uint64_t sums0[3] = {0, 0, 0};
+    Request r[PER];
+    auto scan = [&](uint32_t s0) {
+        uint64_t sum[3] = {0, 0, 0}, in[3];
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            r[i] = request(a, s0 + tid * PER + i);
+            sum[0] += r[i].rows;
+            sum[1] += over(r[i].want, r[i].held);
+            sum[2] += over(r[i].held, r[i].want);
+        }
+        __syncthreads(); // the chunk before is read
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            in[k] = sum[k];
+            for (uint32_t d = 1; d < 64; d *= 2) {
+                const uint64_t x = __shfl_up((unsigned long long)in[k], d);
+                if (lane >= d) in[k] += x;
+            }
+            if (lane == 63) lds.wsum[k][wave] = in[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            in[k] += sums0[k] - sum[k];
+            for (uint32_t w = 0; w < TABLE_THREADS / 64; w++) {
+                if (w < wave) in[k] += lds.wsum[k][w];
+                sums0[k] += lds.wsum[k][w];
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            const uint32_t l = tid * PER + i;
+            lds.rows[l] = in[0];
+            lds.take[l] = in[1];
+            lds.back[l] = in[2];
+            lds.before[l] = r[i].before;
+            lds.held[l] = r[i].held;
+            lds.want[l] = r[i].want;
+            in[0] += r[i].rows;
+            in[1] += over(r[i].want, r[i].held);
+            in[2] += over(r[i].held, r[i].want);
+        }
+        if (tid == TABLE_THREADS - 1) {
+            lds.rows[SCAN] = in[0];
+            lds.take[SCAN] = in[1];
+            lds.back[SCAN] = in[2];
+        }
+        __syncthreads();
+    };
+    // Whether all that the chunk's sequences up to l take is there.
+    auto served = [&](uint32_t l) { return lds.take[l + 1] <= count; };
+    auto row_items = [&](uint32_t s0, uint32_t n) {
+        const uint64_t end = min(lds.rows[n], (uint64_t)a.n_rows);
+        for (uint64_t i = lds.rows[0] + me; i < end; i += all) {
+            const uint32_t l = find(lds.rows, i, n);
+            const uint64_t p = (uint64_t)lds.before[l] + (i - lds.rows[l]);
+            const uint32_t at = (uint32_t)min(p, (uint64_t)INT_MAX), col = a.page_size.quot(at);
+            if (a.pos) a.pos[i] = a.depth ? (int32_t)((uint32_t)lds.before[l] + (uint32_t)a.depth[i]) : (int32_t)at;
+            if (a.slots) { // in a page held before, or taken now
+                int32_t page = -1;
+                if (col < lds.want[l] && p <= INT_MAX) {
+                    if (col < lds.held[l]) page = a.pages[(size_t)(s0 + l) * a.max_pages + col];
+                    else if (served(l)) page = ring(lds.take[l] + (col - lds.held[l]));
+                }
+                a.slots[i] = (uint32_t)page < a.n_pages ? (int64_t)page * a.page_size.d + (at - col * a.page_size.d) : -1;
+            }
+        }
+    };
+    auto page_items = [&](uint32_t s0, uint32_t n) {
+        for (uint64_t i = lds.take[0] + me; i < lds.take[n]; i += all) {
+            const uint32_t l = find(lds.take, i, n), col = lds.held[l] + (uint32_t)(i - lds.take[l]);
+            a.pages[(size_t)(s0 + l) * a.max_pages + col] = served(l) ? ring(i) : -1;
+        }
+        for (uint64_t i = lds.back[0] + me; i < lds.back[n]; i += all) { // behind the pages that were free
+            const uint32_t l = find(lds.back, i, n), col = lds.want[l] + (uint32_t)(i - lds.back[l]);
+            ring(count + i) = a.pages[(size_t)(s0 + l) * a.max_pages + col];
+        }
+    };
+
+    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += SCAN) {
+        scan(s0);
+        row_items(s0, min(a.n_seq - s0, SCAN));
+        page_items(s0, min(a.n_seq - s0, SCAN));
+    }
+    for (uint64_t i = sums0[0] + me; i < a.n_rows; i += all) { // behind the last sequence
+        if (a.pos) a.pos[i] = 0;
+        if (a.slots) a.slots[i] = -1;
+    }
+
+    if (gridDim.x > 1) { // what was read is read; the counter ends at 0 again
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) lds.last = atomicInc((unsigned *)&a.state_out[2], gridDim.x - 1) == gridDim.x - 1;
+        __syncthreads();
+        if (!lds.last) return;
+        __threadfence();
+    }
+    if (tid == 0) lds.taken = 0;
+    if (a.n_seq > SCAN) sums0[0] = sums0[1] = sums0[2] = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += SCAN) {
+        if (a.n_seq > SCAN) scan(s0); // else still there
+        else __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            const uint32_t l = tid * PER + i, s = s0 + l;
+            if (s >= a.n_seq) continue;
+            const uint32_t take = over(r[i].want, r[i].held);
+            a.row_start[s] = (int32_t)min(lds.rows[l], (uint64_t)INT_MAX);
+            a.kv_len[s] = r[i].len;
+            a.held_out[s] = (int32_t)(served(l) ? r[i].want : min(r[i].held, r[i].want));
+            if (a.missing) a.missing[s] = (int32_t)(r[i].need - r[i].want + (served(l) ? 0u : take));
+            if (served(l) && take) atomicMax((unsigned long long *)&lds.taken, (unsigned long long)lds.take[l + 1]);
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        a.row_start[a.n_seq] = (int32_t)min(sums0[0], (uint64_t)INT_MAX);
+        const uint32_t taken = (uint32_t)lds.taken; // at most count
+        a.state_out[0] = (int32_t)((first + (uint64_t)taken) % a.n_pages);
+        a.state_out[1] = (int32_t)min(count - taken + sums0[2], (uint64_t)a.n_pages);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- the commit
+constexpr uint32_t MAX_CACHES = 64; // of a launch
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+
+struct CommitArgs {
+    PagedKv kv; // the shape of all; k and v unused
+    PagedBatch b;
+    const int32_t *path, *path_len;
+    int32_t *kv_len_out;
+    uint32_t max_path, chunks; // 16-byte pieces of a row of all heads
+    FastDiv per_head;          // of one head's
+    char *pools[2 * MAX_CACHES];
+};
+
+__global__ void __launch_bounds__(256) commit_kernel(CommitArgs a) {
+    constexpr int FLIGHT = 8;
+    const uint32_t seq = blockIdx.x, lane = threadIdx.x & 63;
+    char *const pool = a.pools[blockIdx.y];
+    const int32_t *path = a.path + (size_t)seq * a.max_path, *table = a.b.pages + (size_t)seq * a.b.max_pages;
+    const SeqRows sr = paged_seq(a.b, seq);
+    const int32_t fresh = sr.len - sr.base; // all of its new rows
+    const uint32_t len = (uint32_t)min(max(a.path_len[seq], 0), (int32_t)min(a.max_path, (uint32_t)INT_MAX));
+    int32_t before = -1;  // the entry before the 64
+    uint32_t kept = 0;
+    bool whole = true;
+    for (uint32_t e0 = 0; e0 < len && whole; e0 += 64) { // uniform
+        const uint32_t e = e0 + lane;
+        const int32_t from = e < len ? path[e] : -1;
+        const int32_t prev = lane ? __shfl_up(from, 1) : before;
+        const uint64_t good = __ballot(e < len && from > prev && from < fresh);
+        const uint32_t n = good == ~0ull ? 64u : (uint32_t)__builtin_ctzll(~good); // up to the first that does not rise
+        before = __shfl(from, 63);
+        kept += n;
+        whole = n == 64;
+        const int32_t src = sr.base + from, dst = sr.base + (int32_t)e;
+        uint32_t from_units = 0, to_units = 0;
+        bool moves = lane < n && from != (int32_t)e && dst >= 0;
+        if (moves) {
+            const uint32_t x = paged_entry(a.kv, table, a.b.max_pages, (uint32_t)src),
+                           y = paged_entry(a.kv, table, a.b.max_pages, (uint32_t)dst);
+            moves = paged_units(a.kv, x, (uint32_t)src, &from_units);
+            moves = paged_units(a.kv, y, (uint32_t)dst, &to_units) && moves;
+        }
+        const uint64_t todo = __ballot(moves);
+        if (!todo) continue;
+        for (uint32_t c = threadIdx.x; c < a.chunks; c += blockDim.x) {
+            const uint32_t head = a.per_head.quot(c);
+            char *const at = pool + (uint64_t)head * a.kv.head_bytes + (c - head * a.per_head.d) * 16;
+            uint64_t rest = todo;
+            while (rest) { // uniform
+                u4 x[FLIGHT];
+                uint64_t left = rest;
+#pragma unroll
+                for (int i = 0; i < FLIGHT; i++) {
+                    if (!left) break;
+                    const int l = __builtin_ctzll(left);
+                    left &= left - 1;
+                    x[i] = *reinterpret_cast<const u4 *>(
+                        at + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)from_units, l) << a.kv.unit_shift));
+                }
+#pragma unroll
+                for (int i = 0; i < FLIGHT; i++) {
+                    if (!rest) break;
+                    const int l = __builtin_ctzll(rest);
+                    rest &= rest - 1;
+                    *reinterpret_cast<u4 *>(
+                        at + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)to_units, l) << a.kv.unit_shift)) = x[i];
+                }
+            }
+        }
+    }
+    if (a.kv_len_out && blockIdx.y == 0 && threadIdx.x == 0) a.kv_len_out[seq] = max(sr.base + (int32_t)kept, 0);
+}
+
+} // namespace
+} // namespace aq
+
+using namespace aq;
+
+extern "C" {
+
+int aq_paged_tables(aq_ctx *ctx, const aq_page_tables *t, const int32_t *kv_before, const int32_t *n_new, uint32_t n_rows,
+                    int32_t *row_start, int32_t *kv_len, int32_t *missing, int32_t *pos, int64_t *slots,
+                    const int32_t *row_depth, void *stream) {
+    AQ_REQUIRE(ctx && t, "aq_paged_tables: null argument");
+    AQ_REQUIRE(t->n_seq < (1u << 24) && n_rows < (1u << 24), "aq_paged_tables: batch size (fewer than 2^24 rows)");
+    AQ_REQUIRE(t->n_pages > 0 && t->n_pages < (1u << 31) && t->page_size > 0 && t->page_size < (1u << 31),
+               "aq_paged_tables: pages");
+    AQ_REQUIRE(t->n_seq == 0 || t->max_pages > 0, "aq_paged_tables: max_pages");
+    AQ_REQUIRE((uint64_t)t->max_pages * t->page_size <= (1ull << 31) - 1024,
+               "aq_paged_tables: the page table reaches past 2^31 positions");
+    AQ_REQUIRE(t->free_pages && t->free_state && t->free_state_out, "aq_paged_tables: null free pages");
+    AQ_REQUIRE(t->n_seq == 0 || (t->pages && t->held && t->held_out && kv_before && n_new && kv_len),
+               "aq_paged_tables: null array");
+    AQ_REQUIRE(row_start, "aq_paged_tables: null row_start");
+    AQ_REQUIRE(!row_depth || pos, "aq_paged_tables: depths without positions");
+    const void *all[] = {t->pages, t->held,  t->held_out, t->free_pages, t->free_state, t->free_state_out, kv_before,
+                         n_new,    row_start, kv_len,     missing,       pos,           row_depth};
+    for (const void *p : all) AQ_REQUIRE((uintptr_t)p % 4 == 0, "aq_paged_tables: an array is not aligned to its type");
+    AQ_REQUIRE((uintptr_t)slots % 8 == 0, "aq_paged_tables: an array is not aligned to its type");
+    AQ_REQUIRE(t->n_seq == 0 || (n_new != kv_len && n_new != t->held_out && n_new != row_start && kv_before != row_start &&
+                                 kv_before != t->held_out && t->held != kv_len),
+               "aq_paged_tables: an output lies over another input");
+    TablesArgs a;
+    a.before = kv_before;
+    a.fresh = n_new;
+    a.held = t->held;
+    a.state = t->free_state;
+    a.depth = row_depth;
+    a.pages = t->pages;
+    a.ring = t->free_pages;
+    a.held_out = t->held_out;
+    a.state_out = t->free_state_out;
+    a.row_start = row_start;
+    a.kv_len = kv_len;
+    a.missing = missing;
+    a.pos = pos;
+    a.slots = slots;
+    a.n_seq = t->n_seq;
+    a.max_pages = t->max_pages;
+    a.n_pages = t->n_pages;
+    a.n_rows = n_rows;
+    a.page_size = FastDiv(t->page_size);
+    const uint32_t items = (n_rows > t->n_seq ? n_rows : t->n_seq) / (4 * TABLE_THREADS);
+    const uint32_t grid = items < 1 ? 1 : items > 256 ? 256 : items;
+    AQ_HIP(hipSetDevice(ctx->device));
+    tables_kernel<<<grid, TABLE_THREADS, 0, stream ? (hipStream_t)stream : ctx->stream>>>(a);
+    AQ_HIP(hipGetLastError());
+    return 0;
+}
+
+int aq_paged_tree_commit(aq_ctx *ctx, const aq_paged_kv *kv, uint32_t n_kv, const aq_paged_batch *batch,
+                         const int32_t *path_dev, const int32_t *path_len_dev, uint32_t max_path, int32_t *kv_len_out,
+                         void *stream) {
+    const char *call = "aq_paged_tree_commit";
+    AQ_REQUIRE(ctx && kv && n_kv > 0, "aq_paged_tree_commit: null argument");
+    CommitArgs a;
+    for (uint32_t i = 0; i < n_kv; i++) {
+        const int rc = check_paged(call, kv + i, batch, &a.kv, &a.b);
+        if (rc) return rc;
+        const aq_paged_kv &x = kv[i], &y = kv[0];
+        AQ_REQUIRE(x.type == y.type && x.n_pages == y.n_pages && x.page_size == y.page_size && x.n_head_kv == y.n_head_kv &&
+                       x.head_dim == y.head_dim && x.page_stride == y.page_stride && x.slot_stride == y.slot_stride &&
+                       x.head_stride == y.head_stride,
+                   "aq_paged_tree_commit: caches of different shapes");
+    }
+    AQ_REQUIRE(batch->n_seq == 0 || (path_dev && path_len_dev && max_path > 0), "aq_paged_tree_commit: null path");
+    AQ_REQUIRE(max_path < (1u << 24), "aq_paged_tree_commit: max_path");
+    AQ_REQUIRE((uintptr_t)path_dev % 4 == 0 && (uintptr_t)path_len_dev % 4 == 0 && (uintptr_t)kv_len_out % 4 == 0,
+               "aq_paged_tree_commit: an array is not aligned to its type");
+    AQ_REQUIRE(!kv_len_out || batch->n_seq == 0 || (kv_len_out != batch->kv_len && kv_len_out != path_len_dev),
+               "aq_paged_tree_commit: kv_len_out lies over an input");
+    if (batch->n_seq == 0) return 0;
+    a.path = path_dev;
+    a.path_len = path_len_dev;
+    a.max_path = max_path;
+    const uint32_t per_head = (uint32_t)(kv->head_dim * type_bytes(kv->type) / 16);
+    a.chunks = per_head * kv->n_head_kv;
+    a.per_head = FastDiv(per_head);
+    uint32_t threads = 64;
+    while (threads < 256 && threads < a.chunks) threads *= 2;
+    AQ_HIP(hipSetDevice(ctx->device));
+    const hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
+    for (uint32_t i = 0; i < n_kv; i += MAX_CACHES) {
+        const uint32_t n = n_kv - i < MAX_CACHES ? n_kv - i : MAX_CACHES;
+        for (uint32_t j = 0; j < n; j++) {
+            a.pools[2 * j] = (char *)kv[i + j].k;
+            a.pools[2 * j + 1] = (char *)kv[i + j].v;
+        }
+        a.kv_len_out = i ? nullptr : kv_len_out;
+        commit_kernel<<<dim3(batch->n_seq, 2 * n), threads, 0, st>>>(a);
+        AQ_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+} // extern "C"

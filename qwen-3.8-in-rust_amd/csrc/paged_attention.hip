@@ -1,5 +1,5 @@
-// paged_attention.hip — attention over a paged K/V cache (aq_paged_attention): the choice of kernel (paged_few.h for
-// few rows and for f32 rows, paged_chunk.hip for many 16-bit rows), the plan and the join of split sequences.
+// paged_attention.hip — attention over a paged K/V cache (aq_paged_attention, aq_paged_tree_attention): the choice of kernel
+// (paged_few.h for few rows and for f32 rows, paged_chunk.h for many 16-bit rows), the plan and the join of split sequences.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -134,6 +134,7 @@ void join_pick(const AttnPagedArgs &a, int R, int D, int rows, hipStream_t strea
 // Of batches of more sequences or row tiles than a work-group divides by itself: all row tiles in order, and the prefix
 // sums of their units; one work-group. Around the border (single tokens at 200, 32 heads on 8 of 128, bf16): 1020 sequences
 // 260 us, 1030 265.
+template <bool TREE>
 __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint32_t tk) {
     __shared__ uint32_t wsum[16], carry, first[1024];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(AttnPagedArgs a, int R, uint
     for (uint32_t j0 = 0; j0 < n_seg; j0 += 1024) {
         const uint32_t j = j0 + tid;
         uint32_t n = 0;
-        if (j < n_seg) n = tile_count(a, a.tiles[j].seq, a.tiles[j].rt, R, tk); // its own, or ordered by the barriers above
+        if (j < n_seg) n = tile_count<TREE>(a, a.tiles[j].seq, a.tiles[j].rt, R, tk); // its own, or ordered by the barriers above
         const uint32_t end = scan(n);
         if (j < n_seg) a.plan[PLAN_HEAD + j + 1] = end;
     }
@@ -212,7 +213,7 @@ int compute_units(int device) {
 
 // Which kernel, its row tile and padded head size, and how its work is split.
 struct Choice {
-    bool many = false; // paged_chunk.hip
+    bool many = false; // paged_chunk.h
     int R = 16, D = 64;
     uint32_t unit = 0, per = 0, shares = 0, min_chunk = 1, lead = 0, whole = 0, n_seg = 0, cap = 0;
     bool planned = false, join = false;
@@ -307,8 +308,9 @@ int check_attention(const char *call, aq_ctx *ctx, const aq_paged_kv *kv, const 
 
 } // namespace
 
-int launch_paged_plan(const AttnPagedArgs &a, int R, uint32_t tk, hipStream_t stream) {
-    plan_kernel<<<1, 1024, 0, stream>>>(a, R, tk);
+int launch_paged_plan(const AttnPagedArgs &a, bool tree, int R, uint32_t tk, hipStream_t stream) {
+    if (tree) plan_kernel<true><<<1, 1024, 0, stream>>>(a, R, tk);
+    else plan_kernel<false><<<1, 1024, 0, stream>>>(a, R, tk);
     AQ_HIP(hipGetLastError());
     return 0;
 }
@@ -322,6 +324,80 @@ int launch_paged_combine(const AttnPagedArgs &a, int R, int D, int rows, hipStre
     AQ_HIP(hipGetLastError());
     return 0;
 }
+
+namespace {
+// Both calls; mask null: each row sees what stands up to its own position.
+int attend(const char *call, aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, const uint32_t *mask,
+           uint32_t mask_words, uint32_t n_head, const aq_heads *q, const aq_heads *out, float scale, uint32_t window,
+           const aq_heads *gate, void *workspace, size_t workspace_bytes, void *stream) {
+    auto who = [&] { return std::string(call); };
+    AttnPagedArgs a;
+    int rc = check_attention(call, ctx, kv, batch, n_head, &a.kv, &a.b);
+    if (rc) return rc;
+    const uint32_t rows = batch->n_rows, hd = kv->head_dim;
+    rc = check_heads(call, "q", q, rows, n_head, hd);
+    if (!rc) rc = check_heads(call, "out", out, rows, n_head, hd);
+    if (!rc && gate) rc = check_heads(call, "gate", gate, rows, n_head, hd);
+    if (rc) return rc;
+    AQ_REQUIRE(q->type == AQ_TYPE_F32 || q->type == kv->type, who() + ": rows are F32 or of the cache's type");
+    AQ_REQUIRE(out->type == q->type && (!gate || gate->type == q->type),
+               who() + ": q, gate and out of different types");
+    auto apart = [&](const aq_heads *x) { // each output where its own input is, or in memory of its own
+        return out->data != x->data || ((rows <= 1 || out->row_stride == x->row_stride) &&
+                                        (n_head <= 1 || out->head_stride == x->head_stride));
+    };
+    AQ_REQUIRE(apart(q) && (!gate || apart(gate)), who() + ": in place needs the same strides");
+    AQ_REQUIRE(std::isfinite(scale) && scale > 0.0f, who() + ": scale");
+    if (rows == 0 || batch->n_seq == 0 || batch->max_rows == 0) return 0;
+    Choice c;
+    rc = choose(call, kv, batch, n_head, q->type == AQ_TYPE_F32, ctx->device, &c);
+    if (rc) return rc;
+    AQ_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0, who() + ": workspace is null or not 16-byte aligned");
+    AQ_REQUIRE(workspace_bytes >= c.space.bytes, who() + ": workspace of " + std::to_string(workspace_bytes) +
+                                                     " bytes, " + std::to_string(c.space.bytes) + " needed");
+    a.q = heads_view(q);
+    a.out = heads_view(out);
+    if (gate) a.gate = heads_view(gate);
+    a.n_head = (int)n_head;
+    a.G = (int)(n_head / kv->n_head_kv);
+    a.by_g = FastDiv((uint32_t)a.G);
+    a.window = window;
+    a.mask = mask;
+    a.mask_words = mask_words;
+    a.cap = c.cap;
+    a.scale_log2 = scale * 1.44269504088896340736f;
+    a.q_wide = heads_aligned(q, rows, n_head);
+    a.out_wide = heads_aligned(out, rows, n_head) && (!gate || heads_aligned(gate, rows, n_head));
+    a.shares = c.shares;
+    a.min_chunk = c.min_chunk;
+    a.lead = c.lead;
+    a.whole = c.whole;
+    a.n_seg = c.n_seg;
+    a.planned = c.planned;
+    char *ws = (char *)workspace;
+    a.plan = (uint32_t *)(ws + c.space.plan);
+    a.tiles = (RowTile *)(ws + c.space.seg);
+    a.part_o = (float *)(ws + c.space.o);
+    a.part_ml = (float *)(ws + c.space.ml);
+    AQ_HIP(hipSetDevice(ctx->device));
+    const hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
+    if (c.planned) {
+        rc = launch_paged_plan(a, mask != nullptr, c.R, c.unit, st);
+        if (rc) return rc;
+    }
+    if (c.many) {
+        rc = mask ? launch_tree_chunk(a, c.D, st) : launch_paged_chunk(a, c.D, st);
+    } else if (kv->type == AQ_TYPE_F32) {
+        rc = mask ? launch_tree_few_f32(a, c.D, c.R, st) : launch_paged_few_f32(a, c.D, c.R, st);
+    } else if (kv->type == AQ_TYPE_F16) {
+        rc = mask ? launch_tree_few_f16(a, c.D, c.R, st) : launch_paged_few_f16(a, c.D, c.R, st);
+    } else {
+        rc = mask ? launch_tree_few_bf16(a, c.D, c.R, st) : launch_paged_few_bf16(a, c.D, c.R, st);
+    }
+    if (rc || !c.join) return rc;
+    return launch_paged_combine(a, c.R, c.D, (int)std::min<uint64_t>((uint64_t)c.R, (uint64_t)batch->max_rows * a.G), st);
+}
+} // namespace
 
 } // namespace aq
 
@@ -352,70 +428,22 @@ int aq_paged_attention_workspace(aq_ctx *ctx, const aq_paged_kv *kv, const aq_pa
 int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, uint32_t n_head,
                        const aq_heads *q, const aq_heads *out, float scale, uint32_t window, const aq_heads *gate,
                        void *workspace, size_t workspace_bytes, void *stream) {
-    const char *call = "aq_paged_attention";
-    AttnPagedArgs a;
-    int rc = check_attention(call, ctx, kv, batch, n_head, &a.kv, &a.b);
-    if (rc) return rc;
-    const uint32_t rows = batch->n_rows, hd = kv->head_dim;
-    rc = check_heads(call, "q", q, rows, n_head, hd);
-    if (!rc) rc = check_heads(call, "out", out, rows, n_head, hd);
-    if (!rc && gate) rc = check_heads(call, "gate", gate, rows, n_head, hd);
-    if (rc) return rc;
-    AQ_REQUIRE(q->type == AQ_TYPE_F32 || q->type == kv->type, "aq_paged_attention: rows are F32 or of the cache's type");
-    AQ_REQUIRE(out->type == q->type && (!gate || gate->type == q->type),
-               "aq_paged_attention: q, gate and out of different types");
-    auto apart = [&](const aq_heads *x) { // each output where its own input is, or in memory of its own
-        return out->data != x->data || ((rows <= 1 || out->row_stride == x->row_stride) &&
-                                        (n_head <= 1 || out->head_stride == x->head_stride));
-    };
-    AQ_REQUIRE(apart(q) && (!gate || apart(gate)), "aq_paged_attention: in place needs the same strides");
-    AQ_REQUIRE(std::isfinite(scale) && scale > 0.0f, "aq_paged_attention: scale");
-    if (rows == 0 || batch->n_seq == 0 || batch->max_rows == 0) return 0;
-    Choice c;
-    rc = choose(call, kv, batch, n_head, q->type == AQ_TYPE_F32, ctx->device, &c);
-    if (rc) return rc;
-    AQ_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0, "aq_paged_attention: workspace is null or not 16-byte aligned");
-    AQ_REQUIRE(workspace_bytes >= c.space.bytes, "aq_paged_attention: workspace of " + std::to_string(workspace_bytes) +
-                                                     " bytes, " + std::to_string(c.space.bytes) + " needed");
-    a.q = heads_view(q);
-    a.out = heads_view(out);
-    if (gate) a.gate = heads_view(gate);
-    a.n_head = (int)n_head;
-    a.G = (int)(n_head / kv->n_head_kv);
-    a.by_g = FastDiv((uint32_t)a.G);
-    a.window = window;
-    a.cap = c.cap;
-    a.scale_log2 = scale * 1.44269504088896340736f;
-    a.q_wide = heads_aligned(q, rows, n_head);
-    a.out_wide = heads_aligned(out, rows, n_head) && (!gate || heads_aligned(gate, rows, n_head));
-    a.shares = c.shares;
-    a.min_chunk = c.min_chunk;
-    a.lead = c.lead;
-    a.whole = c.whole;
-    a.n_seg = c.n_seg;
-    a.planned = c.planned;
-    char *ws = (char *)workspace;
-    a.plan = (uint32_t *)(ws + c.space.plan);
-    a.tiles = (RowTile *)(ws + c.space.seg);
-    a.part_o = (float *)(ws + c.space.o);
-    a.part_ml = (float *)(ws + c.space.ml);
-    AQ_HIP(hipSetDevice(ctx->device));
-    const hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
-    if (c.planned) {
-        rc = launch_paged_plan(a, c.R, c.unit, st);
-        if (rc) return rc;
-    }
-    if (c.many) {
-        rc = launch_paged_chunk(a, c.D, st);
-    } else if (kv->type == AQ_TYPE_F32) {
-        rc = launch_paged_few_f32(a, c.D, c.R, st);
-    } else if (kv->type == AQ_TYPE_F16) {
-        rc = launch_paged_few_f16(a, c.D, c.R, st);
-    } else {
-        rc = launch_paged_few_bf16(a, c.D, c.R, st);
-    }
-    if (rc || !c.join) return rc;
-    return launch_paged_combine(a, c.R, c.D, (int)std::min<uint64_t>((uint64_t)c.R, (uint64_t)batch->max_rows * a.G), st);
+    return attend("aq_paged_attention", ctx, kv, batch, nullptr, 0, n_head, q, out, scale, window, gate, workspace,
+                  workspace_bytes, stream);
+}
+
+int aq_paged_tree_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, const uint32_t *mask_dev,
+                            uint32_t mask_words, uint32_t n_head, const aq_heads *q, const aq_heads *out, float scale,
+                            uint32_t window, const aq_heads *gate, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *call = "aq_paged_tree_attention";
+    AQ_REQUIRE(ctx && kv && batch, "aq_paged_tree_attention: null argument");
+    AQ_REQUIRE(mask_words < (1u << 20) && (uint64_t)mask_words * 32 >= batch->max_rows,
+               "aq_paged_tree_attention: mask of " + std::to_string(mask_words) + " words for " +
+                   std::to_string(batch->max_rows) + " rows");
+    AQ_REQUIRE(batch->max_rows == 0 || mask_dev, "aq_paged_tree_attention: null mask_dev");
+    AQ_REQUIRE((uintptr_t)mask_dev % 4 == 0, "aq_paged_tree_attention: mask_dev is not aligned to its type");
+    return attend(call, ctx, kv, batch, mask_dev, mask_words, n_head, q, out, scale, window, gate, workspace,
+                  workspace_bytes, stream);
 }
 
 } // extern "C"

@@ -1,5 +1,5 @@
 // paged_attn.h — what the two paged attention kernels (paged_few.h: few rows, pages streamed through registers;
-// paged_chunk.hip: many rows, tiles in the LDS) share: the division of the work, the partial results, the outputs.
+// paged_chunk.h: many rows, tiles in the LDS) share: the division of the work, the partial results, the outputs.
 //
 // Rows. The G = n_head / n_head_kv query heads that share a K/V head, times a sequence's new tokens, are its rows over
 // that head's keys: row = token * G + head in the group. A segment is one row tile (R rows) of one sequence on one K/V
@@ -32,6 +32,8 @@ struct AttnPagedArgs {
     int n_head, G;
     FastDiv by_g; // rows to tokens
     uint32_t window; // 0: all
+    const uint32_t *mask; // of each row the new rows of its sequence that it sees (TREE)
+    uint32_t mask_words;
     uint32_t cap;    // positions from here on are not attended: the table's reach, or max_len
     float scale_log2;          // scale * log2(e)
     uint32_t q_wide, out_wide; // 16-byte loads of q; 4-value stores of out and loads of gate
@@ -49,14 +51,16 @@ constexpr uint32_t PLAN_HEAD = 4;
 
 // The units of a row tile: rows r0 .. r0 + R - 1 of a sequence of `sr.n` rows; first unit and one past the last. A tile
 // whose rows see nothing has one unit all the same: the one that writes its zeros.
+// TREE: all rows reach to the sequence's end, and with a window at least as far back as a row that sees no new row.
 struct UnitRange {
     uint32_t lo, hi;
 };
+template <bool TREE>
 __device__ __forceinline__ UnitRange tile_units(const AttnPagedArgs &a, const SeqRows &sr, int32_t r0, int32_t R, uint32_t tk) {
     const int32_t last = min(r0 + R, sr.n * a.G) - 1;
     const int32_t t0 = (int32_t)a.by_g.quot(r0), t1 = (int32_t)a.by_g.quot(last), base = sr.base; // row tokens' positions are base + token
-    const int32_t end = min(max(base + t1 + 1, 0), (int32_t)a.cap);
-    const int64_t begin = a.window ? max((int64_t)base + t0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
+    const int32_t end = min(TREE ? sr.len : max(base + t1 + 1, 0), (int32_t)a.cap);
+    const int64_t begin = a.window ? max((int64_t)base + (TREE ? 0 : t0 + 1) - (int64_t)a.window, (int64_t)0) : 0;
     UnitRange u;
     u.lo = (uint32_t)begin / tk;
     u.hi = ((uint32_t)end + tk - 1) / tk;
@@ -70,6 +74,28 @@ __device__ __forceinline__ uint32_t share_chunk(uint32_t total, uint32_t shares,
 }
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Trees (TREE): a row sees what stands before its sequence's new rows, from `lo` on, and the new rows that its mask names. Of
+// the 32 positions from kb on, those that row `row` of the row tensors sees, but for lo and for positions without a page;
+// base: the first new row's position.
+__device__ __forceinline__ uint32_t tree_bits(const AttnPagedArgs &a, int32_t row, int32_t base, int32_t kb) {
+    const int32_t rel = kb - base; // uniform
+    if (rel <= -32) return ~0u;
+    if (row < 0) return 0u;
+    const uint32_t *m = a.mask + (size_t)row * a.mask_words;
+    if (rel < 0) return m[0] << -rel | ((1u << -rel) - 1);
+    const uint32_t w = (uint32_t)rel / 32;
+    const uint64_t two = (w < a.mask_words ? m[w] : 0u) | (uint64_t)(w + 1 < a.mask_words ? m[w + 1] : 0u) << 32;
+    return (uint32_t)(two >> (rel % 32));
+}
+// The first position that a row sees before the new rows: with a window, as many places back as that leaves beside the n new
+// rows it sees.
+__device__ __forceinline__ int32_t tree_lo(const AttnPagedArgs &a, int32_t row, int32_t base) {
+    if (!a.window || row < 0) return 0;
+    int64_t own = base;
+    for (uint32_t w = 0; w < a.mask_words; w++) own += __popc(a.mask[(size_t)row * a.mask_words + w]);
+    return (int32_t)max(min(own - (int64_t)a.window, (int64_t)base), (int64_t)0);
+}
 
 // x, of which the compiler knows nothing more: what is computed from it stays where it is used, instead of waiting in a
 // register from before a loop.
@@ -141,12 +167,14 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t *wsum) {
 __device__ __forceinline__ uint32_t seq_tiles(const AttnPagedArgs &a, uint32_t s, int R) {
     return s < a.b.n_seq ? (uint32_t)((paged_seq(a.b, s).n * a.G + R - 1) / R) : 0u;
 }
+template <bool TREE>
 __device__ __forceinline__ uint32_t tile_count(const AttnPagedArgs &a, uint32_t s, uint32_t rt, int R, uint32_t tk) {
     if (a.whole) return a.whole;
-    const UnitRange u = tile_units(a, paged_seq(a.b, s), (int32_t)rt * R, R, tk);
+    const UnitRange u = tile_units<TREE>(a, paged_seq(a.b, s), (int32_t)rt * R, R, tk);
     return u.hi - u.lo + a.lead;
 }
 
+template <bool TREE>
 __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint32_t tk, PlanLds &lds) {
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t nkv = (uint32_t)a.kv.nkv;
@@ -176,7 +204,7 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
             uint32_t units = 0;
             if ((uint32_t)lane < n_seg) {
                 const uint32_t s = lds.seq[lane];
-                units = tile_count(a, s, lane - lds.first[s], R, tk);
+                units = tile_count<TREE>(a, s, lane - lds.first[s], R, tk);
             }
             const uint32_t sum = wave_scan(units, (int)n_seg);
             if (lane == 0) lds.pre[0] = 0;
@@ -203,7 +231,7 @@ __device__ __forceinline__ Share take_share(const AttnPagedArgs &a, int R, uint3
             for (int i = 0; i < PER; i++) {
                 const uint32_t j = tid * PER + i;
                 mine[i] = 0;
-                if (j < n_seg) mine[i] = tile_count(a, lds.seq[j], j - lds.first[lds.seq[j]], R, tk);
+                if (j < n_seg) mine[i] = tile_count<TREE>(a, lds.seq[j], j - lds.first[lds.seq[j]], R, tk);
                 sum += mine[i];
             }
             at = group_scan(sum, lds.wsum) - sum;
@@ -265,6 +293,7 @@ struct Segment {
     uint32_t kvh, seq, cnt;
     int32_t t0, t1, r0;
 };
+template <bool TREE>
 __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, uint32_t tk, const PlanLds &lds, const Share &sh,
                                                 uint32_t &u, uint32_t &j, uint32_t &kvh) {
     const uint32_t nkv = (uint32_t)a.kv.nkv;
@@ -303,7 +332,7 @@ __device__ __forceinline__ Segment next_segment(const AttnPagedArgs &a, int R, u
     s.seq = same(t.seq);
     s.r0 = (int32_t)t.rt * R;
     if (tk && a.whole) {
-        const UnitRange range = tile_units(a, paged_seq(a.b, s.seq), s.r0, R, tk);
+        const UnitRange range = tile_units<TREE>(a, paged_seq(a.b, s.seq), s.r0, R, tk);
         s.t0 = 0;
         s.t1 = (int32_t)(s.cnt = range.hi - range.lo);
     }
@@ -396,12 +425,17 @@ inline PagedSpace paged_space(size_t shares, size_t n_seg, size_t R, size_t D) {
     return s;
 }
 
-int launch_paged_plan(const AttnPagedArgs &a, int R, uint32_t tk, hipStream_t stream);
+int launch_paged_plan(const AttnPagedArgs &a, bool tree, int R, uint32_t tk, hipStream_t stream);
 // The few-row kernel (paged_few.h): a cache of this type, rows of its type or f32; D the padded head size, R 16 or 32 rows.
 int launch_paged_few_f32(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
 int launch_paged_few_f16(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
 int launch_paged_few_bf16(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
 int launch_paged_chunk(const AttnPagedArgs &a, int D, hipStream_t stream); // 16-bit rows and cache
+// The same with TREE.
+int launch_tree_few_f32(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
+int launch_tree_few_f16(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
+int launch_tree_few_bf16(const AttnPagedArgs &a, int D, int R, hipStream_t stream);
+int launch_tree_chunk(const AttnPagedArgs &a, int D, hipStream_t stream);
 int launch_paged_combine(const AttnPagedArgs &a, int R, int D, int rows, hipStream_t stream);
 
 constexpr int WAVES = 4;
@@ -413,7 +447,7 @@ constexpr int few_tile(int D) { return D == 256 ? 16 : 32; }
 constexpr int few_groups(int CT, int D, int R) { return R == 32 && (D == 256 || (CT == AQ_TYPE_F32 && D == 128)) ? 2 : 1; }
 constexpr int few_unit(int CT, int D, int R) { return WAVES / few_groups(CT, D, R) * few_tile(D); }
 
-constexpr int CHUNK_ROWS = 128;                                   // paged_chunk.hip's row tile
+constexpr int CHUNK_ROWS = 128;                                   // paged_chunk.h's row tile
 constexpr int chunk_keys(int D) { return D == 256 ? 32 : 64; } // and its unit
 
 } // namespace aq

@@ -1,5 +1,5 @@
 // paged_few.h — attention of few rows over a paged cache (paged_attn.h): single tokens, verify batches, and f32 rows of any
-// number. Instantiated per cache type in paged_few_*.hip.
+// number. Instantiated per cache type in paged_few_*.hip, for trees in tree_few_*.hip.
 //
 // The kernel for few rows. Single tokens are bound by reading the cache: a wave takes 32 positions at a time straight
 // from the pages into registers, in the matrix cores' operand layout, with no LDS on the way:
@@ -106,8 +106,8 @@ struct FewShape {
     static constexpr int LDS = (QF > CB ? QF : CB) + KW * R * 8;
 };
 
-// EXACT: the head fills D, so that a row's loads differ by constants only.
-template <int CT, bool FQ, int D, int R, bool EXACT>
+// EXACT: the head fills D, so that a row's loads differ by constants only. TREE: the new rows by their masks.
+template <int CT, bool FQ, int D, int R, bool EXACT, bool TREE>
 __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
     using S = FewShape<CT, FQ, D, R>;
     constexpr bool F = S::F;
@@ -127,22 +127,23 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
     const int r = lane & 15, g = lane >> 4, rg = wave % RG, kg = wave / RG; // which rows, which positions
     const int hd = EXACT ? D : a.kv.hd, G = a.G;
 
-    const Share sh = take_share(a, R, UNIT, plan);
+    const Share sh = take_share<TREE>(a, R, UNIT, plan);
     uint32_t u = sh.begin, j = sh.j, kv_at = sh.kvh;
     while (u < sh.end) { // uniform
-        const Segment sg = next_segment(a, R, UNIT, plan, sh, u, j, kv_at);
+        const Segment sg = next_segment<TREE>(a, R, UNIT, plan, sh, u, j, kv_at);
         if (sg.t1 <= sg.t0) continue;
         const uint32_t kvh = sg.kvh;
         const int32_t r0 = sg.r0;
         const SeqRows sr = paged_seq(a.b, sg.seq);
         const int32_t n_rows = sr.n * G, base = sr.base;
-        const UnitRange range = tile_units(a, sr, r0, R, UNIT);
+        const UnitRange range = tile_units<TREE>(a, sr, r0, R, UNIT);
         const int32_t tok0 = (int32_t)a.by_g.quot(r0), tok1 = (int32_t)a.by_g.quot(min(r0 + R, n_rows) - 1);
-        const int32_t kend = min(max(base + tok1 + 1, 0), (int32_t)a.cap);
+        const int32_t kend = min(TREE ? sr.len : max(base + tok1 + 1, 0), (int32_t)a.cap);
         // before this position nobody of the tile looks: there is no page there, whatever it holds
-        const int32_t kbegin = a.window ? (int32_t)max((int64_t)base + tok0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
-        const int32_t min_hi = base + tok0 + 1;
-        const int64_t max_lo = a.window ? (int64_t)base + tok1 + 1 - (int64_t)a.window : INT64_MIN;
+        const int32_t kbegin = a.window ? (int32_t)max((int64_t)base + (TREE ? 0 : tok0 + 1) - (int64_t)a.window, (int64_t)0) : 0;
+        const int32_t min_hi = TREE ? base : base + tok0 + 1;
+        const int64_t max_lo =
+            a.window ? (int64_t)base + (TREE ? (int64_t)a.mask_words * 32 : tok1 + 1) - (int64_t)a.window : INT64_MIN;
         const int32_t *table = a.b.pages + (size_t)sg.seq * a.b.max_pages;
         const uint64_t head_off = (uint64_t)kvh * a.kv.head_bytes;
         const char *const kpool = a.kv.k + head_off, *const vpool = a.kv.v + head_off;
@@ -191,14 +192,20 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             next = entry(tile + KW);
         }
 
-        // this lane's rows: the positions they see are lo .. hi - 1
+        // this lane's rows: the positions they see are lo .. hi - 1 (TREE: hi is the row of the mask, -1: none)
         int32_t hi[NR], lo[NR];
+        uint32_t bits[NR]; // TREE: of a tile's positions those that the row sees
 #pragma unroll
         for (int nr = 0; nr < NR; nr++) {
             const int32_t rr = r0 + 16 * (rg * NR + nr) + r, tok = (int32_t)a.by_g.quot(rr);
-            hi[nr] = rr < n_rows ? base + tok + 1 : 0;
-            const int64_t l = a.window ? (int64_t)base + tok + 1 - (int64_t)a.window : 0;
-            lo[nr] = l > 0 ? (int32_t)l : 0;
+            if constexpr (TREE) {
+                hi[nr] = rr < n_rows ? sr.first + tok : -1;
+                lo[nr] = tree_lo(a, hi[nr], base);
+            } else {
+                hi[nr] = rr < n_rows ? base + tok + 1 : 0;
+                const int64_t l = a.window ? (int64_t)base + tok + 1 - (int64_t)a.window : 0;
+                lo[nr] = l > 0 ? (int32_t)l : 0;
+            }
         }
 
         __syncthreads(); // the LDS of the segment before is read
@@ -280,8 +287,8 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             for (int e = 0; e < E; e++) x[e] *= rscale[nr];
             if (edge) {
                 const int gh = here(4 * g);
-                const int hr = hi[nr] - kb - gh, lr = lo[nr] - kb - gh; // of the lane's first position
-                const uint32_t mine = ok >> gh;
+                const int hr = TREE ? TILE : hi[nr] - kb - gh, lr = lo[nr] - kb - gh; // of the lane's first position
+                const uint32_t mine = (TREE ? ok & bits[nr] : ok) >> gh;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     const int pos = 16 * (e / 4) + e % 4;
@@ -314,6 +321,13 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             const int32_t kb = tile * TILE;
             const uint32_t now = units, ok = okm;
             const bool edge = kb + TILE > min_hi || (int64_t)kb < max_lo || ok != ALL; // uniform
+            if constexpr (TREE) {
+#pragma unroll
+                for (int nr = 0; nr < NR; nr++) bits[nr] = tree_bits(a, hi[nr], base, kb);
+            }
+            auto sees = [&](int nr, int pos) { // whether row nr sees the tile's position
+                return (TREE ? (bits[nr] >> pos) & 1 : kb + pos < hi[nr]) && kb + pos >= lo[nr];
+            };
             f4 s[NR][HT];
 #pragma unroll
             for (int nr = 0; nr < NR; nr++)
@@ -395,7 +409,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                             t[h] = __builtin_amdgcn_perm(v[c][2 * h + 1][jj / 2], v[c][2 * h][jj / 2], sel);
                         return t;
                     };
-                    if ((edge && tok0 < tok1) || NP > 1) { // one token's rows all see what has a page
+                    if ((edge && (TREE || tok0 < tok1)) || NP > 1) { // one token's rows all see what has a page
                         // Nor are infinities and NaN of positions that only some of the rows see, and an infinity times
                         // the pieces of one number is a NaN: such values are added position by position, to the rows
                         // that see them, by the probability's first piece, and taken out of the product of the others.
@@ -416,7 +430,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                                 if (pos % 16 / 4 == g) only[e / 2] = e & 1 ? 0xFFFF0000u : 0x0000FFFFu;
 #pragma unroll
                                 for (int nr = 0; nr < NR; nr++) {
-                                    const bool sees = kb + pos < hi[nr] && kb + pos >= lo[nr];
+                                    const bool seen = sees(nr, pos);
 #pragma unroll
                                     for (int jj = 0; jj < VB; jj++) {
                                         VP vt = product(jj) & only;
@@ -425,7 +439,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                                         const f4 t = mfma_pv<CT>(vt, pf[nr][0], o[nr][c * VB + jj]);
 #pragma unroll
                                         for (int x = 0; x < 4; x++)
-                                            o[nr][c * VB + jj][x] = sees ? t[x] : o[nr][c * VB + jj][x];
+                                            o[nr][c * VB + jj][x] = seen ? t[x] : o[nr][c * VB + jj][x];
                                     }
                                 }
                             }
@@ -499,14 +513,13 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                                     is_odd |= odd_f32(v[c][(4 * t + i) % VI][y]);
                                 }
                             const uint64_t b = __ballot(is_odd);
-                            if (b && tok0 < tok1) {
+                            if (b && (TREE || tok0 < tok1)) {
 #pragma unroll 1
                                 for (int gg = 0; gg < 4; gg++) {
                                     if (!((b >> (16 * gg)) & 0xFFFFu)) continue; // uniform
-                                    const int pos = kb + pos0 + 4 * gg;
 #pragma unroll
                                     for (int nr = 0; nr < NR; nr++) {
-                                        const bool sees = pos < hi[nr] && pos >= lo[nr];
+                                        const bool seen = sees(nr, pos0 + 4 * gg);
 #pragma unroll
                                         for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
@@ -515,7 +528,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
                                                                  __float_as_uint(x[nr][4 * t + i]), o[nr][c * 4 + y]);
 #pragma unroll
                                                 for (int z = 0; z < 4; z++)
-                                                    o[nr][c * 4 + y][z] = sees ? n[z] : o[nr][c * 4 + y][z];
+                                                    o[nr][c * 4 + y][z] = seen ? n[z] : o[nr][c * 4 + y][z];
                                             }
                                     }
                                 }
@@ -636,25 +649,26 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
     }
 }
 
-template <int CT, bool FQ, int D, int R, bool EXACT>
+template <int CT, bool FQ, int D, int R, bool EXACT, bool TREE>
 int few_launch(const AttnPagedArgs &a, hipStream_t stream) {
     using S = FewShape<CT, FQ, D, R>;
-    const auto kernel = few_rows_kernel<CT, FQ, D, R, EXACT>;
+    const auto kernel = few_rows_kernel<CT, FQ, D, R, EXACT, TREE>;
     static_assert(S::LDS + sizeof(PlanLds) + R * 4 <= 64 * 1024, "more LDS than a launch has without asking for it");
     kernel<<<a.shares, 256, S::LDS, stream>>>(a);
     AQ_HIP(hipGetLastError());
     return 0;
 }
-template <int CT, bool FQ, int D>
+template <int CT, bool FQ, int D, bool TREE>
 int few_rows(const AttnPagedArgs &a, int R, hipStream_t stream) {
-    if (a.kv.hd == D) return R == 16 ? few_launch<CT, FQ, D, 16, true>(a, stream) : few_launch<CT, FQ, D, 32, true>(a, stream);
-    return R == 16 ? few_launch<CT, FQ, D, 16, false>(a, stream) : few_launch<CT, FQ, D, 32, false>(a, stream);
+    if (a.kv.hd == D)
+        return R == 16 ? few_launch<CT, FQ, D, 16, true, TREE>(a, stream) : few_launch<CT, FQ, D, 32, true, TREE>(a, stream);
+    return R == 16 ? few_launch<CT, FQ, D, 16, false, TREE>(a, stream) : few_launch<CT, FQ, D, 32, false, TREE>(a, stream);
 }
-template <int CT, bool FQ>
+template <int CT, bool FQ, bool TREE>
 int few_pick(const AttnPagedArgs &a, int D, int R, hipStream_t stream) {
-    if (D == 64) return few_rows<CT, FQ, 64>(a, R, stream);
-    if (D == 128) return few_rows<CT, FQ, 128>(a, R, stream);
-    return few_rows<CT, FQ, 256>(a, R, stream);
+    if (D == 64) return few_rows<CT, FQ, 64, TREE>(a, R, stream);
+    if (D == 128) return few_rows<CT, FQ, 128, TREE>(a, R, stream);
+    return few_rows<CT, FQ, 256, TREE>(a, R, stream);
 }
 
 } // namespace

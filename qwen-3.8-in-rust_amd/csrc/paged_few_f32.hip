@@ -4,7 +4,7 @@
 namespace aq {
 
 int launch_paged_few_f32(const AttnPagedArgs &a, int D, int R, hipStream_t stream) {
-    return few_pick<AQ_TYPE_F32, true>(a, D, R, stream);
+    return few_pick<AQ_TYPE_F32, true, false>(a, D, R, stream);
 }
 
 } // namespace aq

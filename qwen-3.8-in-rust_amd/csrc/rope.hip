@@ -13,14 +13,7 @@
 #include <memory>
 #include <new>
 
-#include "paged.h"
-
-struct aq_rope {
-    aq_ctx *ctx = nullptr;
-    uint32_t dim = 0, layout = 0;
-    float gain = 1.0f;
-    double *freq = nullptr; // dim / 2 turns per position
-};
+#include "rope.h"
 
 namespace aq {
 
@@ -100,44 +93,6 @@ int check_paged(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b
 
 namespace {
 
-// N values at p as f32, and back with one rounding; 16 bytes at a time where W.
-template <int T, int N, bool W>
-__device__ __forceinline__ void load_n(const typename RowType<T>::type *p, float *v) {
-    using E = typename RowType<T>::type;
-    if constexpr (W) {
-        constexpr int C = 16 / (int)sizeof(E);
-        typedef E vec __attribute__((ext_vector_type(C)));
-#pragma unroll
-        for (int i = 0; i < N / C; i++) {
-            const vec x = *reinterpret_cast<const vec *>(p + i * C);
-#pragma unroll
-            for (int j = 0; j < C; j++) v[i * C + j] = (float)x[j];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = (float)p[i];
-    }
-}
-
-template <int T, int N, bool W>
-__device__ __forceinline__ void store_n(typename RowType<T>::type *p, const float *v) {
-    using E = typename RowType<T>::type;
-    if constexpr (W) {
-        constexpr int C = 16 / (int)sizeof(E);
-        typedef E vec __attribute__((ext_vector_type(C)));
-#pragma unroll
-        for (int i = 0; i < N / C; i++) {
-            vec x;
-#pragma unroll
-            for (int j = 0; j < C; j++) x[j] = (E)v[i * C + j];
-            *reinterpret_cast<vec *>(p + i * C) = x;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) p[i] = (E)v[i];
-    }
-}
-
 // The rotation of one unit: half layout VEC pairs (values u..u+VEC-1 with those dim/2 further), interleaved VEC / 2
 // pairs of neighbours.
 template <bool INTER, int VEC>
@@ -148,9 +103,8 @@ struct Unit {
     __device__ __forceinline__ void angles(const double *freq, uint32_t unit, int32_t pos, float gain, float sign) {
 #pragma unroll
         for (int i = 0; i < PAIRS; i++) {
-            const double t = (double)pos * freq[unit * PAIRS + i];
             float sn, cs;
-            sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
+            rope_angle(freq[unit * PAIRS + i], pos, &sn, &cs);
             c[i] = cs * gain;
             s[i] = sn * gain * sign;
         }
@@ -269,15 +223,6 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
                                       (int64_t)(a.kv.head_bytes / sizeof(EO)), h0,
                                       min(h0 + (int)a.heads_per, a.kv.nkv), rot, unit, isv ? 0u : a.dim,
                                       isv ? 0u : a.rot_units, u);
-}
-
-// How a head divides into units: `vec` values each (half layout: of either half), then the values that pass through.
-void unit_shape(uint32_t layout, uint32_t dim, uint32_t hd, uint32_t vec, uint32_t *rot, uint32_t *all) {
-    *rot = layout == AQ_ROPE_INTERLEAVED ? dim / vec : dim / 2 / vec;
-    *all = *rot + (hd - dim) / vec;
-}
-bool wide_fits(uint32_t layout, uint32_t dim, uint32_t hd, uint32_t vec) {
-    return hd % vec == 0 && dim % vec == 0 && (layout == AQ_ROPE_INTERLEAVED || (dim / 2) % vec == 0);
 }
 
 template <int T, bool INTER, bool W>
