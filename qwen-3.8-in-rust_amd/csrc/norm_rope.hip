@@ -2,18 +2,27 @@
 // (aq_qk_norm_rope) and on the way into the pages (aq_paged_append_norm).
 //
 // y = x / sqrt(mean(x^2) + eps) * weight over the head's values, in 32 bits, then its pairs turned as rope.hip turns them, and
-// one rounding at the store. A head's values lie on a group of lanes, one unit (rope.h) each, so that both values of a pair are
-// in one lane and the sum of squares is one exchange per doubling of the group. A row's angles are computed once for all of
-// its heads, one a thread, and handed over in the LDS; the first heads' values are on their way meanwhile.
+// one rounding at the store. A head's values lie on a group of lanes, one unit each, so that both values of a pair are in one
+// lane and the sum of squares is one exchange per doubling of the group. A wave has as many heads of one row as fit it,
+// computes the row's angles once, one a lane, and hands them over in the LDS: no work-group to wait for, and the values are
+// on their way meanwhile.
+//
+// Bound by their bytes, with about as many cycles of arithmetic: 8191 rows of 40 heads of 128 (bf16) 33.6 us, 5.0 TB/s, what a
+// large copy reaches; with the angles over a work-group behind a barrier 42.2, with work-groups that go on from row to row
+// 46.6 (too few waves); with a branch for every lane that has no unit or no pair 36.0. 6000 rows of 24 query and 4 K/V heads
+// of 256 (f32 into f16) appended in 61.9 us, 5.3 TB/s. Single tokens: an empty launch and three latencies.
 #include <cmath>
-#include <type_traits>
 
 #include "rope.h"
 
 namespace aq {
 namespace {
 
-constexpr int MAX_HEAD = 256, MAX_THREADS = 512;
+constexpr int MAX_HEAD = 256;
+// Heads of a lane, so that it has 32 bytes to load. One and two heads: 8191 rows of 40 heads of 128 (bf16), 32 bytes of each
+// (half layout) 33.6 and 39.8 us, 16 (neighbours) 38.0 and 35.3; 6000 rows of 32 heads of 256 (f32 into f16), 32 bytes,
+// 61.9 and 66.5.
+constexpr uint32_t heads_per_lane(uint32_t bytes) { return bytes < 32 ? 2 : 1; }
 
 struct NormArgs {
     PagedKv kv;
@@ -22,156 +31,191 @@ struct NormArgs {
     const float *qw, *kw;
     const double *freq;
     const int32_t *pos; // of each row; null: its place in its sequence
-    uint32_t n_rows, dim, rot_units, units, lane_shift;
+    uint32_t n_rows, dim, rot_units, pass_units, pass_seconds, units, lane_shift;
     uint32_t nq, nqk, jobs; // heads of a row: queries, keys after them, values after those
+    uint32_t parts;         // waves of a row
+    FastDiv by_parts;
     float eps, inv_hd, gain;
 };
 
-// One row per blockIdx.x, its heads over blockIdx.y and the threads' groups of 2^lane_shift lanes, two at a time. NU: units a
-// lane has at most (one where 16 bytes are moved at a time).
+// A unit's N values as they are stored.
+template <int T, int N>
+struct Raw {
+    using E = typename RowType<T>::type;
+    typedef E vec __attribute__((ext_vector_type(N)));
+    vec x;
+};
+// V values at p: into x[at ..], and back from v, at most 16 bytes at a time where W.
+template <int V, bool W, typename E, typename VEC>
+__device__ __forceinline__ void load_raw(const E *p, VEC &x, int at) {
+    constexpr int C = !W ? 1 : V * (int)sizeof(E) > 16 ? 16 / (int)sizeof(E) : V;
+    typedef E vec __attribute__((ext_vector_type(C)));
+#pragma unroll
+    for (int i = 0; i < V / C; i++) {
+        const vec y = *reinterpret_cast<const vec *>(p + i * C);
+#pragma unroll
+        for (int e = 0; e < C; e++) x[at + i * C + e] = y[e];
+    }
+}
+template <int V, bool W, typename E>
+__device__ __forceinline__ void store_raw(E *p, const float *v) {
+    constexpr int C = !W ? 1 : V * (int)sizeof(E) > 16 ? 16 / (int)sizeof(E) : V;
+    typedef E vec __attribute__((ext_vector_type(C)));
+#pragma unroll
+    for (int i = 0; i < V / C; i++) {
+        vec y;
+#pragma unroll
+        for (int e = 0; e < C; e++) y[e] = (E)v[i * C + e];
+        *reinterpret_cast<vec *>(p + i * C) = y;
+    }
+}
+
+// One wave has one row's heads `part * HB * heads a wave` and on, of `parts` waves a row; a head lies on 2^lane_shift lanes,
+// and a wave takes HB times as many heads as fit it. NU: units a lane has at most (one where 16 bytes are moved at a time).
+// A unit: VEC values of either half of what is turned (half layout), of either half of what passes through, or VEC neighbours.
+// Little of it branches: a lane past the head's units has the first one's once more, a unit without second values its first
+// ones twice, a head past the last the last's, and only the stores are left out.
 template <int TI, int TO, bool INTER, int VEC, bool W, int NU, bool PAGED>
-__global__ void __launch_bounds__(MAX_THREADS) norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(256, 8) norm_kernel(NormArgs a) {
     using EI = typename RowType<TI>::type;
     using EO = typename RowType<TO>::type;
-    constexpr int N = INTER ? VEC : 2 * VEC, PAIRS = N / 2, HB = 2;
-    __shared__ float cosines[MAX_HEAD / 2], sines[MAX_HEAD / 2];
-    const uint32_t row = blockIdx.x, lanes = 1u << a.lane_shift;
+    constexpr int N = INTER ? VEC : 2 * VEC, PAIRS = N / 2;
+    constexpr uint32_t HB = heads_per_lane(N * sizeof(EI));
+    __shared__ __align__(16) float turns[4][2][MAX_HEAD / 2]; // each wave's cosines and sines
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lanes = 1u << a.lane_shift;
+    const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane((int)((blockIdx.y * gridDim.x + blockIdx.x) * 4 + wave));
+    const uint32_t row = a.by_parts.quot(id), part = id - row * a.parts;
+    if (row >= a.n_rows) return;
+
+    // Where each of this lane's units begins, its second values and its angles; whether it has them, and turns them.
+    uint32_t at[NU], two[NU], pair[NU];
+    bool have[NU], both[NU], rot[NU];
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+        const uint32_t u = (lane & (lanes - 1)) + ((uint32_t)i << a.lane_shift);
+        have[i] = u < a.units;
+        rot[i] = u < a.rot_units;
+        at[i] = rot[i] ? u * VEC : have[i] ? a.dim + (u - a.rot_units) * VEC : 0;
+        both[i] = !INTER && (rot[i] || (have[i] && u - a.rot_units < a.pass_seconds));
+        two[i] = at[i] + (both[i] ? (rot[i] ? a.dim / 2 : a.pass_units * VEC) : 0);
+        pair[i] = rot[i] ? (INTER ? at[i] / 2 : at[i]) : 0;
+    }
+    // A job: one head of the row's queries, keys or values.
+    const uint32_t per = 64u >> a.lane_shift, j0 = part * HB * per + (lane >> a.lane_shift);
+    Raw<TI, N> raw[HB][NU];
+#pragma unroll
+    for (int h = 0; h < (int)HB; h++) {
+        const uint32_t j = min(j0 + h * per, a.jobs - 1);
+        const bool q = j < a.nq, k = j < a.nqk;
+        const EI *p = (const EI *)(q ? a.q.p : k ? a.k.p : a.v.p) + row * (q ? a.q.row : k ? a.k.row : a.v.row) +
+                      (int64_t)(j - (q ? 0 : k ? a.nq : a.nqk)) * (q ? a.q.head : k ? a.k.head : a.v.head);
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            load_raw<VEC, W>(p + at[i], raw[h][i].x, 0);
+            if (!INTER) load_raw<VEC, W>(p + two[i], raw[h][i].x, N - VEC);
+        }
+    }
+
+    // Where the row is rotated and stored; a row of no sequence is left alone.
     int32_t pos = 0;
     bool store = true;
     uint32_t off = 0;
     if constexpr (PAGED) {
         const uint32_t seq = paged_seq_of(a.b, row);
-        if (seq >= a.b.n_seq) return; // uniform in the work-group, as all of this
+        if (seq >= a.b.n_seq) return; // uniform in the wave, as all of this
         const SeqRows sr = paged_seq(a.b, seq);
         if ((int32_t)row < sr.first) return; // before the first sequence's rows
         pos = sr.base + ((int32_t)row - sr.first);
         store = pos >= 0 && paged_slot(a.kv, a.b.pages + (size_t)seq * a.b.max_pages, a.b.max_pages, (uint32_t)pos, &off);
     }
     if (a.pos) pos = a.pos[row];
-
-    const uint32_t lane0 = threadIdx.x & (lanes - 1);
-    uint32_t at[NU]; // where each of this lane's units begins; bit i: it is there, it is turned
-    uint32_t have = 0, rot = 0;
-#pragma unroll
-    for (int i = 0; i < NU; i++) {
-        const uint32_t u = lane0 + ((uint32_t)i << a.lane_shift);
-        have |= u < a.units ? 1u << i : 0u;
-        rot |= u < a.rot_units ? 1u << i : 0u;
-        at[i] = u < a.rot_units ? u * VEC : a.dim + (u - a.rot_units) * VEC;
-    }
-    // A job: one head of the row's queries, keys or values.
-    float v[HB][NU][N];
-    auto source = [&](uint32_t j) {
-        const HeadsView &s = j < a.nq ? a.q : j < a.nqk ? a.k : a.v;
-        const uint32_t head = j < a.nq ? j : j < a.nqk ? j - a.nq : j - a.nqk;
-        return (const EI *)s.p + (int64_t)row * s.row + (int64_t)head * s.head;
-    };
-    auto fetch = [&](uint32_t j, float (*x)[N]) {
-        const EI *p = source(j);
-#pragma unroll
-        for (int i = 0; i < NU; i++) {
-            if (!((have >> i) & 1)) continue;
-            load_n<TI, VEC, W>(p + at[i], x[i]);
-            if (!INTER && ((rot >> i) & 1)) load_n<TI, VEC, W>(p + at[i] + a.dim / 2, x[i] + N - VEC);
-        }
-    };
-    const uint32_t group = (blockIdx.y * blockDim.x + threadIdx.x) >> a.lane_shift,
-                   groups = (gridDim.y * blockDim.x) >> a.lane_shift;
-#pragma unroll
-    for (int h = 0; h < HB; h++)
-        if (group + h * groups < a.jobs) fetch(group + h * groups, v[h]);
-
-    for (uint32_t i = threadIdx.x; i < a.dim / 2; i += blockDim.x) {
+    float *const cosines = turns[wave][0], *const sines = turns[wave][1];
+    for (uint32_t i = lane; i < a.dim / 2; i += 64) {
         float sn, cs;
         rope_angle(a.freq[i], pos, &sn, &cs);
         cosines[i] = cs * a.gain;
         sines[i] = sn * a.gain;
     }
-    __syncthreads();
-    float c[NU][PAIRS], s[NU][PAIRS];
-#pragma unroll
-    for (int i = 0; i < NU; i++)
-#pragma unroll
-        for (int e = 0; e < PAIRS; e++) {
-            const uint32_t pair = (rot >> i) & 1 ? (INTER ? at[i] / 2 : at[i]) + e : 0;
-            c[i][e] = cosines[pair];
-            s[i][e] = sines[pair];
-        }
+    __builtin_amdgcn_wave_barrier(); // written and read by one wave, in order
 
-    for (uint32_t j0 = group; j0 < a.jobs; j0 += HB * groups) {
-        if (j0 != group) {
 #pragma unroll
-            for (int h = 0; h < HB; h++)
-                if (j0 + h * groups < a.jobs) fetch(j0 + h * groups, v[h]);
+    for (int h = 0; h < (int)HB; h++) {
+        const uint32_t j = j0 + h * per;
+        const bool q = j < a.nq, k = j < a.nqk;
+        float v[NU][N];
+#pragma unroll
+        for (int i = 0; i < NU; i++)
+#pragma unroll
+            for (int e = 0; e < N; e++) v[i][e] = (float)raw[h][i].x[e];
+        if (!PAGED || k) { // values pass as they are
+            const float *w = q ? a.qw : a.kw;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NU; i++) {
+                float one = 0.0f, second = 0.0f;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) one = fmaf(v[i][e], v[i][e], one);
+                if (!INTER) {
+#pragma unroll
+                    for (int e = VEC; e < N; e++) second = fmaf(v[i][e], v[i][e], second);
+                }
+                sum += (have[i] ? one : 0.0f) + (both[i] ? second : 0.0f);
+            }
+            for (uint32_t d = 1; d < lanes; d *= 2) sum += __shfl_xor(sum, (int)d);
+            const float scale = rsqrtf(sum * a.inv_hd + a.eps);
+#pragma unroll
+            for (int i = 0; i < NU; i++) {
+                float x[N], c[PAIRS], s[PAIRS];
+                load_n<AQ_TYPE_F32, VEC, W>(w + at[i], x);
+                if (!INTER) load_n<AQ_TYPE_F32, VEC, W>(w + two[i], x + N - VEC);
+#pragma unroll
+                for (int e = 0; e < PAIRS; e++) {
+                    c[e] = cosines[pair[i] + e];
+                    s[e] = sines[pair[i] + e];
+                }
+#pragma unroll
+                for (int e = 0; e < N; e++) x[e] *= v[i][e] * scale;
+#pragma unroll
+                for (int e = 0; e < PAIRS; e++) {
+                    const int ia = INTER ? 2 * e : e, ib = INTER ? 2 * e + 1 : VEC + e;
+                    const float p = fmaf(x[ia], c[e], -(x[ib] * s[e])), r = fmaf(x[ib], c[e], x[ia] * s[e]);
+                    v[i][ia] = rot[i] ? p : x[ia];
+                    v[i][ib] = rot[i] ? r : x[ib];
+                }
+            }
         }
+        if (j >= a.jobs) continue;
+        auto put = [&](auto *to) {
 #pragma unroll
-        for (int h = 0; h < HB; h++) {
-            const uint32_t j = j0 + h * groups;
-            if (j >= a.jobs) continue;
-            if (j < a.nqk) {
-                const float *w = j < a.nq ? a.qw : a.kw;
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NU; i++) {
-                    if (!((have >> i) & 1)) continue;
-#pragma unroll
-                    for (int e = 0; e < N; e++)
-                        if (INTER || e < VEC || ((rot >> i) & 1)) sum = fmaf(v[h][i][e], v[h][i][e], sum);
-                }
-                for (uint32_t d = 1; d < lanes; d *= 2) sum += __shfl_xor(sum, (int)d);
-                const float scale = rsqrtf(sum * a.inv_hd + a.eps);
-#pragma unroll
-                for (int i = 0; i < NU; i++) {
-                    if (!((have >> i) & 1)) continue;
-                    const bool turned = (rot >> i) & 1;
-                    float x[N];
-                    load_n<AQ_TYPE_F32, VEC, W>(w + at[i], x);
-                    if (!INTER && turned) load_n<AQ_TYPE_F32, VEC, W>(w + at[i] + a.dim / 2, x + N - VEC);
-#pragma unroll
-                    for (int e = 0; e < N; e++)
-                        if (INTER || e < VEC || turned) x[e] = v[h][i][e] * scale * x[e];
-#pragma unroll
-                    for (int e = 0; e < PAIRS; e++) {
-                        const int ia = INTER ? 2 * e : e, ib = INTER ? 2 * e + 1 : VEC + e;
-                        const float p = x[ia], r = x[ib];
-                        v[h][i][ia] = turned ? fmaf(p, c[i][e], -(r * s[i][e])) : p;
-                        v[h][i][ib] = turned ? fmaf(r, c[i][e], p * s[i][e]) : r;
-                    }
-                }
+            for (int i = 0; i < NU; i++) {
+                if (have[i]) store_raw<VEC, W>(to + at[i], v[i]);
+                if (both[i]) store_raw<VEC, W>(to + two[i], v[i] + N - VEC);
             }
-            auto put = [&](auto *p, auto type) {
-                constexpr int T = decltype(type)::value;
-#pragma unroll
-                for (int i = 0; i < NU; i++) {
-                    if (!((have >> i) & 1)) continue;
-                    store_n<T, VEC, W>(p + at[i], v[h][i]);
-                    if (!INTER && ((rot >> i) & 1)) store_n<T, VEC, W>(p + at[i] + a.dim / 2, v[h][i] + N - VEC);
-                }
-            };
-            if (j < a.nq) {
-                put((EI *)a.qo.p + (int64_t)row * a.qo.row + (int64_t)j * a.qo.head, std::integral_constant<int, TI>());
-            } else if constexpr (PAGED) {
-                const bool key = j < a.nqk;
-                char *p = const_cast<char *>(key ? a.kv.k : a.kv.v) + ((uint64_t)off << a.kv.unit_shift) +
-                          (uint64_t)(key ? j - a.nq : j - a.nqk) * a.kv.head_bytes;
-                if (store) put((EO *)p, std::integral_constant<int, TO>());
-            } else {
-                put((EI *)a.ko.p + (int64_t)row * a.ko.row + (int64_t)(j - a.nq) * a.ko.head,
-                    std::integral_constant<int, TI>());
-            }
+        };
+        if (q) {
+            put((EI *)a.qo.p + row * a.qo.row + (int64_t)j * a.qo.head);
+        } else if constexpr (PAGED) {
+            char *to = const_cast<char *>(k ? a.kv.k : a.kv.v) + ((uint64_t)off << a.kv.unit_shift) +
+                       (uint64_t)(k ? j - a.nq : j - a.nqk) * a.kv.head_bytes;
+            if (store) put((EO *)to);
+        } else {
+            put((EI *)a.ko.p + row * a.ko.row + (int64_t)(j - a.nq) * a.ko.head);
         }
     }
 }
 
+// vec: values moved at a time, 0: one (two neighbours) after the other.
 template <int TI, int TO, bool PAGED>
-int norm_pick(const NormArgs &a, bool inter, bool wide, dim3 grid, uint32_t threads, hipStream_t stream) {
-    constexpr int VW = TI == AQ_TYPE_F32 && TO == AQ_TYPE_F32 ? 4 : 8;
+int norm_pick(const NormArgs &a, bool inter, uint32_t vec, dim3 grid, hipStream_t stream) {
+    constexpr int WIDE = TI == AQ_TYPE_F32 && TO == AQ_TYPE_F32 ? 4 : 8;
     if (inter) {
-        if (wide) norm_kernel<TI, TO, true, VW, true, 1, PAGED><<<grid, threads, 0, stream>>>(a);
-        else norm_kernel<TI, TO, true, 2, false, 2, PAGED><<<grid, threads, 0, stream>>>(a);
+        if (vec == WIDE) norm_kernel<TI, TO, true, WIDE, true, 1, PAGED><<<grid, 256, 0, stream>>>(a);
+        else if (vec) norm_kernel<TI, TO, true, 4, true, 1, PAGED><<<grid, 256, 0, stream>>>(a);
+        else norm_kernel<TI, TO, true, 2, false, 2, PAGED><<<grid, 256, 0, stream>>>(a);
     } else {
-        if (wide) norm_kernel<TI, TO, false, VW, true, 1, PAGED><<<grid, threads, 0, stream>>>(a);
-        else norm_kernel<TI, TO, false, 1, false, 4, PAGED><<<grid, threads, 0, stream>>>(a);
+        if (vec == WIDE) norm_kernel<TI, TO, false, WIDE, true, 1, PAGED><<<grid, 256, 0, stream>>>(a);
+        else if (vec) norm_kernel<TI, TO, false, 4, true, 1, PAGED><<<grid, 256, 0, stream>>>(a);
+        else norm_kernel<TI, TO, false, 1, false, 2, PAGED><<<grid, 256, 0, stream>>>(a);
     }
     AQ_HIP(hipGetLastError());
     return 0;
@@ -200,27 +244,37 @@ int check_in_place(const char *call, const aq_heads *x, const aq_heads *y) {
     return 0;
 }
 
-// The units, the lanes of a head, and the launch. `vec`: values moved at a time where `wide`.
-void shape(NormArgs &a, const aq_rope *rope, uint32_t hd, uint32_t vec, bool wide, float eps, dim3 *grid, uint32_t *threads) {
+// Values moved at a time: as many as 16 bytes of the rows or of the cache hold, or 4, where the units and all that is read and
+// written allow it (6000 rows of 32 heads of 80 of which 40 are turned, bf16: 4 a time 16.6 us, 1 a time 59.8).
+uint32_t values_at_once(const aq_rope *rope, uint32_t hd, bool f32, bool aligned) {
+    const uint32_t layout = rope ? rope->layout : (uint32_t)AQ_ROPE_HALF, dim = rope ? rope->dim : 0;
+    if (aligned && !f32 && wide_fits(layout, dim, hd, 8)) return 8;
+    return aligned && wide_fits(layout, dim, hd, 4) ? 4 : 0;
+}
+
+// The units, the lanes of a head, and the launch (row_bytes: of a value of the rows); false: more waves than a launch has.
+bool shape(NormArgs &a, const aq_rope *rope, uint32_t hd, uint32_t vec, uint32_t row_bytes, float eps, dim3 *grid) {
     const bool inter = rope && rope->layout == AQ_ROPE_INTERLEAVED;
     a.dim = rope ? rope->dim : 0;
     a.freq = rope ? rope->freq : nullptr;
     a.gain = rope ? rope->gain : 1.0f;
     a.eps = eps;
     a.inv_hd = 1.0f / (float)hd;
-    unit_shape(inter ? AQ_ROPE_INTERLEAVED : AQ_ROPE_HALF, a.dim, hd, wide ? vec : inter ? 2 : 1, &a.rot_units, &a.units);
+    const uint32_t v = vec ? vec : inter ? 2 : 1, pass = (hd - a.dim) / v;
+    a.rot_units = a.dim / v / (inter ? 1 : 2);
+    a.pass_units = inter ? pass : (pass + 1) / 2;
+    a.pass_seconds = pass - a.pass_units;
+    a.units = a.rot_units + a.pass_units;
     a.lane_shift = 0;
     while (a.lane_shift < 6 && (1u << a.lane_shift) < a.units) a.lane_shift++;
-    const uint32_t items = a.jobs << a.lane_shift; // lanes that a row needs at once
-    // Few rows: a work-group to each wave's heads; many: a row to a work-group, two heads a group of lanes.
-    uint32_t t = 64;
-    if ((uint64_t)a.n_rows * items > (1u << 18)) {
-        while (t < MAX_THREADS && t * 2 < items && (uint64_t)(t + 64) * a.n_rows < (1ull << 32)) t += 64;
-        *grid = dim3(a.n_rows);
-    } else {
-        *grid = dim3(a.n_rows, (items + t - 1) / t);
-    }
-    *threads = t;
+    const uint32_t per = heads_per_lane((inter ? v : 2 * v) * row_bytes) * (64u >> a.lane_shift);
+    a.parts = (a.jobs + per - 1) / per;
+    a.by_parts = FastDiv(a.parts);
+    const uint64_t waves = (uint64_t)a.parts * a.n_rows;
+    if (waves >= (1ull << 31) - (1u << 23)) return false;
+    const uint32_t groups = (uint32_t)((waves + 3) / 4), most = 1u << 20;
+    *grid = groups <= most ? dim3(groups) : dim3(most, (groups + most - 1) / most);
+    return true;
 }
 
 } // namespace
@@ -256,11 +310,11 @@ int aq_qk_norm_rope(aq_ctx *ctx, const aq_heads *q, const aq_heads *q_out, uint3
     if (n_rows == 0) return 0;
     const int type = q ? q->type : k->type;
     const bool inter = rope && rope->layout == AQ_ROPE_INTERLEAVED;
-    const uint32_t vec = 16 / (uint32_t)type_bytes(type);
-    const bool wide = (!q || (heads_aligned(q, n_rows, n_head) && heads_aligned(q_out, n_rows, n_head) && weight_aligned(q_weight))) &&
-                      (!k || (heads_aligned(k, n_rows, n_head_kv) && heads_aligned(k_out, n_rows, n_head_kv) && weight_aligned(k_weight))) &&
-                      wide_fits(inter ? AQ_ROPE_INTERLEAVED : AQ_ROPE_HALF, rope ? rope->dim : 0, head_dim, vec);
-    AQ_REQUIRE(wide || !inter || head_dim % 2 == 0, "aq_qk_norm_rope: head_dim is odd");
+    const bool aligned =
+        (!q || (heads_aligned(q, n_rows, n_head) && heads_aligned(q_out, n_rows, n_head) && weight_aligned(q_weight))) &&
+        (!k || (heads_aligned(k, n_rows, n_head_kv) && heads_aligned(k_out, n_rows, n_head_kv) && weight_aligned(k_weight)));
+    const uint32_t vec = values_at_once(rope, head_dim, type == AQ_TYPE_F32, aligned);
+    AQ_REQUIRE(vec || !inter || head_dim % 2 == 0, "aq_qk_norm_rope: head_dim is odd");
     NormArgs a = {};
     if (q) {
         a.q = heads_view(q);
@@ -277,14 +331,14 @@ int aq_qk_norm_rope(aq_ctx *ctx, const aq_heads *q, const aq_heads *q_out, uint3
     a.nq = q ? n_head : 0;
     a.jobs = a.nqk = a.nq + (k ? n_head_kv : 0);
     dim3 grid;
-    uint32_t threads;
-    shape(a, rope, head_dim, vec, wide, eps, &grid, &threads);
+    if (!shape(a, rope, head_dim, vec, (uint32_t)type_bytes(type), eps, &grid))
+        return fail(AQ_EUNSUP, "aq_qk_norm_rope: more than 2^31 pieces of rows");
     AQ_HIP(hipSetDevice(ctx->device));
     const hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
     switch (type) {
-    case AQ_TYPE_F32: return norm_pick<AQ_TYPE_F32, AQ_TYPE_F32, false>(a, inter, wide, grid, threads, st);
-    case AQ_TYPE_F16: return norm_pick<AQ_TYPE_F16, AQ_TYPE_F16, false>(a, inter, wide, grid, threads, st);
-    default: return norm_pick<AQ_TYPE_BF16, AQ_TYPE_BF16, false>(a, inter, wide, grid, threads, st);
+    case AQ_TYPE_F32: return norm_pick<AQ_TYPE_F32, AQ_TYPE_F32, false>(a, inter, vec, grid, st);
+    case AQ_TYPE_F16: return norm_pick<AQ_TYPE_F16, AQ_TYPE_F16, false>(a, inter, vec, grid, st);
+    default: return norm_pick<AQ_TYPE_BF16, AQ_TYPE_BF16, false>(a, inter, vec, grid, st);
     }
 }
 
@@ -317,10 +371,10 @@ int aq_paged_append_norm(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batc
     AQ_REQUIRE(rope || !pos_dev, "aq_paged_append_norm: positions without a rope");
     if (rows == 0 || batch->n_seq == 0) return 0;
     const bool inter = rope && rope->layout == AQ_ROPE_INTERLEAVED;
-    const uint32_t vec = k->type == AQ_TYPE_F32 && kv->type == AQ_TYPE_F32 ? 4 : 8;
-    const bool wide = heads_aligned(k, rows, kv->n_head_kv) && heads_aligned(v, rows, kv->n_head_kv) && weight_aligned(k_weight) &&
-                      (!q || (heads_aligned(q, rows, n_head) && heads_aligned(q_out, rows, n_head) && weight_aligned(q_weight))) &&
-                      wide_fits(inter ? AQ_ROPE_INTERLEAVED : AQ_ROPE_HALF, rope ? rope->dim : 0, hd, vec);
+    const bool aligned =
+        heads_aligned(k, rows, kv->n_head_kv) && heads_aligned(v, rows, kv->n_head_kv) && weight_aligned(k_weight) &&
+        (!q || (heads_aligned(q, rows, n_head) && heads_aligned(q_out, rows, n_head) && weight_aligned(q_weight)));
+    const uint32_t vec = values_at_once(rope, hd, kv->type == AQ_TYPE_F32, aligned);
     a.k = heads_view(k);
     a.v = heads_view(v);
     a.kw = k_weight;
@@ -335,17 +389,17 @@ int aq_paged_append_norm(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batc
     a.nqk = a.nq + kv->n_head_kv;
     a.jobs = a.nqk + kv->n_head_kv;
     dim3 grid;
-    uint32_t threads;
-    shape(a, rope, hd, vec, wide, eps, &grid, &threads);
+    if (!shape(a, rope, hd, vec, (uint32_t)type_bytes(k->type), eps, &grid))
+        return fail(AQ_EUNSUP, "aq_paged_append_norm: more than 2^31 pieces of rows");
     AQ_HIP(hipSetDevice(ctx->device));
     const hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
     if (k->type == AQ_TYPE_F32) {
-        if (kv->type == AQ_TYPE_F32) return norm_pick<AQ_TYPE_F32, AQ_TYPE_F32, true>(a, inter, wide, grid, threads, st);
-        if (kv->type == AQ_TYPE_F16) return norm_pick<AQ_TYPE_F32, AQ_TYPE_F16, true>(a, inter, wide, grid, threads, st);
-        return norm_pick<AQ_TYPE_F32, AQ_TYPE_BF16, true>(a, inter, wide, grid, threads, st);
+        if (kv->type == AQ_TYPE_F32) return norm_pick<AQ_TYPE_F32, AQ_TYPE_F32, true>(a, inter, vec, grid, st);
+        if (kv->type == AQ_TYPE_F16) return norm_pick<AQ_TYPE_F32, AQ_TYPE_F16, true>(a, inter, vec, grid, st);
+        return norm_pick<AQ_TYPE_F32, AQ_TYPE_BF16, true>(a, inter, vec, grid, st);
     }
-    if (kv->type == AQ_TYPE_F16) return norm_pick<AQ_TYPE_F16, AQ_TYPE_F16, true>(a, inter, wide, grid, threads, st);
-    return norm_pick<AQ_TYPE_BF16, AQ_TYPE_BF16, true>(a, inter, wide, grid, threads, st);
+    if (kv->type == AQ_TYPE_F16) return norm_pick<AQ_TYPE_F16, AQ_TYPE_F16, true>(a, inter, vec, grid, st);
+    return norm_pick<AQ_TYPE_BF16, AQ_TYPE_BF16, true>(a, inter, vec, grid, st);
 }
 
 } // extern "C"
