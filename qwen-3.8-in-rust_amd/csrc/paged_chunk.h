@@ -371,12 +371,24 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                     }
                     return x;
                 };
+                uint64_t odd = 0; // the positions that hold an infinity or a NaN
+                if (CAREFUL) {
+                    unsigned any = 0;
+                    const int ln = here(lane);
+#pragma unroll 4
+                    for (int c = 0; c < S::CPR; c++) {
+                        const u4 x = *reinterpret_cast<const u4 *>(vt + (ln % KEYS) * S::RB + ((c + ln) % S::CPR) * 16);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) any |= odd_bits<CT>(x[e]);
+                    }
+                    odd = __ballot(any & 0x80008000u) & ALL;
+                }
 #pragma unroll
                 for (int kk = 0; kk < 2 * HALVES; kk++)
 #pragma unroll
                     for (int db = 0; db < DB; db++) {
                         u4 x = v_operand(kk, db);
-                        if (CAREFUL) {
+                        if (CAREFUL && odd) { // uniform
 #pragma unroll
                             for (int y = 0; y < 4; y++) x[y] &= ~odd_mask<CT>(x[y]);
                         }
@@ -386,16 +398,8 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                 if (CAREFUL) {
                     // A position that only some rows see must not reach the others as a 0 times an infinity or a NaN: such
                     // values were left out above, and are added here to the rows that see them.
-                    unsigned any = 0;
-                    const int ln = here(lane);
-#pragma unroll 4
-                    for (int c = 0; c < S::CPR; c++) {
-                        const u4 x = *reinterpret_cast<const u4 *>(vt + (ln % KEYS) * S::RB + ((c + ln) % S::CPR) * 16);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) any |= odd_bits<CT>(x[e]);
-                    }
 #pragma unroll 1
-                    for (uint64_t rest = __ballot(any & 0x80008000u) & ALL; rest; rest &= rest - 1) {
+                    for (uint64_t rest = odd; rest; rest &= rest - 1) {
                         const int pos = __builtin_ctzll(rest);
                         unsigned w = 0; // the word of p that has the position's, in the lanes of its half
 #pragma unroll
