@@ -8,7 +8,7 @@
 // apart, and every work-group can work all of it out by itself: each scans the sequences, 1024 at a time, then takes every
 // so many of the rows, of the pages taken and of those put back. Only the lengths, the counts and the ring's state may be
 // written over what the others still read: then the last work-group to arrive at a counter writes those. Bound by latency:
-// lengths, scan, search, page entry, store. One row each of 48 requests 6.2 us, 700 requests of 90 rows 13.3, where an empty
+// lengths, scan, search, page entry, store. One row each of 48 requests 6.0 us, 700 requests of 90 rows 10.3, where an empty
 // launch takes 2.4.
 //
 // Commit. A path's rows rise, so its e-th row lies at or past place e, and moved in order none overwrites one that is still
@@ -20,8 +20,6 @@
 
 namespace aq {
 namespace {
-
-constexpr uint32_t TABLE_THREADS = 256;
 
 struct TablesArgs {
     const int32_t *before, *fresh, *held, *state, *depth;
@@ -35,7 +33,7 @@ struct TablesArgs {
 // Of a chunk of sequences: the sums of rows, of pages taken and of pages put back before each, and what each has and wants.
 template <uint32_t SCAN>
 struct TablesLds {
-    uint32_t rows[SCAN + 1], take[SCAN + 1], back[SCAN + 1], held[SCAN], want[SCAN], wsum[3][4], taken, last;
+    uint32_t rows[SCAN + 1], take[SCAN + 1], back[SCAN + 1], held[SCAN], want[SCAN], wsum[3][8], taken, last;
     int32_t before[SCAN];
 };
 
@@ -63,13 +61,13 @@ __device__ __forceinline__ uint32_t over(uint32_t x, uint32_t y) { return x > y 
 __device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
 
 // PER: sequences a thread scans at a time.
-template <uint32_t PER>
-__global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(TablesArgs a) {
-    constexpr uint32_t SCAN = PER * TABLE_THREADS;
+template <uint32_t PER, uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS) tables_kernel(TablesArgs a) {
+    constexpr uint32_t SCAN = PER * THREADS;
     __shared__ TablesLds<SCAN> lds;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t state0 = a.state[0], state1 = a.state[1];
-    const uint32_t me = blockIdx.x * TABLE_THREADS + tid, all = gridDim.x * TABLE_THREADS;
+    const uint32_t me = blockIdx.x * THREADS + tid, all = gridDim.x * THREADS;
 
     // The chunk of sequences from s0 on, onto the sums of those before it.
     uint32_t sums0[3] = {0, 0, 0};
@@ -105,7 +103,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(TablesArgs a) {
             at = lane ? at : 0u;
             for (uint32_t w = 0; w < wave; w++) at = plus(at, lds.wsum[k][w]);
             in[k] = plus(at, sums0[k]);
-            for (uint32_t w = 0; w < TABLE_THREADS / 64; w++) sums0[k] = plus(sums0[k], lds.wsum[k][w]);
+            for (uint32_t w = 0; w < THREADS / 64; w++) sums0[k] = plus(sums0[k], lds.wsum[k][w]);
         }
 #pragma unroll
         for (uint32_t i = 0; i < PER; i++) {
@@ -120,7 +118,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(TablesArgs a) {
             in[1] += over(r[i].want, r[i].held);
             in[2] += over(r[i].held, r[i].want);
         }
-        if (tid == TABLE_THREADS - 1) {
+        if (tid == THREADS - 1) {
             lds.rows[SCAN] = in[0];
             lds.take[SCAN] = in[1];
             lds.back[SCAN] = in[2];
@@ -138,7 +136,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(TablesArgs a) {
     auto served = [&](uint32_t l) { return lds.take[l + 1] <= count; };
     // Every so many of the chunk's rows, of the pages it takes and of those it puts back, ROWS, PAGES and PAGES of them a round:
     // all searches side by side, then all loads, then all stores, so that a round waits once for each (with the searches one
-    // after the other, 700 requests of 90 rows 17.5 us for 13.3).
+    // after the other, 700 requests of 90 rows 4 us more).
     auto items = [&](uint32_t s0, uint32_t n) {
                 constexpr int ROWS = 2, PAGES = 1, ALL = ROWS + 2 * PAGES;
         const uint32_t step0 = n > 1 ? 1u << (31 - __builtin_clz(n - 1)) : 0u;
@@ -382,15 +380,17 @@ int aq_paged_tables(aq_ctx *ctx, const aq_page_tables *t, const int32_t *kv_befo
     a.n_rows = n_rows;
     a.apart = a.held_out != a.held && a.state_out != a.state && a.kv_len != a.before;
     a.page_size = FastDiv(t->page_size);
-    // A work-group to 256 rows, or to 16 sequences, whose pages put back are not known here: 700 requests of 90 rows with 49,
-    // 98 and 197 work-groups 17.7, 15.3 and 13.3 us; 300 of one row, some of which ended, with one and 18 17.7 and 7.9. In
-    // place no more than 64: each arrives at the counter, 256 of them 6 us later.
+    // A row to a thread, or 16 threads to a sequence, whose pages put back are not known here: 700 requests of 90 rows with 49,
+    // 98 and 197 work-groups of 256 17.7, 15.3 and 13.3 us, with 99 of 512 10.3; 300 of one row, some of which ended, with one
+    // and 18 of 256 17.7 and 7.9. In place no more than 64: each arrives at the counter, 256 of them 6 us later.
     const uint64_t work = (uint64_t)t->n_seq * 16 > n_rows ? (uint64_t)t->n_seq * 16 : n_rows;
-    const uint32_t most = a.apart ? 256 : 64, grid = work < 512 ? 1 : work / 256 > most ? most : (uint32_t)(work / 256);
+    const bool small = t->n_seq <= 256;
+    const uint32_t threads = small ? 256 : 512, most = a.apart ? 65536 / threads : 64;
+    const uint32_t grid = work < 2 * threads ? 1 : work / threads > most ? most : (uint32_t)(work / threads);
     AQ_HIP(hipSetDevice(ctx->device));
     const hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
-    if (t->n_seq <= TABLE_THREADS) tables_kernel<1><<<grid, TABLE_THREADS, 0, st>>>(a);
-    else tables_kernel<4><<<grid, TABLE_THREADS, 0, st>>>(a);
+    if (small) tables_kernel<1, 256><<<grid, threads, 0, st>>>(a);
+    else tables_kernel<2, 512><<<grid, threads, 0, st>>>(a); // 1024 sequences a scan
     AQ_HIP(hipGetLastError());
     return 0;
 }
