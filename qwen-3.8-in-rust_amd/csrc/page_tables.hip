@@ -13,7 +13,8 @@
 //
 // Commit. A path's rows rise, so its e-th row lies at or past place e, and moved in order none overwrites one that is still
 // to move. A work-group has one sequence's K or V rows in one cache: its lanes find 64 entries' places at a time, then each
-// thread moves its 16 bytes of a row for entry after entry, eight on their way.
+// thread moves its 16 bytes of a row for entry after entry, eight on their way. Bound by latency: lengths, path, page entries,
+// rows. Paths of 48 trees of 8 in 16 caches (8 heads of 128, bf16), 24 MB: 6.6 us, of one of 5 (4 heads of 256, f16) 3.3.
 #include <climits>
 
 #include "paged.h"
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(TablesArgs a) {
     // all searches side by side, then all loads, then all stores, so that a round waits once for each (with the searches one
     // after the other, 700 requests of 90 rows 4 us more).
     auto items = [&](uint32_t s0, uint32_t n) {
-                constexpr int ROWS = 2, PAGES = 1, ALL = ROWS + 2 * PAGES;
+        constexpr int ROWS = 2, PAGES = 1, ALL = ROWS + 2 * PAGES;
         const uint32_t step0 = n > 1 ? 1u << (31 - __builtin_clz(n - 1)) : 0u;
         const uint32_t row_end = min(lds.rows[SCAN], a.n_rows), take_end = lds.take[SCAN], back_end = lds.back[SCAN];
         for (uint64_t row = (uint64_t)lds.rows[0] + me, take = (uint64_t)lds.take[0] + me, back = (uint64_t)lds.back[0] + me;
@@ -414,7 +415,8 @@ int aq_paged_tree_commit(aq_ctx *ctx, const aq_paged_kv *kv, uint32_t n_kv, cons
     AQ_REQUIRE(max_path < (1u << 24), "aq_paged_tree_commit: max_path");
     AQ_REQUIRE((uintptr_t)path_dev % 4 == 0 && (uintptr_t)path_len_dev % 4 == 0 && (uintptr_t)kv_len_out % 4 == 0,
                "aq_paged_tree_commit: an array is not aligned to its type");
-    AQ_REQUIRE(!kv_len_out || batch->n_seq == 0 || (kv_len_out != batch->kv_len && kv_len_out != path_len_dev),
+    AQ_REQUIRE(!kv_len_out || batch->n_seq == 0 || (kv_len_out != batch->kv_len && kv_len_out != path_len_dev &&
+                                                    kv_len_out != batch->row_start && kv_len_out != path_dev),
                "aq_paged_tree_commit: kv_len_out lies over an input");
     if (batch->n_seq == 0) return 0;
     a.path = path_dev;

@@ -119,6 +119,7 @@ def test_tree_commit(ctx):
     go(aq.AQ_EINVAL, "max_path", max_path=1 << 24)
     go(aq.AQ_EINVAL, "aligned to its type", path_len=FAKE + 1)
     go(aq.AQ_EINVAL, "lies over", kv_len_out=FAKE)
+    go(aq.AQ_EINVAL, "lies over", path=FAR)
     for kw in (dict(type=aq.BF16), dict(n_pages=63), dict(page_size=8), dict(n_head_kv=1, slot_stride=128), dict(slot_stride=256),
                dict(page_stride=1 << 14)):
         go(aq.AQ_EINVAL, "different shapes", kvs=aq.paged_kv_array([good_kv(), good_kv(**kw)]))
