@@ -78,7 +78,7 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 // Trees (TREE): a row sees what stands before its sequence's new rows, from `lo` on, and the new rows that its mask names. Of
 // the 32 positions from kb on, those that row `row` of the row tensors sees, but for lo and for positions without a page;
 // base: the first new row's position. Only the tiles that meet the new rows ask for it: 16 trees of 32 rows at 3000 (32 heads
-// on 8 of 128, bf16) 76.0 us, four of 64 at 16,000 (24 on 4 of 256) 143.7, bound as the paged attention of as many rows.
+// on 8 of 128, bf16) 75.6 us, four of 64 at 16,000 (24 on 4 of 256) 140.5, bound as the paged attention of as many rows.
 __device__ __forceinline__ uint32_t tree_bits(const AttnPagedArgs &a, int32_t row, int32_t base, int32_t kb) {
     const int32_t rel = kb - base; // uniform
     if (rel <= -32) return ~0u;

@@ -60,6 +60,26 @@ __device__ __forceinline__ unsigned pack2(float x, float y) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, e2));
 }
 
+// Whether BYTES of the LDS hold an infinity or a NaN; at: where they begin, and the lane's 16 bytes. 0 times one of them is a
+// NaN, so that products with zeros find them, in whatever order they lie; looking at each value took as many cycles as the tile's
+// own products (one tree of 64 rows at 4000, 24 heads on 4 of 256: 40.0 us, so 43.9; four at 16,000 140.5 and 144).
+template <int CT, int BYTES>
+__device__ __forceinline__ bool any_odd(const char *at) {
+    f4 z[2] = {};
+#pragma unroll
+    for (int i = 0; i < BYTES / 1024; i++) {
+        const u4 x = *reinterpret_cast<const u4 *>(at + i * 1024), none = {0, 0, 0, 0};
+        if constexpr (CT == AQ_TYPE_F16)
+            z[i % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, none), z[i % 2], 0, 0, 0);
+        else
+            z[i % 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, none), z[i % 2], 0, 0, 0);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0); // no more than these reads in registers
+    }
+    const f4 sum = z[0] + z[1];
+    const float any = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    return __any(any != any);
+}
+
 // The larger of x's two halves (lanes l and l + 32).
 __device__ __forceinline__ float both_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -372,7 +392,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                     return x;
                 };
                 uint64_t odd = 0; // the positions that hold an infinity or a NaN
-                if (CAREFUL) {
+                if (CAREFUL && any_odd<CT, S::TILE_BYTES>(vt + here(lane) * 16)) {
                     unsigned any = 0;
                     const int ln = here(lane);
 #pragma unroll 4
@@ -383,17 +403,23 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                     }
                     odd = __ballot(any & 0x80008000u) & ALL;
                 }
+                constexpr int TOGETHER = DB < 4 ? DB : 4; // V operands between two of the branches that leave values out
 #pragma unroll
                 for (int kk = 0; kk < 2 * HALVES; kk++)
 #pragma unroll
-                    for (int db = 0; db < DB; db++) {
-                        u4 x = v_operand(kk, db);
+                    for (int db = 0; db < DB; db += TOGETHER) {
+                        u4 x[TOGETHER];
+#pragma unroll
+                        for (int i = 0; i < TOGETHER; i++) x[i] = v_operand(kk, db + i);
                         if (CAREFUL && odd) { // uniform
 #pragma unroll
-                            for (int y = 0; y < 4; y++) x[y] &= ~odd_mask<CT>(x[y]);
+                            for (int i = 0; i < TOGETHER; i++)
+#pragma unroll
+                                for (int y = 0; y < 4; y++) x[i][y] &= ~odd_mask<CT>(x[i][y]);
                         }
-                        o[db] = mfma32<CT>(x, p[kk], o[db]);
-                        if (CAREFUL || (D == 256 && db % 4 == 3)) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int i = 0; i < TOGETHER; i++) o[db + i] = mfma32<CT>(x[i], p[kk], o[db + i]);
+                        if (CAREFUL || D == 256) __builtin_amdgcn_sched_barrier(0);
                     }
                 if (CAREFUL) {
                     // A position that only some rows see must not reach the others as a 0 times an infinity or a NaN: such
