@@ -80,6 +80,9 @@ __device__ __forceinline__ bool any_odd(const char *at) {
     return __any(any != any);
 }
 
+// The lowest n bits of a word.
+__device__ __forceinline__ uint32_t ones_below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+
 // The larger of x's two halves (lanes l and l + 32).
 __device__ __forceinline__ float both_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -303,10 +306,12 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
             auto sum_tile = [&](auto careful) __attribute__((always_inline)) {
                 constexpr bool CAREFUL = decltype(careful)::value;
                 f16v s[HALVES];
-                uint32_t bits[HALVES] = {}; // TREE: the positions that the row sees
-                if constexpr (TREE && CAREFUL) {
+                uint32_t bits[HALVES] = {}; // the positions that the row sees
+                if constexpr (CAREFUL) {
 #pragma unroll
-                    for (int k = 0; k < HALVES; k++) bits[k] = tree_bits(a, hi, base, kb + 32 * k);
+                    for (int k = 0; k < HALVES; k++)
+                        bits[k] = (TREE ? tree_bits(a, hi, base, kb + 32 * k) : ones_below(hi - kb - 32 * k)) &
+                                  ~ones_below(lo - kb - 32 * k);
                 }
                 const int ka = here(kaddr0), va = here(vaddr0);
 #pragma unroll
@@ -322,22 +327,14 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                         if (D == 256 && st % 8 == 7) __builtin_amdgcn_sched_barrier(0);
                     }
                 if (CAREFUL && edge) {
-                    const int hr = hi - kb - 4 * h, lr = lo - kb - 4 * h; // of position 0 of this lane's
 #pragma unroll
-                    for (int k = 0; k < HALVES; k++)
+                    for (int k = 0; k < HALVES; k++) {
+                        const uint32_t mine = (bits[k] & (uint32_t)(ok_now >> (32 * k))) >> (4 * here(h));
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const int pos = 32 * k + 8 * (i / 4) + i % 4;
-                            const bool seen = TREE ? (bits[k] >> (4 * h) >> (pos - 32 * k)) & 1 : pos < hr;
-                            s[k][i] = seen && pos >= lr ? s[k][i] : -INFINITY;
+                            const uint32_t all = (uint32_t)__builtin_amdgcn_sbfe((int)mine, 8 * (i / 4) + i % 4, 1); // all ones: seen
+                            s[k][i] = __uint_as_float((__float_as_uint(s[k][i]) & all) | (~all & 0xFF800000u));
                         }
-                    if (ok_now != ALL) {
-                        const uint64_t mine = ok_now >> (4 * here(h));
-#pragma unroll
-                        for (int k = 0; k < HALVES; k++)
-#pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                s[k][i] = (mine >> (32 * k + 8 * (i / 4) + i % 4)) & 1 ? s[k][i] : -INFINITY;
                     }
                 }
                 float mt = s[0][0];
@@ -435,8 +432,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
                         w = (unsigned)__shfl((int)w, here(n) + 32 * (pos / 4 % 2));
                         using T = typename RowType<CT>::type;
                         const float pv = (float)__builtin_bit_cast(T, (uint16_t)(pos & 1 ? w >> 16 : w));
-                        const bool sees = (TREE ? (bits[HALVES > 1 && pos >= 32 ? 1 : 0] >> pos % 32) & 1 : kb + pos < hi) &&
-                                          kb + pos >= lo;
+                        const bool sees = (bits[HALVES > 1 && pos >= 32 ? 1 : 0] >> pos % 32) & 1;
                         const char *row = vt + pos * S::RB + here(8 * h);
 #pragma unroll
                         for (int db = 0; db < DB; db++)
