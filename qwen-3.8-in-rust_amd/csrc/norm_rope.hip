@@ -74,7 +74,7 @@ __device__ __forceinline__ void store_raw(E *p, const float *v) {
 // and a wave takes HB times as many heads as fit it. NU: units a lane has at most (one where 16 bytes are moved at a time).
 // A unit: VEC values of either half of what is turned (half layout), of either half of what passes through, or VEC neighbours.
 // Little of it branches: a lane past the head's units has the first one's once more, a unit without second values its first
-// ones twice, a head past the last the last's, and only the stores are left out.
+// ones twice, a head past the last is the last one again (its values, its weight), and only the stores are left out.
 template <int TI, int TO, bool INTER, int VEC, bool W, int NU, bool PAGED>
 __global__ void __launch_bounds__(256, 8) norm_kernel(NormArgs a) {
     using EI = typename RowType<TI>::type;
@@ -100,12 +100,14 @@ __global__ void __launch_bounds__(256, 8) norm_kernel(NormArgs a) {
         two[i] = at[i] + (both[i] ? (rot[i] ? a.dim / 2 : a.pass_units * VEC) : 0);
         pair[i] = rot[i] ? (INTER ? at[i] / 2 : at[i]) : 0;
     }
-    // A job: one head of the row's queries, keys or values.
+    // A job: one head of the row's queries, keys or values. What is not there has null pointers, so a job past the last is
+    // the last one again wherever it chooses between them.
     const uint32_t per = 64u >> a.lane_shift, j0 = part * HB * per + (lane >> a.lane_shift);
+    auto job = [&](int h) { return min(j0 + h * per, a.jobs - 1); };
     Raw<TI, N> raw[HB][NU];
 #pragma unroll
     for (int h = 0; h < (int)HB; h++) {
-        const uint32_t j = min(j0 + h * per, a.jobs - 1);
+        const uint32_t j = job(h);
         const bool q = j < a.nq, k = j < a.nqk;
         const EI *p = (const EI *)(q ? a.q.p : k ? a.k.p : a.v.p) + row * (q ? a.q.row : k ? a.k.row : a.v.row) +
                       (int64_t)(j - (q ? 0 : k ? a.nq : a.nqk)) * (q ? a.q.head : k ? a.k.head : a.v.head);
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(256, 8) norm_kernel(NormArgs a) {
 
 #pragma unroll
     for (int h = 0; h < (int)HB; h++) {
-        const uint32_t j = j0 + h * per;
+        const uint32_t j = job(h);
         const bool q = j < a.nq, k = j < a.nqk;
         float v[NU][N];
 #pragma unroll
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(256, 8) norm_kernel(NormArgs a) {
                 }
             }
         }
-        if (j >= a.jobs) continue;
+        if (j0 + h * per >= a.jobs) continue;
         auto put = [&](auto *to) {
 #pragma unroll
             for (int i = 0; i < NU; i++) {
