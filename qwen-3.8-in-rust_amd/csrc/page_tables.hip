@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(256) commit_kernel(CommitArgs a) {
     char *const pool = a.pools[blockIdx.y];
     const int32_t *path = a.path + (size_t)seq * a.max_path, *table = a.b.pages + (size_t)seq * a.b.max_pages;
     const SeqRows sr = paged_seq(a.b, seq);
-    const int32_t fresh = sr.len - sr.base; // all of its new rows
+    const int32_t base = sr.before, fresh = sr.len - base; // all of its new rows
     const uint32_t len = (uint32_t)min(max(a.path_len[seq], 0), (int32_t)min(a.max_path, (uint32_t)INT_MAX));
     int32_t before = -1;  // the entry before the 64
     uint32_t kept = 0;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(256) commit_kernel(CommitArgs a) {
         before = __shfl(from, 63);
         kept += n;
         whole = n == 64;
-        const int32_t src = sr.base + from, dst = sr.base + (int32_t)e;
+        const int32_t src = base + from, dst = base + (int32_t)e;
         uint32_t from_units = 0, to_units = 0;
         bool moves = lane < n && from != (int32_t)e && dst >= 0;
         if (moves) {
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(256) commit_kernel(CommitArgs a) {
             }
         }
     }
-    if (a.kv_len_out && blockIdx.y == 0 && threadIdx.x == 0) a.kv_len_out[seq] = max(sr.base + (int32_t)kept, 0);
+    if (a.kv_len_out && blockIdx.y == 0 && threadIdx.x == 0) a.kv_len_out[seq] = max(base + (int32_t)kept, 0);
 }
 
 } // namespace

@@ -97,9 +97,10 @@ __device__ __forceinline__ uint32_t paged_seq_of(const PagedBatch &b, uint32_t r
 }
 
 // A sequence's rows within the tensors' n_rows, whatever row_start holds, the position of the first of them and one past the
-// last of all: a sequence that begins before the tensors or ends past them keeps its other rows' positions.
+// last of all: a sequence that begins before the tensors or ends past them keeps its other rows' positions. before: the
+// position of its first new row, also where that lies before the tensors (a tree's masks and paths count from there).
 struct SeqRows {
-    int32_t first, n, base, len;
+    int32_t first, n, base, len, before;
 };
 __device__ __forceinline__ SeqRows paged_seq(const PagedBatch &b, uint32_t s) {
     const int32_t lo = b.row_start[s], hi = b.row_start[s + 1], len = b.kv_len[s];
@@ -109,6 +110,7 @@ __device__ __forceinline__ SeqRows paged_seq(const PagedBatch &b, uint32_t s) {
     r.n = end > r.first ? end - r.first : 0;
     r.len = len > 0 ? len : 0;
     r.base = r.len - (hi > r.first ? hi - r.first : 0);
+    r.before = r.len - (hi > lo ? (int32_t)min((uint32_t)hi - (uint32_t)lo, 0x7FFFFFFFu) : 0);
     return r;
 }
 

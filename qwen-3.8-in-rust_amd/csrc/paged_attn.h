@@ -58,7 +58,8 @@ struct UnitRange {
 template <bool TREE>
 __device__ __forceinline__ UnitRange tile_units(const AttnPagedArgs &a, const SeqRows &sr, int32_t r0, int32_t R, uint32_t tk) {
     const int32_t last = min(r0 + R, sr.n * a.G) - 1;
-    const int32_t t0 = (int32_t)a.by_g.quot(r0), t1 = (int32_t)a.by_g.quot(last), base = sr.base; // row tokens' positions are base + token
+    const int32_t t0 = (int32_t)a.by_g.quot(r0), t1 = (int32_t)a.by_g.quot(last);
+    const int32_t base = TREE ? sr.before : sr.base; // row tokens' positions are base + token; TREE: the first new row's
     const int32_t end = min(TREE ? sr.len : max(base + t1 + 1, 0), (int32_t)a.cap);
     const int64_t begin = a.window ? max((int64_t)base + (TREE ? 0 : t0 + 1) - (int64_t)a.window, (int64_t)0) : 0;
     UnitRange u;

@@ -1,5 +1,8 @@
-"""The calls of a speculative step over pages where their arguments end: heads that leave lanes of a wave without one. Against
-the definitions in 64 bits; tolerances: tree_plain.norm_bound and paged_plain.bound, by arithmetic."""
+"""The calls of a speculative step over pages where their arguments end: heads that leave lanes of a wave without one, trees
+that begin before the row tensors. Against the definitions in 64 bits; tolerances: tree_plain.norm_bound and paged_plain.bound,
+by arithmetic."""
+import math
+
 import numpy as np
 import pytest
 
@@ -40,3 +43,54 @@ def test_one_tensor_of_any_number_of_heads(ctx, t, layout, hd, dim, pad):
                             None if first else dw.buf, EPS, rope, dpos.buf)
             ctx.sync()
             assert np.all(np.abs(out.get() - want) <= limit)
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("new,window", [(7, 0), (7, 9), (70, 0), (70, 90)])
+def test_trees_that_begin_before_the_tensors(ctx, row_t, cache_t, new, window):
+    """row_start below 0: the rows that there are have their own masks, whose bits count from the tree's first row."""
+    print(f"begins before {row_t}/{cache_t} new {new} window {window}", flush=True)
+    rng = np.random.default_rng(new)
+    heads, kv, hd, skip = 4, 2, 128, new // 2 + 1
+    pg = P.Paged(ctx, rng, [new, 5], [new + 200, 77], kv, hd, 16, cache_t)
+    masks = [m | (rng.random(len(m)) < 0.3) for m in T.random_trees(rng, pg.new)]
+    x = rng.standard_normal((pg.rows, heads, hd))
+    scale = float(np.float32(1.0 / math.sqrt(hd)))
+    want, parts = T.tree_attention(pg, masks, P.values(P.store(x, row_t), row_t), scale, window)
+    limit = P.bound(parts, want, row_t, cache_t, hd)[skip:]
+    q, out = P.Rows(ctx, x[skip:], row_t), P.Rows(ctx, np.full(x[skip:].shape, 9.0), row_t)
+    starts, words = P.Dev(ctx, (pg.starts - skip).astype(np.int32)), -(-new // 32)
+    dm = P.Dev(ctx, T.pack(masks[skip:], words))
+    cache, _ = pg.structs()
+    for most in (pg.max_len, 5 << 20):  # the second: bounds with which many 16-bit rows take a kernel of their own
+        table = np.full((2, -(-max(most, 300) // 16)), -1, np.int32)
+        table[:, : pg.cols] = pg.table
+        dt = P.Dev(ctx, table)
+        b = aq.paged_batch(2, starts.buf, pg.dlens.buf, dt.buf, table.shape[1], q.rows, new, most)
+        ws = aq.DeviceBuffer(ctx, aq.paged_attention_workspace(ctx, cache, b, heads))
+        aq.paged_tree_attention(ctx, cache, b, dm.buf, words, heads, q.heads_struct(), out.heads_struct(), scale, window, None, ws)
+        ctx.sync()
+        assert np.all(np.abs(out.get() - want[skip:]) <= limit)
+
+
+def test_paths_of_trees_that_begin_before_the_tensors(ctx):
+    """The rows to move lie in the pages, wherever the row tensors begin: of one that begins before them, of one that ends
+    before them, and of one that ends past them."""
+    rng = np.random.default_rng(3)
+    pg = P.Paged(ctx, rng, [4, 9, 6], [30, 50, 21], 2, 64, 16, "bf16")
+    paths, m = np.array([[1, 3, -1, -1], [0, 2, 5, 8], [2, 3, 5, -1]], np.int32), np.array([2, 4, 3], np.int32)
+    starts, dp, dm = P.Dev(ctx, pg.starts - 7), P.Dev(ctx, paths), P.Dev(ctx, m)
+    out = P.Dev(ctx, np.full(3, 5, np.int32))
+    cache, _ = pg.structs()
+    b = aq.paged_batch(3, starts.buf, pg.dlens.buf, pg.dtable.buf, pg.cols, 9, 9, 50)
+    aq.paged_tree_commit(ctx, aq.paged_kv_array([cache]), b, dp.buf, dm.buf, 4, out.buf)
+    ctx.sync()
+    k, v = pg.k.copy(), pg.v.copy()
+    for s in range(3):
+        base = pg.lens[s] - pg.new[s]
+        for i in range(int(m[s])):
+            a, to = pg.row_of(s, base + int(paths[s, i])), pg.row_of(s, base + i)
+            k[to], v[to] = k[a], v[a]
+    got = pg.pools()
+    assert np.array_equal(got[0], k, equal_nan=True) and np.array_equal(got[1], v, equal_nan=True)
+    assert out.get().tolist() == [n - w + int(x) for n, w, x in zip(pg.lens, pg.new, m)]
