@@ -76,6 +76,9 @@ __device__ __forceinline__ uint32_t share_chunk(uint32_t total, uint32_t shares,
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The lowest n bits of a word.
+__device__ __forceinline__ uint32_t ones_below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+
 // Trees (TREE): a row sees what stands before its sequence's new rows, from `lo` on, and the new rows that its mask names. Of
 // the 32 positions from kb on, those that row `row` of the row tensors sees, but for lo and for positions without a page;
 // base: the first new row's position. Only the tiles that meet the new rows ask for it: 16 trees of 32 rows at 3000 (32 heads
@@ -90,12 +93,14 @@ __device__ __forceinline__ uint32_t tree_bits(const AttnPagedArgs &a, int32_t ro
     const uint64_t two = (w < a.mask_words ? m[w] : 0u) | (uint64_t)(w + 1 < a.mask_words ? m[w + 1] : 0u) << 32;
     return (uint32_t)(two >> (rel % 32));
 }
-// The first position that a row sees before the new rows: with a window, as many places back as that leaves beside the n new
-// rows it sees.
-__device__ __forceinline__ int32_t tree_lo(const AttnPagedArgs &a, int32_t row, int32_t base) {
+// The first position that a row sees before the `fresh` new rows: with a window, as many places back as that leaves beside the
+// new rows it sees. Bits past the new rows name none.
+__device__ __forceinline__ int32_t tree_lo(const AttnPagedArgs &a, int32_t row, int32_t base, int32_t fresh) {
     if (!a.window || row < 0) return 0;
     int64_t own = base;
-    for (uint32_t w = 0; w < a.mask_words; w++) own += __popc(a.mask[(size_t)row * a.mask_words + w]);
+    const uint32_t words = min(a.mask_words, ((uint32_t)fresh + 31) / 32);
+    for (uint32_t w = 0; w < words; w++)
+        own += __popc(a.mask[(size_t)row * a.mask_words + w] & ones_below(fresh - 32 * (int32_t)w));
     return (int32_t)max(min(own - (int64_t)a.window, (int64_t)base), (int64_t)0);
 }
 

@@ -80,9 +80,6 @@ __device__ __forceinline__ bool any_odd(const char *at) {
     return __any(any != any);
 }
 
-// The lowest n bits of a word.
-__device__ __forceinline__ uint32_t ones_below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
-
 // The larger of x's two halves (lanes l and l + 32).
 __device__ __forceinline__ float both_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -196,7 +193,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnPagedArgs a) {
         const bool have = rr < n_rows;
         const int32_t hi = have ? (TREE ? sr.first + tok : base + tok + 1) : (TREE ? -1 : 0); // TREE: its row of the mask
         const int64_t lo64 = a.window ? (int64_t)base + tok + 1 - (int64_t)a.window : 0;
-        const int32_t lo = TREE ? tree_lo(a, hi, base) : lo64 > 0 ? (int32_t)lo64 : 0;
+        const int32_t lo = TREE ? tree_lo(a, hi, base, sr.len - base) : lo64 > 0 ? (int32_t)lo64 : 0;
         const int32_t w0 = sg.r0 + 32 * wave, w1 = min(w0 + 32, n_rows) - 1;
         const bool idle = w0 >= n_rows; // a wave without rows only loads
         const int32_t tok0 = (int32_t)a.by_g.quot(w0), tok1 = idle ? tok0 : (int32_t)a.by_g.quot(w1);

@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256, 2) few_rows_kernel(AttnPagedArgs a) {
             const int32_t rr = r0 + 16 * (rg * NR + nr) + r, tok = (int32_t)a.by_g.quot(rr);
             if constexpr (TREE) {
                 hi[nr] = rr < n_rows ? sr.first + tok : -1;
-                lo[nr] = tree_lo(a, hi[nr], base);
+                lo[nr] = tree_lo(a, hi[nr], base, sr.len - base);
             } else {
                 hi[nr] = rr < n_rows ? base + tok + 1 : 0;
                 const int64_t l = a.window ? (int64_t)base + tok + 1 - (int64_t)a.window : 0;

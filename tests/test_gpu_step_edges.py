@@ -1,6 +1,6 @@
 """The calls of a speculative step over pages where their arguments end: heads that leave lanes of a wave without one, trees
-that begin before the row tensors. Against the definitions in 64 bits; tolerances: tree_plain.norm_bound and paged_plain.bound,
-by arithmetic."""
+that begin before the row tensors, mask words longer than a tree. Against the definitions in 64 bits; tolerances:
+tree_plain.norm_bound and paged_plain.bound, by arithmetic."""
 import math
 
 import numpy as np
@@ -94,3 +94,37 @@ def test_paths_of_trees_that_begin_before_the_tensors(ctx):
     got = pg.pools()
     assert np.array_equal(got[0], k, equal_nan=True) and np.array_equal(got[1], v, equal_nan=True)
     assert out.get().tolist() == [n - w + int(x) for n, w, x in zip(pg.lens, pg.new, m)]
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("n", [1, 5, 31, 32, 33])
+def test_bits_past_a_short_tree(ctx, row_t, cache_t, n):
+    """Beside a large tree a small one whose words hold ones past its own rows: with a window they count for nothing."""
+    print(f"spare bits {row_t}/{cache_t} {n}", flush=True)
+    rng = np.random.default_rng(n)
+    heads, kv, hd, big, words = 4, 2, 64, 70, 4
+    pg = P.Paged(ctx, rng, [n, big, n], [n + 100, big + 60, n + 3], kv, hd, 16, cache_t)
+    masks = T.random_trees(rng, pg.new)
+    packed = T.pack(masks, words)
+    for r, m in enumerate(masks):
+        spare = np.ones(32 * words, bool)
+        spare[: len(m)] = False
+        packed[r] |= T.pack([spare], words)[0]
+    dm = P.Dev(ctx, packed)
+    q = P.Rows(ctx, rng.standard_normal((pg.rows, heads, hd)), row_t)
+    scale = float(np.float32(1.0 / math.sqrt(hd)))
+    for window in (1, 40, 140):
+        want, parts = T.tree_attention(pg, masks, q.values(), scale, window)
+        limit = P.bound(parts, want, row_t, cache_t, hd)
+        for most in (pg.max_len, 5 << 16):
+            table = np.full((3, -(-most // 16)), -1, np.int32)
+            table[:, : pg.cols] = pg.table[:, : table.shape[1]]
+            dt = P.Dev(ctx, table)
+            cache, _ = pg.structs()
+            b = aq.paged_batch(3, pg.dstarts.buf, pg.dlens.buf, dt.buf, table.shape[1], pg.rows, big, most)
+            ws = aq.DeviceBuffer(ctx, aq.paged_attention_workspace(ctx, cache, b, heads))
+            out = P.Rows(ctx, np.full((pg.rows, heads, hd), 9.0), row_t)
+            aq.paged_tree_attention(ctx, cache, b, dm.buf, words, heads, q.heads_struct(), out.heads_struct(), scale, window, None,
+                                    ws)
+            ctx.sync()
+            assert np.all(np.abs(out.get() - want) <= limit)
