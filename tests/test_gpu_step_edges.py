@@ -128,3 +128,31 @@ def test_bits_past_a_short_tree(ctx, row_t, cache_t, n):
                                     ws)
             ctx.sync()
             assert np.all(np.abs(out.get() - want) <= limit)
+
+
+@pytest.mark.parametrize("row_t,cache_t", PAIRS)
+@pytest.mark.parametrize("new,window", [(6, 4), (70, 33)])
+def test_chains_longer_than_the_window(ctx, row_t, cache_t, new, window):
+    """A tree without branches: paged_attention's outputs up to the row that fills the window; the rows after it see their
+    whole path and nothing before it."""
+    print(f"long chain {row_t}/{cache_t} {new} window {window}", flush=True)
+    rng = np.random.default_rng(window)
+    heads, kv, hd = 4, 2, 128
+    pg = P.Paged(ctx, rng, [new], [new + 100], kv, hd, 16, cache_t)
+    masks = [np.arange(new) <= i for i in range(new)]
+    q = P.Rows(ctx, rng.standard_normal((new, heads, hd)), row_t)
+    scale, words = float(np.float32(1.0 / math.sqrt(hd))), -(-new // 32)
+    want, parts = T.tree_attention(pg, masks, q.values(), scale, window)
+    run, run_parts = P.attention(pg, q.values(), scale, window)
+    limit, run_limit = (P.bound(x, y, row_t, cache_t, hd) for x, y in ((parts, want), (run_parts, run)))
+    assert np.array_equal(parts[2], [max(window, i + 1) for i in range(new)])
+    assert np.abs(want[window:] - run[window:]).max() > 0.1  # another row of values
+    cache, batch = pg.structs()
+    dm = P.Dev(ctx, T.pack(masks, words))
+    ws = aq.DeviceBuffer(ctx, aq.paged_attention_workspace(ctx, cache, batch, heads))
+    tree, chain = (P.Rows(ctx, np.full((new, heads, hd), 9.0), row_t) for _ in range(2))
+    aq.paged_tree_attention(ctx, cache, batch, dm.buf, words, heads, q.heads_struct(), tree.heads_struct(), scale, window, None, ws)
+    aq.paged_attention(ctx, cache, batch, heads, q.heads_struct(), chain.heads_struct(), scale, window, None, ws)
+    ctx.sync()
+    assert np.all(np.abs(tree.get() - want) <= limit) and np.all(np.abs(chain.get() - run) <= run_limit)
+    assert np.all(np.abs(tree.get() - chain.get())[:window] <= (limit + run_limit)[:window])
