@@ -272,6 +272,7 @@ struct CommitArgs {
 __global__ void __launch_bounds__(256) commit_kernel(CommitArgs a) {
     constexpr int FLIGHT = 8;
     const uint32_t seq = blockIdx.x, lane = threadIdx.x & 63;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     char *const pool = a.pools[blockIdx.y];
     const int32_t *path = a.path + (size_t)seq * a.max_path, *table = a.b.pages + (size_t)seq * a.b.max_pages;
     const SeqRows sr = paged_seq(a.b, seq);
@@ -300,28 +301,32 @@ __global__ void __launch_bounds__(256) commit_kernel(CommitArgs a) {
         }
         const uint64_t todo = __ballot(moves);
         if (!todo) continue;
-        for (uint32_t c = threadIdx.x; c < a.chunks; c += blockDim.x) {
-            const uint32_t head = a.per_head.quot(c);
+        // A wave's pieces, 64 at a time. All its lanes are on where a place is read from the lane that has it; only the moves
+        // leave out lanes past the last piece.
+        for (uint32_t c0 = wave * 64; c0 < a.chunks; c0 += blockDim.x) { // uniform
+            const uint32_t c = c0 + lane, head = a.per_head.quot(c);
             char *const at = pool + (uint64_t)head * a.kv.head_bytes + (c - head * a.per_head.d) * 16;
             uint64_t rest = todo;
             while (rest) { // uniform
-                u4 x[FLIGHT];
-                uint64_t left = rest;
-#pragma unroll
-                for (int i = 0; i < FLIGHT; i++) {
-                    if (!left) break;
-                    const int l = __builtin_ctzll(left);
-                    left &= left - 1;
-                    x[i] = *reinterpret_cast<const u4 *>(
-                        at + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)from_units, l) << a.kv.unit_shift));
-                }
+                uint32_t from_at[FLIGHT], to_at[FLIGHT];
+                int flying = 0;
 #pragma unroll
                 for (int i = 0; i < FLIGHT; i++) {
                     if (!rest) break;
                     const int l = __builtin_ctzll(rest);
                     rest &= rest - 1;
-                    *reinterpret_cast<u4 *>(
-                        at + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)to_units, l) << a.kv.unit_shift)) = x[i];
+                    from_at[i] = (uint32_t)__builtin_amdgcn_readlane((int)from_units, l);
+                    to_at[i] = (uint32_t)__builtin_amdgcn_readlane((int)to_units, l);
+                    flying++;
+                }
+                if (c < a.chunks) {
+                    u4 x[FLIGHT];
+#pragma unroll
+                    for (int i = 0; i < FLIGHT; i++)
+                        if (i < flying) x[i] = *reinterpret_cast<const u4 *>(at + ((uint64_t)from_at[i] << a.kv.unit_shift));
+#pragma unroll
+                    for (int i = 0; i < FLIGHT; i++)
+                        if (i < flying) *reinterpret_cast<u4 *>(at + ((uint64_t)to_at[i] << a.kv.unit_shift)) = x[i];
                 }
             }
         }

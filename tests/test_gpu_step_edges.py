@@ -1,6 +1,6 @@
 """The calls of a speculative step over pages where their arguments end: heads that leave lanes of a wave without one, trees
-that begin before the row tensors, mask words longer than a tree. Against the definitions in 64 bits; tolerances:
-tree_plain.norm_bound and paged_plain.bound, by arithmetic."""
+that begin before the row tensors, mask words longer than a tree, rows of any number of pieces to move. Against the
+definitions, in 64 bits; tolerances: tree_plain.norm_bound and paged_plain.bound, by arithmetic; what is copied is equal."""
 import math
 
 import numpy as np
@@ -156,3 +156,28 @@ def test_chains_longer_than_the_window(ctx, row_t, cache_t, new, window):
     ctx.sync()
     assert np.all(np.abs(tree.get() - want) <= limit) and np.all(np.abs(chain.get() - run) <= run_limit)
     assert np.all(np.abs(tree.get() - chain.get())[:window] <= (limit + run_limit)[:window])
+
+
+@pytest.mark.parametrize("kv,hd", [(1, 8), (1, 64), (33, 8), (3, 168), (13, 40), (5, 104), (25, 64), (26, 80), (31, 128), (65, 64)])
+def test_paths_over_rows_of_any_size(ctx, kv, hd):
+    """1, 8, 33, 63, 65, 200, 260, 496 and 520 pieces of 16 bytes in a row: waves with lanes, and whole waves, that have none.
+    Paths of more entries than a wave has lanes, and than are on their way together."""
+    print(f"commit {kv} x {hd}", flush=True)
+    rng = np.random.default_rng(kv * hd)
+    new, keep = [100, 12, 3], [70, 9, 2]
+    pg = P.Paged(ctx, rng, new, [130, 20, 40], kv, hd, 4, "bf16")
+    paths = np.full((3, 80), -1, np.int32)
+    for s in range(3):
+        paths[s, : keep[s]] = np.sort(rng.choice(new[s], keep[s], replace=False))
+    dp, dm = P.Dev(ctx, paths), P.Dev(ctx, np.array(keep, np.int32))
+    cache, batch = pg.structs()
+    aq.paged_tree_commit(ctx, cache, batch, dp.buf, dm.buf, 80)
+    ctx.sync()
+    k, v = pg.k.copy(), pg.v.copy()
+    for s in range(3):
+        base = pg.lens[s] - new[s]
+        for i in range(keep[s]):
+            a, to = pg.row_of(s, base + int(paths[s, i])), pg.row_of(s, base + i)
+            k[to], v[to] = k[a], v[a]
+    got = pg.pools()
+    assert np.array_equal(got[0], k, equal_nan=True) and np.array_equal(got[1], v, equal_nan=True)
