@@ -379,7 +379,8 @@ typedef struct aq_page_tables {
  * table has -1 for them, and missing[s] (nullable) says how many of the pages it needs it lacks. Of row r < n_rows, pos[r]
  * (nullable) is its position, kv_before[s] + row_depth[r] where row_depth is given (a tree's drafts), and slots[r]
  * (nullable) its place in the pool, page * page_size + slot; without a page, and behind the last sequence's rows, -1 (and
- * position 0 there). kv_len may be kv_before, the other outputs are memory of their own. A page is held once. */
+ * position 0 there). kv_len may be kv_before, the other outputs are memory of their own (what lies over another
+ * array of the call, in whole or in part, is refused). A page is held once. */
 int aq_paged_tables(aq_ctx *ctx, const aq_page_tables *tables, const int32_t *kv_before, const int32_t *n_new,
                     uint32_t n_rows, int32_t *row_start, int32_t *kv_len, int32_t *missing, int32_t *pos, int64_t *slots,
                     const int32_t *row_depth, void *stream);

@@ -334,6 +334,16 @@ __global__ void __launch_bounds__(256) commit_kernel(CommitArgs a) {
     if (a.kv_len_out && blockIdx.y == 0 && threadIdx.x == 0) a.kv_len_out[seq] = max(base + (int32_t)kept, 0);
 }
 
+// What the host sees of an array: where it begins, and its bytes.
+struct Span {
+    const void *p;
+    size_t bytes;
+    bool meets(const Span &x) const {
+        const uintptr_t a = (uintptr_t)p, b = (uintptr_t)x.p;
+        return a && b && bytes && x.bytes && a < b + x.bytes && b < a + bytes;
+    }
+};
+
 } // namespace
 } // namespace aq
 
@@ -362,9 +372,16 @@ int aq_paged_tables(aq_ctx *ctx, const aq_page_tables *t, const int32_t *kv_befo
                          n_new,    row_start, kv_len,     missing,       pos,           row_depth};
     for (const void *p : all) AQ_REQUIRE((uintptr_t)p % 4 == 0, "aq_paged_tables: an array is not aligned to its type");
     AQ_REQUIRE((uintptr_t)slots % 8 == 0, "aq_paged_tables: an array is not aligned to its type");
-    AQ_REQUIRE(t->n_seq == 0 || (n_new != kv_len && n_new != t->held_out && n_new != row_start && kv_before != row_start &&
-                                 kv_before != t->held_out && t->held != kv_len),
-               "aq_paged_tables: an output lies over another input");
+    const size_t seqs = (size_t)t->n_seq * 4, rows = (size_t)n_rows * 4;
+    const Span spans[] = {{t->held_out, seqs}, {t->free_state_out, 16}, {kv_len, seqs}, // these three may be an input's own array
+                          {t->held, seqs}, {t->free_state, 16}, {kv_before, seqs}, {n_new, seqs}, {row_depth, rows},
+                          {row_start, seqs + 4}, {missing, seqs}, {pos, rows}, {slots, 2 * rows}, {t->pages, seqs * t->max_pages},
+                          {t->free_pages, (size_t)t->n_pages * 4}};
+    constexpr int OUT = 3, READ = 8, ALL = sizeof(spans) / sizeof(spans[0]); // 3 .. 7 are only read
+    for (int i = 0; i < ALL; i++)
+        for (int j = i + 1; j < ALL; j++)
+            AQ_REQUIRE(!spans[i].meets(spans[j]) || (i >= OUT && j < READ) || (j == i + OUT && i < OUT && spans[i].p == spans[j].p),
+                       "aq_paged_tables: an output lies over another array");
     TablesArgs a;
     a.before = kv_before;
     a.fresh = n_new;

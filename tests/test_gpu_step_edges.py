@@ -181,3 +181,37 @@ def test_paths_over_rows_of_any_size(ctx, kv, hd):
             k[to], v[to] = k[a], v[a]
     got = pg.pools()
     assert np.array_equal(got[0], k, equal_nan=True) and np.array_equal(got[1], v, equal_nan=True)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_tables_of_arrays_side_by_side(ctx, in_place):
+    """All arrays of the call in one allocation, each from where the one before ends: nothing lies over another."""
+    print(f"side by side, in place {in_place}", flush=True)
+    rng = np.random.default_rng(4)
+    n, cols, pool, page, rows = 7, 5, 30, 4, 41
+    w = T.Tables(n, cols, pool, page)
+    w.ring = rng.permutation(pool).astype(np.int32)
+    new = [6, 0, 9, 3, 12, 1, 7]
+    sizes = {"slots": 2 * rows, "pages": n * cols, "held": n, "held_out": n, "ring": pool, "state": 4, "state_out": 4, "before": n,
+             "new": n, "start": n + 1, "len": n, "missing": n, "pos": rows, "depth": rows}
+    first = dict(zip(sizes, np.concatenate([[0], np.cumsum(list(sizes.values()))])))
+    whole = np.zeros(sum(sizes.values()), np.int32)
+    depth = rng.integers(0, 5, rows)
+    for name, x in (("pages", w.pages.ravel()), ("ring", w.ring), ("state", [0, pool, 0, 0]), ("new", new), ("depth", depth)):
+        whole[first[name]: first[name] + sizes[name]] = x
+    d = P.Dev(ctx, whole)
+    at = {name: d.buf.p.value + 4 * int(i) for name, i in first.items()}
+    t = aq.page_tables(n, cols, pool, page, at["pages"], at["held"], at["ring"], at["state"], None if in_place else at["held_out"],
+                       None if in_place else at["state_out"])
+    length = "before" if in_place else "len"
+    aq.paged_tables(ctx, t, at["before"], at["new"], rows, at["start"], at[length], at["missing"], at["pos"], at["slots"],
+                    at["depth"])
+    ctx.sync()
+    got = d.get()
+    want = dict(zip(("start", length, "missing", "pos", "slots"), w.step(np.zeros(n), new, rows, depth)))
+    out = "" if in_place else "_out"
+    want.update({"pages": w.pages, "ring": w.ring, "held" + out: w.held, "state" + out: [w.first, w.count, 0, 0], "new": new,
+                 "depth": depth})
+    for name, x in want.items():
+        x = np.ascontiguousarray(x, np.int64).view(np.int32) if name == "slots" else np.ravel(x)
+        assert np.array_equal(got[first[name]: first[name] + sizes[name]], x), name

@@ -1,0 +1,32 @@
+"""Outputs of the page tables that lie over another array of the call, in whole or in part, are refused, with their codes and
+texts, before anything touches a device (no GPU needed)."""
+import pytest
+
+import aqueduct as aq
+from test_paged_refusals import FakeCtx, refused
+
+N_SEQ, COLS, POOL, ROWS = 5, 8, 64, 20
+WORDS = {"pages": N_SEQ * COLS, "held": N_SEQ, "held_out": N_SEQ, "free_pages": POOL, "free_state": 4, "free_state_out": 4,
+         "kv_before": N_SEQ, "n_new": N_SEQ, "row_start": N_SEQ + 1, "kv_len": N_SEQ, "missing": N_SEQ, "pos": ROWS,
+         "slots": 2 * ROWS, "row_depth": ROWS}
+READ = {"held", "free_state", "kv_before", "n_new", "row_depth"}
+IN_PLACE = {("held", "held_out"), ("free_state", "free_state_out"), ("kv_before", "kv_len")}
+AT = {name: 0x10000 + 0x1000 * i for i, name in enumerate(WORDS)}  # never read: every call here is refused
+
+
+@pytest.mark.parametrize("a", sorted(WORDS))
+def test_tables(a):
+    """Array `a` over the first and over the last bytes of each other, and at the same place."""
+    for b in sorted(WORDS):
+        if a == b or (a in READ and b in READ):
+            continue
+        step = 8 if "slots" in (a, b) else 4
+        for at in (AT[b], AT[b] + 4 * WORDS[b] - step, AT[b] - 4 * WORDS[a] + step):
+            if at == AT[b] and ((a, b) in IN_PLACE or (b, a) in IN_PLACE):
+                continue
+            at -= at % step
+            x = dict(AT, **{a: at})
+            t = aq.page_tables(N_SEQ, COLS, POOL, 16, *(x[n] for n in ("pages", "held", "free_pages", "free_state", "held_out",
+                                                                       "free_state_out")))
+            refused(aq.AQ_EINVAL, "lies over", aq.paged_tables, FakeCtx(), t, x["kv_before"], x["n_new"], ROWS,
+                    *(x[n] for n in ("row_start", "kv_len", "missing", "pos", "slots", "row_depth")))
