@@ -437,9 +437,11 @@ int aq_paged_tree_commit(aq_ctx *ctx, const aq_paged_kv *kv, uint32_t n_kv, cons
     AQ_REQUIRE(max_path < (1u << 24), "aq_paged_tree_commit: max_path");
     AQ_REQUIRE((uintptr_t)path_dev % 4 == 0 && (uintptr_t)path_len_dev % 4 == 0 && (uintptr_t)kv_len_out % 4 == 0,
                "aq_paged_tree_commit: an array is not aligned to its type");
-    AQ_REQUIRE(!kv_len_out || batch->n_seq == 0 || (kv_len_out != batch->kv_len && kv_len_out != path_len_dev &&
-                                                    kv_len_out != batch->row_start && kv_len_out != path_dev),
-               "aq_paged_tree_commit: kv_len_out lies over an input");
+    const size_t seqs = (size_t)batch->n_seq * 4;
+    const Span read[] = {{batch->kv_len, seqs}, {batch->row_start, seqs + 4}, {batch->pages, seqs * batch->max_pages},
+                         {path_dev, seqs * max_path}, {path_len_dev, seqs}};
+    for (const Span &x : read)
+        AQ_REQUIRE(!x.meets({kv_len_out, seqs}), "aq_paged_tree_commit: kv_len_out lies over an input");
     if (batch->n_seq == 0) return 0;
     a.path = path_dev;
     a.path_len = path_len_dev;

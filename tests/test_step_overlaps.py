@@ -1,9 +1,9 @@
-"""Outputs of the page tables that lie over another array of the call, in whole or in part, are refused, with their codes and
-texts, before anything touches a device (no GPU needed)."""
+"""Outputs of the page tables and of accepted paths that lie over another array of the call, in whole or in part, are
+refused, with their codes and texts, before anything touches a device (no GPU needed)."""
 import pytest
 
 import aqueduct as aq
-from test_paged_refusals import FakeCtx, refused
+from test_paged_refusals import FakeCtx, good_batch, good_kv, refused
 
 N_SEQ, COLS, POOL, ROWS = 5, 8, 64, 20
 WORDS = {"pages": N_SEQ * COLS, "held": N_SEQ, "held_out": N_SEQ, "free_pages": POOL, "free_state": 4, "free_state_out": 4,
@@ -30,3 +30,19 @@ def test_tables(a):
                                                                        "free_state_out")))
             refused(aq.AQ_EINVAL, "lies over", aq.paged_tables, FakeCtx(), t, x["kv_before"], x["n_new"], ROWS,
                     *(x[n] for n in ("row_start", "kv_len", "missing", "pos", "slots", "row_depth")))
+
+
+def test_commit():
+    """The lengths over the first and the last bytes of what the call reads."""
+    n, cols, most = 5, 8, 6
+    words = {"row_start": n + 1, "kv_len": n, "pages": n * cols, "path": n * most, "path_len": n}
+    at = {name: 0x10000 + 0x1000 * i for i, name in enumerate(words)}
+    batch = good_batch(n_seq=n, max_pages=cols, n_rows=20, max_rows=9, **{x: at[x] for x in ("row_start", "kv_len", "pages")})
+    pools = [good_kv(k=0x100000 + 0x20000 * i, v=0x110000 + 0x20000 * i) for i in range(3)]
+
+    def go(text, kvs, out):
+        refused(aq.AQ_EINVAL, text, aq.paged_tree_commit, FakeCtx(), aq.paged_kv_array(kvs), batch, at["path"], at["path_len"], most, out)
+
+    for name, size in words.items():
+        for out in (at[name], at[name] + 4 * size - 4, at[name] - 4 * n + 4):
+            go("lies over", pools, out)
