@@ -349,10 +349,10 @@ int aq_paged_tree_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_b
                             uint32_t window, const aq_heads *gate, void *workspace, size_t workspace_bytes, void *stream);
 /* The accepted path of each sequence's tree kept: of sequence s the new rows path_dev[s * max_path + i], i <
  * path_len_dev[s], which rise (a tree whose nodes stand behind their parents: root first), become its new rows 0, 1, .. :
- * their K and V rows move there, in the pages of all n_kv caches (one a layer: the same shape, strides and type, their own k
- * and v), and kv_len_out[s] (nullable; memory that the call does not read) is the length without the others. The path ends at an entry that
- * is no new row or not past the one before it. A row with no page is neither moved nor written over. Pages that are written
- * belong to one sequence. */
+ * their K and V rows move there, in the pages of all n_kv caches (one a layer: the same shape, strides and type, each its own k
+ * and v: a cache that layers share is given once, twice is refused), and kv_len_out[s] (nullable; memory that the call does not
+ * read) is the length without the others. The path ends at an entry that is no new row or not past the one before it. A row
+ * with no page is neither moved nor written over. Pages that are written belong to one sequence. */
 int aq_paged_tree_commit(aq_ctx *ctx, const aq_paged_kv *kv, uint32_t n_kv, const aq_paged_batch *batch,
                          const int32_t *path_dev, const int32_t *path_len_dev, uint32_t max_path, int32_t *kv_len_out,
                          void *stream);

@@ -15,7 +15,10 @@
 // to move. A work-group has one sequence's K or V rows in one cache: its lanes find 64 entries' places at a time, then each
 // thread moves its 16 bytes of a row for entry after entry, eight on their way. Bound by latency: lengths, path, page entries,
 // rows. Paths of 48 trees of 8 in 16 caches (8 heads of 128, bf16), 24 MB: 6.6 us, of one of 5 (4 heads of 256, f16) 3.3.
+#include <algorithm>
 #include <climits>
+#include <memory>
+#include <new>
 
 #include "paged.h"
 
@@ -442,6 +445,16 @@ int aq_paged_tree_commit(aq_ctx *ctx, const aq_paged_kv *kv, uint32_t n_kv, cons
                          {path_dev, seqs * max_path}, {path_len_dev, seqs}};
     for (const Span &x : read)
         AQ_REQUIRE(!x.meets({kv_len_out, seqs}), "aq_paged_tree_commit: kv_len_out lies over an input");
+    // Rows that two of the call's work-groups move would be moved on by the second.
+    std::unique_ptr<const void *[]> pools(new (std::nothrow) const void *[2 * (size_t)n_kv]);
+    if (!pools) return fail(AQ_ENOMEM, "aq_paged_tree_commit: host allocation");
+    for (uint32_t i = 0; i < n_kv; i++) {
+        pools[2 * (size_t)i] = kv[i].k;
+        pools[2 * (size_t)i + 1] = kv[i].v;
+    }
+    std::sort(&pools[0], &pools[0] + 2 * (size_t)n_kv);
+    AQ_REQUIRE(std::adjacent_find(&pools[0], &pools[0] + 2 * (size_t)n_kv) == &pools[0] + 2 * (size_t)n_kv,
+               "aq_paged_tree_commit: two of the caches' k and v are the same memory");
     if (batch->n_seq == 0) return 0;
     a.path = path_dev;
     a.path_len = path_len_dev;

@@ -1,5 +1,5 @@
-"""Outputs of the page tables and of accepted paths that lie over another array of the call, in whole or in part, are
-refused, with their codes and texts, before anything touches a device (no GPU needed)."""
+"""Outputs of the page tables and of accepted paths that lie over another array of the call, in whole or in part, and caches
+given twice are refused, with their codes and texts, before anything touches a device (no GPU needed)."""
 import pytest
 
 import aqueduct as aq
@@ -33,7 +33,7 @@ def test_tables(a):
 
 
 def test_commit():
-    """The lengths over the first and the last bytes of what the call reads."""
+    """The lengths over the first and the last bytes of what the call reads; one cache given twice, also as another's values."""
     n, cols, most = 5, 8, 6
     words = {"row_start": n + 1, "kv_len": n, "pages": n * cols, "path": n * most, "path_len": n}
     at = {name: 0x10000 + 0x1000 * i for i, name in enumerate(words)}
@@ -46,3 +46,7 @@ def test_commit():
     for name, size in words.items():
         for out in (at[name], at[name] + 4 * size - 4, at[name] - 4 * n + 4):
             go("lies over", pools, out)
+    same = good_kv(k=pools[0].k, v=0x300000)
+    crossed = good_kv(k=0x300000, v=pools[1].k)
+    for kvs in ([pools[0], pools[1], pools[0]], [*pools, same], [*pools, crossed], [good_kv(k=0x300000, v=0x300000)]):
+        go("same memory", kvs, None)
