@@ -224,8 +224,9 @@ int norm_pick(const NormArgs &a, bool inter, uint32_t vec, dim3 grid, hipStream_
 }
 
 // What both calls check of the norm and the rotation.
-int check_norm(const char *call, aq_ctx *ctx, const aq_rope *rope, uint32_t hd, float eps) {
+int check_norm(const char *call, aq_ctx *ctx, const aq_rope *rope, const int32_t *pos, uint32_t hd, float eps) {
     auto who = [&] { return std::string(call); };
+    AQ_REQUIRE((uintptr_t)pos % 4 == 0, who() + ": pos_dev is not aligned to its type");
     AQ_REQUIRE(std::isfinite(eps) && eps > 0.0f, who() + ": eps");
     if (rope) {
         AQ_REQUIRE(rope->ctx->device == ctx->device, who() + ": the rope is on another device");
@@ -297,7 +298,7 @@ int aq_qk_norm_rope(aq_ctx *ctx, const aq_heads *q, const aq_heads *q_out, uint3
                "aq_qk_norm_rope: size");
     if (head_dim == 0 || head_dim > MAX_HEAD)
         return fail(AQ_EUNSUP, "aq_qk_norm_rope: head_dim " + std::to_string(head_dim) + " (1 to 256)");
-    int rc = check_norm(call, ctx, rope, head_dim, eps);
+    int rc = check_norm(call, ctx, rope, pos_dev, head_dim, eps);
     if (!rc && q) rc = check_heads(call, "q", q, n_rows, n_head, head_dim);
     if (!rc && q) rc = check_heads(call, "q_out", q_out, n_rows, n_head, head_dim);
     if (!rc && k) rc = check_heads(call, "k", k, n_rows, n_head_kv, head_dim);
@@ -353,7 +354,7 @@ int aq_paged_append_norm(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batc
     int rc = check_paged(call, kv, batch, &a.kv, &a.b);
     if (rc) return rc;
     const uint32_t hd = kv->head_dim, rows = batch->n_rows;
-    rc = check_norm(call, ctx, rope, hd, eps);
+    rc = check_norm(call, ctx, rope, pos_dev, hd, eps);
     if (!rc) rc = check_heads(call, "k", k, rows, kv->n_head_kv, hd);
     if (!rc) rc = check_heads(call, "v", v, rows, kv->n_head_kv, hd);
     if (!rc) rc = check_weight(call, "k_weight", k_weight);

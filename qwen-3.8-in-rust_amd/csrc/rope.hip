@@ -64,6 +64,8 @@ int check_paged(const char *call, const aq_paged_kv *kv, const aq_paged_batch *b
         return fail(AQ_EUNSUP, who() + ": the pool reaches past 2^32 units of " + std::to_string(1ull << sh) + " bytes");
     AQ_REQUIRE(b->n_rows < (1u << 24) && b->n_seq < (1u << 24), who() + ": batch size (fewer than 2^24 rows)");
     AQ_REQUIRE(b->n_seq == 0 || (b->row_start && b->kv_len && b->pages), who() + ": null batch array");
+    AQ_REQUIRE((uintptr_t)b->row_start % 4 == 0 && (uintptr_t)b->kv_len % 4 == 0 && (uintptr_t)b->pages % 4 == 0,
+               who() + ": a batch array is not aligned to its type");
     AQ_REQUIRE(b->n_seq == 0 || b->max_pages > 0, who() + ": max_pages");
     AQ_REQUIRE((uint64_t)b->max_pages * kv->page_size <= (1ull << 31) - 1024,
                who() + ": the page table reaches past 2^31 positions");
@@ -345,6 +347,7 @@ int aq_rope_apply(const aq_rope *r, const aq_heads *x, const aq_heads *y, size_t
     AQ_REQUIRE(x->data != y->data || (x->row_stride == y->row_stride && x->head_stride == y->head_stride),
                "aq_rope_apply: in place needs the same strides");
     AQ_REQUIRE(pos_dev, "aq_rope_apply: null pos_dev");
+    AQ_REQUIRE((uintptr_t)pos_dev % 4 == 0, "aq_rope_apply: pos_dev is not aligned to its type");
     const uint32_t vec = 16 / (uint32_t)type_bytes(x->type);
     const bool inter = r->layout == AQ_ROPE_INTERLEAVED;
     const bool wide = heads_aligned(x, n_rows, n_heads) && heads_aligned(y, n_rows, n_heads) &&

@@ -1,9 +1,10 @@
-"""Outputs of the page tables and of accepted paths that lie over another array of the call, in whole or in part, and caches
-given twice are refused, with their codes and texts, before anything touches a device (no GPU needed)."""
+"""Outputs of the page tables and of accepted paths that lie over another array of the call, in whole or in part, caches given
+twice, and arrays off their alignment are refused, with their codes and texts, before anything touches a device (no GPU
+needed)."""
 import pytest
 
 import aqueduct as aq
-from test_paged_refusals import FakeCtx, good_batch, good_kv, refused
+from test_paged_refusals import FakeCtx, FakeRope, good_batch, good_kv, refused, rows
 
 N_SEQ, COLS, POOL, ROWS = 5, 8, 64, 20
 WORDS = {"pages": N_SEQ * COLS, "held": N_SEQ, "held_out": N_SEQ, "free_pages": POOL, "free_state": 4, "free_state_out": 4,
@@ -50,3 +51,27 @@ def test_commit():
     crossed = good_kv(k=0x300000, v=pools[1].k)
     for kvs in ([pools[0], pools[1], pools[0]], [*pools, same], [*pools, crossed], [good_kv(k=0x300000, v=0x300000)]):
         go("same memory", kvs, None)
+
+
+def test_arrays_off_their_alignment():
+    """Positions and the batch's arrays, each 2 bytes off, in every call that takes them."""
+    ctx = FakeCtx()
+    rope, x, y, at = FakeRope(ctx, 64), rows(heads=4), rows(heads=4, data=0x40000), 0x10000
+
+    def go(call, **kw):
+        refused(aq.AQ_EINVAL, "is not aligned to its type", call, ctx, **kw)
+
+    go(aq.qk_norm_rope, q=x, q_out=y, n_head=4, k=None, k_out=None, n_head_kv=0, head_dim=64, n_rows=3, q_weight=at, k_weight=None,
+       eps=1e-6, rope=rope, pos=at + 2)
+    go(aq.paged_append_norm, kv=good_kv(), batch=good_batch(), k=rows(), v=rows(), q=None, q_out=None, n_head=0, q_weight=None,
+       k_weight=at, eps=1e-6, rope=rope, pos=at + 2)
+    refused(aq.AQ_EINVAL, "is not aligned to its type", aq.rope_apply, rope, x, y, 3, 4, 64, at + 2)
+    for name in ("row_start", "kv_len", "pages"):
+        b = good_batch(**{name: at + 2})
+        go(aq.paged_append, kv=good_kv(), batch=b, k=rows(), v=rows())
+        go(aq.paged_append_norm, kv=good_kv(), batch=b, k=rows(), v=rows(), q=None, q_out=None, n_head=0, q_weight=None, k_weight=at,
+           eps=1e-6)
+        go(aq.paged_attention, kv=good_kv(), batch=b, n_head=4, q=x, out=y, scale=0.1, workspace=at, workspace_bytes=1 << 30)
+        go(aq.paged_tree_attention, kv=good_kv(), batch=b, mask=at, mask_words=1, n_head=4, q=x, out=y, scale=0.1, workspace=at,
+           workspace_bytes=1 << 30)
+        go(aq.paged_tree_commit, kvs=good_kv(v=0x80000), batch=b, path=at, path_len=at, max_path=4)
