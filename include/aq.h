@@ -322,7 +322,8 @@ int aq_paged_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch 
  * full-attention layers take them (gqa_attention.rs:340-363). y[r][h] = x[r][h] / sqrt(mean(x[r][h]^2) + eps) * weight, in 32
  * bits, then rotated by pos_dev[r] and rounded once; the weights are head_dim f32 on the device, eps > 0. q or k may be null
  * (with its output and weight); rope and pos_dev are null together: the norm alone. Both tensors have one type; each
- * output may be its input (same strides), and else must not overlap what the call reads or writes. head_dim 1 to 256.
+ * output may be its input (same strides), and else must not overlap what the call reads or writes. head_dim 1 to 256, even
+ * where neighbours are turned (AQ_ROPE_INTERLEAVED).
  * Queued on `stream`, capturable, nothing allocated, as all of these calls. */
 int aq_qk_norm_rope(aq_ctx *ctx, const aq_heads *q, const aq_heads *q_out, uint32_t n_head, const aq_heads *k,
                     const aq_heads *k_out, uint32_t n_head_kv, uint32_t head_dim, size_t n_rows, const float *q_weight,
