@@ -1,6 +1,7 @@
 """The calls of a speculative step over pages where their arguments end: heads that leave lanes of a wave without one, trees
-that begin before the row tensors, mask words longer than a tree, rows of any number of pieces to move. Against the
-definitions, in 64 bits; tolerances: tree_plain.norm_bound and paged_plain.bound, by arithmetic; what is copied is equal."""
+that begin before the row tensors, mask words longer than a tree, rows of any number of pieces to move, more work-groups
+than one dimension has. Against the definitions, in 64 bits; tolerances: tree_plain.norm_bound and paged_plain.bound, by
+arithmetic; what is copied is equal."""
 import math
 
 import numpy as np
@@ -215,3 +216,26 @@ def test_tables_of_arrays_side_by_side(ctx, in_place):
     for name, x in want.items():
         x = np.ascontiguousarray(x, np.int64).view(np.int32) if name == "slots" else np.ravel(x)
         assert np.array_equal(got[first[name]: first[name] + sizes[name]], x), name
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+def test_more_work_groups_than_one_dimension_has(ctx, t):
+    """More than 2^22 waves: a grid of two dimensions, whose last work-groups have no row. The rows repeat, at a distance that no
+    power of two of rows is a multiple of, so a row taken for another shows."""
+    rows, hd, again = (1 << 22) + 4099, 8, 1009
+    print(f"norm {t} of {rows} rows", flush=True)
+    rng = np.random.default_rng(11)
+    x = rng.standard_normal((again, 1, hd))
+    w = (1 + 0.3 * rng.standard_normal(hd)).astype(np.float32)
+    few = P.Rows(ctx, x, t)
+    stored, which = few.stored().reshape(again, hd), np.arange(rows) % again
+    many, out = P.Dev(ctx, stored[which]), P.Dev(ctx, np.full((rows + 9, hd), 5, stored.dtype))
+    dw = P.Dev(ctx, w)
+    h = [aq.heads(d.buf, P.TYPES[t], hd, hd) for d in (many, out)]
+    aq.qk_norm_rope(ctx, h[0], h[1], 1, None, None, 0, hd, rows, dw.buf, None, EPS)
+    ctx.sync()
+    got = out.get()
+    want = T.normed(few.values(), w.astype(np.float64), EPS)
+    limit = T.norm_bound(few.values(), w.astype(np.float64), EPS, want, t)
+    assert np.all(np.abs(P.values(got[:again], t) - want[:, 0]) <= limit[:, 0])
+    assert np.array_equal(got[:rows], got[:again][which]) and np.all(got[rows:] == 5)
