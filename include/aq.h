@@ -353,7 +353,9 @@ int aq_paged_tree_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_b
  * their K and V rows move there, in the pages of all n_kv caches (one a layer: the same shape, strides and type, each its own k
  * and v: a cache that layers share is given once, twice is refused), and kv_len_out[s] (nullable; memory that the call does not
  * read) is the length without the others. The path ends at an entry that is no new row or not past the one before it. A row
- * with no page is neither moved nor written over. Pages that are written belong to one sequence. */
+ * with no page is neither moved nor written over, but counts as the others do: a caller whose pool can run out ends its paths
+ * before the first row without a page (slots of aq_paged_tables says which), or a later page stands for what was never stored.
+ * Pages that are written belong to one sequence. */
 int aq_paged_tree_commit(aq_ctx *ctx, const aq_paged_kv *kv, uint32_t n_kv, const aq_paged_batch *batch,
                          const int32_t *path_dev, const int32_t *path_len_dev, uint32_t max_path, int32_t *kv_len_out,
                          void *stream);
@@ -380,8 +382,8 @@ typedef struct aq_page_tables {
  * table has -1 for them, and missing[s] (nullable) says how many of the pages it needs it lacks. Of row r < n_rows, pos[r]
  * (nullable) is its position, kv_before[s] + row_depth[r] where row_depth is given (a tree's drafts), and slots[r]
  * (nullable) its place in the pool, page * page_size + slot; without a page, and behind the last sequence's rows, -1 (and
- * position 0 there). kv_len may be kv_before, the other outputs are memory of their own (what lies over another
- * array of the call, in whole or in part, is refused). A page is held once. */
+ * position 0 there). kv_len may be kv_before, the other outputs are memory of their own (what lies over another array of
+ * the call, in whole or in part, is refused). A page is held once. */
 int aq_paged_tables(aq_ctx *ctx, const aq_page_tables *tables, const int32_t *kv_before, const int32_t *n_new,
                     uint32_t n_rows, int32_t *row_start, int32_t *kv_len, int32_t *missing, int32_t *pos, int64_t *slots,
                     const int32_t *row_depth, void *stream);

@@ -1,7 +1,7 @@
 """The calls of a speculative step over pages where their arguments end: heads that leave lanes of a wave without one, trees
 that begin before the row tensors, mask words longer than a tree, rows of any number of pieces to move, more work-groups
-than one dimension has. Against the definitions, in 64 bits; tolerances: tree_plain.norm_bound and paged_plain.bound, by
-arithmetic; what is copied is equal."""
+than one dimension has, a pool that runs out. Against the definitions, in 64 bits; tolerances: tree_plain.norm_bound and
+paged_plain.bound, by arithmetic; what is copied is equal."""
 import math
 
 import numpy as np
@@ -239,3 +239,57 @@ def test_more_work_groups_than_one_dimension_has(ctx, t):
     limit = T.norm_bound(few.values(), w.astype(np.float64), EPS, want, t)
     assert np.all(np.abs(P.values(got[:again], t) - want[:, 0]) <= limit[:, 0])
     assert np.array_equal(got[:rows], got[:again][which]) and np.all(got[rows:] == 5)
+
+
+@pytest.mark.parametrize("cache_t", ["f16", "f32"])
+def test_a_pool_that_runs_out(ctx, cache_t):
+    """Requests that want more pages than there are, step by step: paths end before the first row without a slot, so that every
+    position that counts was stored, and requests that waited go on when another's pages come back."""
+    print(f"short pool {cache_t}", flush=True)
+    rng = np.random.default_rng(6)
+    n, cols, pool, page, kv, hd, most, goal = 4, 8, 13, 4, 1, 16, 6, [20, 24, 14, 17]
+    rows = n * most
+    dev = lambda a: P.Dev(ctx, a)  # noqa: E731
+    pages, held, ring = dev(np.full((n, cols), -1, np.int32)), dev(np.zeros(n, np.int32)), dev(np.arange(pool, dtype=np.int32))
+    state, before, new, start = (dev(x) for x in (np.array([0, pool, 0, 0], np.int32), np.zeros(n, np.int32), np.zeros(n, np.int32),
+                                                  np.zeros(n + 1, np.int32)))
+    length, missing, pos, slots = (dev(np.zeros(k, t)) for k, t in ((n, np.int32), (n, np.int32), (rows, np.int32), (rows, np.int64)))
+    nan = P.store(np.full((pool, page, kv, hd), np.nan), cache_t)
+    k, v = dev(nan), dev(nan)
+    cache = aq.paged_kv(k.buf, v.buf, P.TYPES[cache_t], pool, page, kv, hd)
+    batch = aq.paged_batch(n, start.buf, length.buf, pages.buf, cols, rows, most, cols * page)
+    t = aq.page_tables(n, cols, pool, page, pages.buf, held.buf, ring.buf, state.buf)
+    lens, done, waited, went_on = np.zeros(n, np.int64), np.zeros(n, bool), np.zeros(n, bool), np.zeros(n, bool)
+    for step in range(60):
+        count = np.where(done, -1, np.minimum(rng.integers(2, most + 1, n), cols * page - lens))
+        new.buf.upload(count.astype(np.int32))
+        aq.paged_tables(ctx, t, before.buf, new.buf, rows, start.buf, length.buf, missing.buf, pos.buf, slots.buf)
+        ctx.sync()
+        first, slot, short = start.get(), slots.get(), missing.get()
+        # the tree's row j is accepted for the j-th of some rising choice; the stored value says whose and which position
+        path, m = np.full((n, most), -1, np.int32), np.zeros(n, np.int32)
+        x = np.full((rows, kv, hd), 99.0)
+        for s in range(n):
+            c = max(int(count[s]), 0)
+            take = np.sort(rng.choice(c, rng.integers(1, c + 1), replace=False)) if c else np.zeros(0, int)
+            for i, j in enumerate(take):
+                x[first[s] + j] = s * 64 + lens[s] + i
+            fits = [j for j in take if slot[first[s] + j] >= 0]
+            path[s, : len(fits)], m[s] = fits, len(fits)
+            went_on[s] |= waited[s] and len(fits) > 0
+            waited[s] |= len(fits) < len(take)
+            assert (short[s] > 0) >= (len(fits) < len(take))
+        r, dp, dm = P.Rows(ctx, x, cache_t), dev(path), dev(m)
+        aq.paged_append(ctx, cache, batch, r.heads_struct(), r.heads_struct())
+        aq.paged_tree_commit(ctx, cache, batch, dp.buf, dm.buf, most, before.buf)
+        ctx.sync()
+        lens = np.where(done, 0, lens + m)
+        assert before.get().tolist() == lens.tolist()
+        table, got = pages.get(), [P.values(p.get().reshape(pool, page, kv, hd), cache_t) for p in (k, v)]
+        for s in range(n):
+            for p in range(int(lens[s])):
+                assert all(np.all(g[table[s, p // page], p % page] == s * 64 + p) for g in got), (step, s, p)
+        done |= lens >= goal
+        if done.all():
+            break
+    assert done.all() and went_on.any()
