@@ -138,7 +138,11 @@ __global__ void __launch_bounds__(256, 8) norm_kernel(NormArgs a) {
         cosines[i] = cs * a.gain;
         sines[i] = sn * a.gain;
     }
-    __builtin_amdgcn_wave_barrier(); // written and read by one wave, in order
+    // Written and read by one wave: the hardware keeps its order, the fences make the compiler keep it (no instruction comes
+    // of them).
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 
 #pragma unroll
     for (int h = 0; h < (int)HB; h++) {
