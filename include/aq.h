@@ -337,14 +337,14 @@ int aq_paged_append_norm(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batc
                          const float *q_weight, const float *k_weight, float eps, const aq_rope *rope,
                          const int32_t *pos_dev, void *stream);
 
-/* Attention of trees of drafted tokens: each sequence's new rows are a tree's nodes, in any order. aq_paged_attention, but a
- * row sees all that stands before its sequence's new rows, and of the new rows those that its mask names: bit j of the
- * mask_words 32-bit words at mask_dev + r * mask_words (n_rows rows; mask_words * 32 at least max_rows) is the j-th new row of
- * row r's sequence, its own among them (a row does not see itself unless its bit says so); bits past its
- * sequence's new rows name nothing, whatever they are. With window > 0 a row whose mask names n rows sees of what stands
- * before the new rows the last window - n positions, as the n-th of a run would up to n = window; a longer path sees itself in
- * whole and nothing before it, where a run's row would see its last window positions only. The same
- * workspace (aq_paged_attention_workspace). A row that sees nothing is 0. */
+/* Attention of trees of drafted tokens: each sequence's new rows are a tree's nodes, in any order. aq_paged_attention, with its
+ * types and its rounding of 16-bit rows' probabilities, but a row sees all that stands before its sequence's new rows, and of
+ * the new rows those that its mask names: bit j of the mask_words 32-bit words at mask_dev + r * mask_words (n_rows rows;
+ * mask_words * 32 at least max_rows) is the j-th new row of row r's sequence, its own among them (a row does not see itself
+ * unless its bit says so); bits past its sequence's new rows name nothing, whatever they are. With window > 0 a row whose mask
+ * names n rows sees of what stands before the new rows the last window - n positions, as the n-th of a run would up to
+ * n = window; a longer path sees itself in whole and nothing before it, where a run's row would see its last window positions
+ * only. The same workspace (aq_paged_attention_workspace). A row that sees nothing is 0. */
 int aq_paged_tree_attention(aq_ctx *ctx, const aq_paged_kv *kv, const aq_paged_batch *batch, const uint32_t *mask_dev,
                             uint32_t mask_words, uint32_t n_head, const aq_heads *q, const aq_heads *out, float scale,
                             uint32_t window, const aq_heads *gate, void *workspace, size_t workspace_bytes, void *stream);

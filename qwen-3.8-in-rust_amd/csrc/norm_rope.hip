@@ -9,7 +9,7 @@
 //
 // Bound by their bytes, with about as many cycles of arithmetic: 8191 rows of 40 heads of 128 (bf16) 33.6 us, 5.0 TB/s, what a
 // large copy reaches; with the angles over a work-group behind a barrier 42.2, with work-groups that go on from row to row
-// 46.6 (too few waves); with a branch for every lane that has no unit or no pair 36.0. 6000 rows of 24 query and 4 K/V heads
+// 46.6 (too few waves); with a branch for every lane that has no unit or no pair 36.0. 5342 rows of 24 query and 4 K/V heads
 // of 256 (f32 into f16) appended in 61.9 us, 5.3 TB/s. Single tokens: an empty launch and three latencies.
 #include <cmath>
 
@@ -20,7 +20,7 @@ namespace {
 
 constexpr int MAX_HEAD = 256;
 // Heads of a lane, so that it has 32 bytes to load. One and two heads: 8191 rows of 40 heads of 128 (bf16), 32 bytes of each
-// (half layout) 33.6 and 39.8 us, 16 (neighbours) 38.0 and 35.3; 6000 rows of 32 heads of 256 (f32 into f16), 32 bytes,
+// (half layout) 33.6 and 39.8 us, 16 (neighbours) 38.0 and 35.3; 5342 rows of 32 heads of 256 (f32 into f16), 32 bytes,
 // 61.9 and 66.5.
 constexpr uint32_t heads_per_lane(uint32_t bytes) { return bytes < 32 ? 2 : 1; }
 

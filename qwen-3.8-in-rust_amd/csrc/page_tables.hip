@@ -5,16 +5,17 @@
 // ring of free pages, what it has too many it puts at the ring's end, and each knows its place in the ring from the sums over
 // the sequences before it: the same call gives the same tables. Pages put back are for the next call, so that what is read
 // (the ring's free pages, the tables' held entries) and what is written (the ring behind them, the entries past them) are
-// apart, and every work-group can work all of it out by itself: each scans the sequences, 1024 at a time, then takes every
-// so many of the rows, of the pages taken and of those put back. Only the lengths, the counts and the ring's state may be
-// written over what the others still read: then the last work-group to arrive at a counter writes those. Bound by latency:
-// lengths, scan, search, page entry, store. One row each of 48 requests 6.0 us, 700 requests of 90 rows 10.3, where an empty
-// launch takes 2.4.
+// apart, and every work-group can work all of it out by itself: each scans the sequences, 256 or 1024 at a time, then
+// takes every so many of the rows, of the pages taken and of those put back. Only the lengths, the counts and the ring's state
+// may be written over what the others still read: then the last work-group to arrive at a counter writes those. Bound by
+// latency: lengths, scan, search, page entry, store. One row each of 48 requests 5.3 us, 50,044 rows of 700 requests 10.5, where
+// an empty launch takes 2.4. In place a step that takes pages and one that puts them back, in turn, 6.4 and 18.6 us a call for
+// 5.1 and 8.9 into other arrays: the counter, and 64 work-groups for 97.
 //
 // Commit. A path's rows rise, so its e-th row lies at or past place e, and moved in order none overwrites one that is still
 // to move. A work-group has one sequence's K or V rows in one cache: its lanes find 64 entries' places at a time, then each
 // thread moves its 16 bytes of a row for entry after entry, eight on their way. Bound by latency: lengths, path, page entries,
-// rows. Paths of 48 trees of 8 in 16 caches (8 heads of 128, bf16), 24 MB: 6.6 us, of one of 5 (4 heads of 256, f16) 3.3.
+// rows. Paths of 48 trees of 8 in 16 caches (8 heads of 128, bf16), 24 MB: 6.6 us, of one of 5 (4 heads of 256, f16) 3.6.
 #include <algorithm>
 #include <climits>
 #include <memory>
@@ -407,7 +408,7 @@ int aq_paged_tables(aq_ctx *ctx, const aq_page_tables *t, const int32_t *kv_befo
     a.apart = a.held_out != a.held && a.state_out != a.state && a.kv_len != a.before;
     a.page_size = FastDiv(t->page_size);
     // A row to a thread, or 16 threads to a sequence, whose pages put back are not known here: 700 requests of 90 rows with 49,
-    // 98 and 197 work-groups of 256 17.7, 15.3 and 13.3 us, with 99 of 512 10.3; 300 of one row, some of which ended, with one
+    // 98 and 197 work-groups of 256 17.7, 15.3 and 13.3 us, with 97 of 512 10.5; 300 of one row, some of which ended, with one
     // and 18 of 256 17.7 and 7.9. In place no more than 64: each arrives at the counter, 256 of them 6 us later.
     const uint64_t work = (uint64_t)t->n_seq * 16 > n_rows ? (uint64_t)t->n_seq * 16 : n_rows;
     const bool small = t->n_seq <= 256;

@@ -253,7 +253,7 @@ def test_a_pool_that_runs_out(ctx, cache_t):
     pages, held, ring = dev(np.full((n, cols), -1, np.int32)), dev(np.zeros(n, np.int32)), dev(np.arange(pool, dtype=np.int32))
     state, before, new, start = (dev(x) for x in (np.array([0, pool, 0, 0], np.int32), np.zeros(n, np.int32), np.zeros(n, np.int32),
                                                   np.zeros(n + 1, np.int32)))
-    length, missing, pos, slots = (dev(np.zeros(k, t)) for k, t in ((n, np.int32), (n, np.int32), (rows, np.int32), (rows, np.int64)))
+    length, missing, pos, slots = (dev(np.zeros(*x)) for x in ((n, np.int32), (n, np.int32), (rows, np.int32), (rows, np.int64)))
     nan = P.store(np.full((pool, page, kv, hd), np.nan), cache_t)
     k, v = dev(nan), dev(nan)
     cache = aq.paged_kv(k.buf, v.buf, P.TYPES[cache_t], pool, page, kv, hd)

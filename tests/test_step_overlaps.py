@@ -42,7 +42,8 @@ def test_commit():
     pools = [good_kv(k=0x100000 + 0x20000 * i, v=0x110000 + 0x20000 * i) for i in range(3)]
 
     def go(text, kvs, out):
-        refused(aq.AQ_EINVAL, text, aq.paged_tree_commit, FakeCtx(), aq.paged_kv_array(kvs), batch, at["path"], at["path_len"], most, out)
+        refused(aq.AQ_EINVAL, text, aq.paged_tree_commit, FakeCtx(), aq.paged_kv_array(kvs), batch, at["path"], at["path_len"],
+                most, out)
 
     for name, size in words.items():
         for out in (at[name], at[name] + 4 * size - 4, at[name] - 4 * n + 4):
@@ -69,8 +70,8 @@ def test_arrays_off_their_alignment():
     for name in ("row_start", "kv_len", "pages"):
         b = good_batch(**{name: at + 2})
         go(aq.paged_append, kv=good_kv(), batch=b, k=rows(), v=rows())
-        go(aq.paged_append_norm, kv=good_kv(), batch=b, k=rows(), v=rows(), q=None, q_out=None, n_head=0, q_weight=None, k_weight=at,
-           eps=1e-6)
+        go(aq.paged_append_norm, kv=good_kv(), batch=b, k=rows(), v=rows(), q=None, q_out=None, n_head=0, q_weight=None,
+           k_weight=at, eps=1e-6)
         go(aq.paged_attention, kv=good_kv(), batch=b, n_head=4, q=x, out=y, scale=0.1, workspace=at, workspace_bytes=1 << 30)
         go(aq.paged_tree_attention, kv=good_kv(), batch=b, mask=at, mask_words=1, n_head=4, q=x, out=y, scale=0.1, workspace=at,
            workspace_bytes=1 << 30)
